@@ -81,7 +81,8 @@ def quantised(x, bits):
     """Rows ``x [..., 128]`` -> ``(stored codes uint8, scales bf16 [..., groups])``."""
     groups, most = (1, 127) if bits == 8 else (4, 7)
     x = x.float().reshape(*x.shape[:-1], groups, D // groups)
-    scale = (x.abs().amax(-1) / most).to(torch.bfloat16)
+    top = x.abs().amax(-1)
+    scale = (top / torch.full_like(top, most)).to(torch.bfloat16)     # a quotient, not a product with 1 / most
     s = scale.float().unsqueeze(-1)
     code = torch.where(s > 0, (x / s).round().clamp(-most, most), 0.0).to(torch.int32)
     if bits == 8:

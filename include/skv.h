@@ -430,6 +430,66 @@ int skv_gemv_attended(const void *W, int N, int K, void *y, int B, const float *
  * outweigh the weights it multiplies them with (many sequences of a long row: use a library GEMM there). */
 int skv_gemv_supported(int N, int K, int B, int mode);
 
+/* One layer of a KV cache held in 8 or 4 bits (no counterpart in the reference, whose cache is bf16).
+ * A row is one token of one KV head, d = 128 values.  bits 8: one scale per row, 128 bytes; bits 4: one scale for each
+ * 32 values, 64 bytes, two codes per byte (the lower nibble first), the row's 32 runs of four values in the order
+ * (run % 8, run / 8).  scale = bf16(largest magnitude / M), M = 127 or 7; stored = round(x / scale) within +-M, plus 128
+ * or 8.  A group whose scale would be below the smallest normal number holds zeros; a group with an Inf or NaN has a NaN
+ * scale and reads back as NaN. */
+typedef struct skv_qcache {
+    void *k, *v;          /* [batch, h_kv, capacity, 16 * bits] bytes, 16-byte aligned */
+    void *scale;          /* [batch, h_kv, capacity, 2, groups] bf16: the key's scales, then the value's */
+    int32_t *status;      /* [batch * h_kv] SKV_ST_* bits, or null */
+    int32_t batch, h_kv, capacity;
+    int32_t d;            /* 128 */
+    int32_t bits;         /* 8 or 4 */
+    int32_t reserved;
+} skv_qcache;
+
+/* Quantises rows as they are written: k, v [batch, h_kv, tokens, 128] (dtype; element strides, unit last stride, rows
+ * 16-byte aligned) into rows [first, first + tokens) of the first `batch` sequences; first = pos[0], or pos[sequence]
+ * with pos_per_seq, in device memory, or pos0 where pos is null.  Rows that fall outside the cache by a device position
+ * are left out and recorded (SKV_ST_BAD_INDEX); a pos0 outside is SKV_E_RANGE. */
+int skv_quant_write(const skv_qcache *c, const void *k, const void *v, int dtype, int batch, int tokens,
+                    int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride, int64_t v_batch_stride,
+                    int64_t v_head_stride, int64_t v_row_stride, const int64_t *pos, int pos_per_seq, int64_t pos0,
+                    void *stream);
+/* The way back: value = code * scale, rounded once to dtype.  Rows outside the cache come back as zeros, recorded. */
+int skv_quant_read(const skv_qcache *c, void *k, void *v, int dtype, int batch, int tokens, int64_t k_batch_stride,
+                   int64_t k_head_stride, int64_t k_row_stride, int64_t v_batch_stride, int64_t v_head_stride,
+                   int64_t v_row_stride, const int64_t *pos, int pos_per_seq, int64_t pos0, void *stream);
+/* skv_qk_rope_cache with a quantised cache: the same queries, and the key and value rows that skv_quant_write would store
+ * of that call's cache rows.  qkv [batch, (H + 2 h_kv) * 128] bf16; the tables need `capacity` rows.  A position outside
+ * the cache is recorded and its sequence left out. */
+int skv_qk_rope_quant(const skv_qcache *c, const void *qkv, const void *q_norm_w, const void *k_norm_w,
+                      const void *cos_table, const void *sin_table, const int64_t *pos, int pos_per_seq, void *q_out,
+                      int batch, int H, float eps, void *stream);
+/* Softmax attention of one query per query head over the quantised rows [0, n): skv_attend's dense mode
+ * (ssa/kernels/graph_kernels.py:27-59) for a quantised cache.  q, out [batch * h_kv * G, 128] dtype, G <= 8; n_dev and
+ * n_group as everywhere (a length beyond the capacity counts as the capacity); workspace of
+ * skv_attend_workspace_bytes(batch * h_kv, G, 128, splits), zero-initialised once; a head without rows gets zeros. */
+int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, int G, const int32_t *n_dev, int n_group, void *out,
+                     void *workspace, int splits, float scale, void *stream);
+
+/* Attention of a batch whose sequences share a prefix: query row of (sequence b, KV head h) attends over the prefix's
+ * rows [0, prefix) of head h, which exist once, and over its own rows [0, n) of cache head b * h_kv + h.  The reference
+ * keeps and reads the prompt's rows once per sequence (ssa/models/graph_decode.py:29-157).
+ *   q, out             [batch * h_kv * G, 128] dtype, G <= 8
+ *   k_prefix, v_prefix [h_kv, prefix, 128]; may be null when prefix == 0
+ *   k, v               [batch * h_kv, rows_limit, 128]; element strides, unit last stride, rows 16-byte aligned
+ *   n_dev, n_group     own lengths as everywhere; one beyond rows_limit counts as rows_limit and is recorded in `status`
+ *                      ([batch * h_kv], may be null)
+ *   splits             skv_prefix_splits(batch, h_kv, G, dtype); workspace of skv_prefix_workspace_bytes bytes,
+ *                      zero-initialised once
+ * A row without any key gets zeros. */
+int skv_prefix_splits(int batch, int h_kv, int G, int dtype);
+int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d, int splits);
+int skv_attend_prefix(const void *q, const void *k_prefix, const void *v_prefix, int prefix, const void *k, const void *v,
+                      const int32_t *n_dev, int n_group, void *out, void *workspace, int32_t *status, int batch, int h_kv,
+                      int G, int d, int dtype, int64_t kp_head_stride, int64_t kp_row_stride, int64_t vp_head_stride,
+                      int64_t vp_row_stride, int64_t k_head_stride, int64_t k_row_stride, int64_t v_head_stride,
+                      int64_t v_row_stride, int rows_limit, int splits, float scale, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,7 +21,9 @@ EXPORTS = ("skv_version", "skv_error_string", "skv_last_cuda_error", "skv_attend
            "skv_attend_workspace_bytes", "skv_attend", "skv_attend_static", "skv_attend_weighted", "skv_attend_labels", "skv_step", "skv_step_clusters", "skv_step_workspace_bytes", "skv_debug_step_probe", "skv_merge", "skv_select_workspace_bytes", "skv_select", "skv_debug_select_probe", "skv_debug_attend_probe", "skv_set_overlap", "skv_insert",
            "skv_insert_max_members", "skv_fit_tensor_cores", "skv_fit_workspace_bytes", "skv_fit", "skv_rebin",
            "skv_add_rmsnorm", "skv_qk_rope_cache", "skv_silu_mul", "skv_gemv", "skv_gemv_attended", "skv_gemv_supported", "skv_gemv_tp", "skv_comm_bytes", "skv_comm_alloc",
-           "skv_comm_export", "skv_comm_open", "skv_comm_close", "skv_comm_free", "skv_comm_view", "skv_comm_tick", "skv_comm_push", "skv_comm_reduce", "skv_comm_status")
+           "skv_comm_export", "skv_comm_open", "skv_comm_close", "skv_comm_free", "skv_comm_view", "skv_comm_tick", "skv_comm_push", "skv_comm_reduce", "skv_comm_status",
+           "skv_quant_write", "skv_quant_read", "skv_qk_rope_quant", "skv_attend_quant", "skv_prefix_splits",
+           "skv_prefix_workspace_bytes", "skv_attend_prefix")
 
 
 class SkvError(RuntimeError):
@@ -41,6 +43,13 @@ class SkvRope(C.Structure):
                 ("v_cache", C.c_void_p), ("H", C.c_int32), ("H_kv", C.c_int32), ("cache_batch_stride", C.c_int64),
                 ("cache_head_stride", C.c_int64), ("cache_row_stride", C.c_int64), ("eps", C.c_float),
                 ("pos_per_seq", C.c_int32)]
+
+
+class SkvQCache(C.Structure):
+    """``skv_qcache`` of include/skv.h: one layer of a quantised KV cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("scale", C.c_void_p), ("status", C.c_void_p),
+                ("batch", C.c_int32), ("h_kv", C.c_int32), ("capacity", C.c_int32), ("d", C.c_int32),
+                ("bits", C.c_int32), ("reserved", C.c_int32)]
 
 
 class SkvState(C.Structure):
@@ -148,6 +157,22 @@ def _declare(lib) -> None:
     lib.skv_gemv_supported.argtypes = [i32, i32, i32, i32]
     lib.skv_gemv.restype = i32
     lib.skv_gemv.argtypes = [vp, i32, i32, vp, i32, i32, vp, vp, vp, vp, vp, f32, vp]
+    qc = C.POINTER(SkvQCache)
+    lib.skv_quant_write.restype = i32
+    lib.skv_quant_write.argtypes = [qc, vp, vp, i32, i32, i32, i64, i64, i64, i64, i64, i64, vp, i32, i64, vp]
+    lib.skv_quant_read.restype = i32
+    lib.skv_quant_read.argtypes = lib.skv_quant_write.argtypes
+    lib.skv_qk_rope_quant.restype = i32
+    lib.skv_qk_rope_quant.argtypes = [qc, vp, vp, vp, vp, vp, vp, i32, vp, i32, i32, f32, vp]
+    lib.skv_attend_quant.restype = i32
+    lib.skv_attend_quant.argtypes = [qc, vp, i32, i32, vp, i32, vp, vp, i32, f32, vp]
+    lib.skv_prefix_splits.restype = i32
+    lib.skv_prefix_splits.argtypes = [i32, i32, i32, i32]
+    lib.skv_prefix_workspace_bytes.restype = i64
+    lib.skv_prefix_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
+    lib.skv_attend_prefix.restype = i32
+    lib.skv_attend_prefix.argtypes = [vp, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64,
+                                      i64, i64, i64, i64, i64, i32, i32, f32, vp]
     lib.skv_rebin.restype = i32
     lib.skv_rebin.argtypes = [C.POINTER(SkvState), vp, i32, i32, vp, i32, i64, i64, f32, i32, f32, vp, i64, vp]
 
@@ -168,7 +193,8 @@ def lib():
 # entry points that launch exactly one kernel each: counted, so that a caller can tell how many of the library's
 # kernels a captured decode step holds (GraphDecoder.launches_per_step)
 _ONE_LAUNCH = {"skv_insert", "skv_select", "skv_attend", "skv_attend_weighted", "skv_attend_labels", "skv_step", "skv_gemv", "skv_gemv_tp", "skv_gemv_attended",
-               "skv_add_rmsnorm", "skv_qk_rope_cache", "skv_silu_mul", "skv_comm_push", "skv_comm_reduce", "skv_comm_tick"}
+               "skv_add_rmsnorm", "skv_qk_rope_cache", "skv_silu_mul", "skv_comm_push", "skv_comm_reduce", "skv_comm_tick",
+               "skv_quant_write", "skv_quant_read", "skv_qk_rope_quant", "skv_attend_quant", "skv_attend_prefix"}
 launches = 0
 
 
@@ -194,6 +220,25 @@ def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.float32:
         return SKV_F32
     raise ValueError(f"unsupported cache dtype {dt}; the kernels take bfloat16 or float32")
+
+
+class _Nothing:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def on_device(device):
+    """Context in which ``device`` is the current CUDA device: a launch goes to the current device, a caller's tensors
+    may live on another."""
+    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
+        return _NOTHING
+    return torch.cuda.device(device)
 
 
 def stream_ptr(device=None) -> int:

@@ -5,7 +5,8 @@ keywords, ``prepare(n)``, ``capture()``, ``step(token, pos)``, the attributes ``
 ``H, H_kv, d, B`` and ``_heads(cache)``.  The position lives in device memory, so a step is a single
 graph launch; the batch is folded into the KV heads (``B`` sequences x ``H_kv`` heads are ``B*H_kv``
 independent heads for every attention kernel).  Modes: ``"cluster"`` (aliases ``"sphere"``,
-``"voronoi"``) and ``"dense"`` (exact attention by the same gather kernel in its dense mode).
+``"voronoi"``) and ``"dense"`` (exact attention by the same gather kernel in its dense mode, or, by the type of the
+cache, over quantised rows (``QuantKVCache``) or over a prefix the batch shares (``PrefixKVCache``)).
 """
 
 from __future__ import annotations
@@ -22,6 +23,8 @@ import torch.nn.functional as F
 from . import _lib
 from ._lib import check, dtype_code, lib, stream_ptr
 from .cluster_state import AttentionPartials, ClusterArena, SphereIndexGraph, fit_layers, fit_layers_ragged
+from .prefix_cache import PrefixAttentionGraph, PrefixKVCache
+from .quant_cache import QuantAttentionGraph, QuantKVCache
 from .qwen3 import Qwen3Model, apply_rope
 
 
@@ -94,7 +97,10 @@ class GraphDecoder:
         mode = "cluster" if mode in ("sphere", "voronoi") else mode
         if mode not in ("dense", "cluster"):
             raise ValueError(f"unknown mode {mode!r}")
+        if mode != "dense" and isinstance(cache, (QuantKVCache, PrefixKVCache)):
+            raise ValueError("clustered attention reads a plain cache: decode this one with mode='dense'")
         self.model, self.cache, self.mode = model, cache, mode
+        self.first = 0                                     # position of the cache's first row (a shared prefix: its length)
         self.H, self.H_kv, self.d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         self.B = B = cache.k[0].shape[0]
         p = next(model.parameters())
@@ -104,7 +110,13 @@ class GraphDecoder:
         self.n_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         cap = cache.max_seq_len
         nl = len(model.layers)
-        if mode == "dense":
+        if isinstance(cache, QuantKVCache):
+            one = QuantAttentionGraph(H=B * self.H, H_kv=B * self.H_kv, d=self.d, dtype=dtype, device=dev)
+            self.attn = [one] * nl                         # the layers run one after another: one workspace serves all
+        elif isinstance(cache, PrefixKVCache):
+            one = PrefixAttentionGraph(B=B, H=self.H, H_kv=self.H_kv, d=self.d, dtype=dtype, device=dev)
+            self.attn = [one] * nl
+        elif mode == "dense":
             self.attn = [DenseAttentionGraph(H=B * self.H, H_kv=B * self.H_kv, d=self.d, dtype=dtype, device=dev)
                          for _ in range(nl)]
         else:
@@ -174,7 +186,8 @@ class GraphDecoder:
         """Build the attention state from the first ``n`` cached positions (after the prompt).  ``n`` may be a
         list with one length per sequence: the batch then decodes sequences of different lengths (each head reads
         its own sequence's length and position from device memory), which lifts the reference's equal-length limit
-        (README.md:62); ``step`` then takes one position per sequence."""
+        (README.md:62); ``step`` then takes one position per sequence.  Lengths and positions count a shared prefix."""
+        self.first = getattr(self.cache, "first", 0)
         if not isinstance(n, int):
             return self._prepare_ragged([int(x) for x in n])
         if self.mode != "cluster":
@@ -224,6 +237,9 @@ class GraphDecoder:
             raise ValueError("a variable-length batch needs the bundled bf16 model's fused layers")
         dev = self.tok.device
         self.ragged = True
+        lengths = [n - self.first for n in lengths]        # own rows
+        if min(lengths) < 0:
+            raise ValueError(f"the sequences begin behind the prefix's {self.first} rows")
         self.pos = torch.tensor(lengths, dtype=torch.long, device=dev)
         self.n_dev = torch.tensor(lengths, dtype=torch.int32, device=dev)
         self.n_next = torch.zeros_like(self.n_dev)
@@ -254,6 +270,7 @@ class GraphDecoder:
         """Restore what ``state_dict`` saved, in place of ``prepare``: no fit runs.  The cache this decoder was
         built on must already hold the ``sd["n"]`` positions the state describes; call ``capture`` afterwards."""
         n = int(sd["n"])
+        self.first = getattr(self.cache, "first", 0)
         self.cache.cur_len = n
         if self.mode != "cluster":
             return
@@ -278,8 +295,8 @@ class GraphDecoder:
         if self.insert_all is not None and not self.insert_ahead:
             self.insert_all(self.n_dev)
         h = m.embed(self.tok)
-        cos = m.rope_cos.index_select(0, self.pos)
-        sin = m.rope_sin.index_select(0, self.pos)
+        cos = m.rope_cos[self.first:].index_select(0, self.pos)
+        sin = m.rope_sin[self.first:].index_select(0, self.pos)
         for i, layer in enumerate(m.layers):
             a = layer.attn
             x = layer.norm1(h)
@@ -288,17 +305,47 @@ class GraphDecoder:
             v = a.v(x).view(B, 1, H_kv, d).transpose(1, 2)
             q, k = apply_rope(q, k, cos, sin)
             kc, vc = self.cache.k[i], self.cache.v[i]
-            kc.index_copy_(2, self.pos, k)
-            vc.index_copy_(2, self.pos, v)
+            if isinstance(self.cache, QuantKVCache):
+                self.cache.write(i, k, v, self.pos)
+            else:
+                kc.index_copy_(2, self.pos, k)
+                vc.index_copy_(2, self.pos, v)
             qh = q.reshape(B * H, d)
             if self.mode == "dense":
-                out = self.attn[i](qh, self._heads(kc), self._heads(vc), self.n_dev)
+                out = self._dense(i, qh)
             else:
                 out = self.attn[i].step(qh, self._heads(kc), self._heads(vc), self.n_dev,
                                         insert=self.insert_all is None)
             h = h + a.tp.all_reduce(a.o(out.view(B, 1, H * d)))
             h = h + layer.ffn(layer.norm2(h))
         return self._finish(m.final_norm(h))
+
+    def _dense(self, i: int, qh: torch.Tensor) -> torch.Tensor:
+        """Layer ``i``'s exact attention of the rotated queries, whichever cache holds the rows."""
+        cache = self.cache
+        if isinstance(cache, QuantKVCache):
+            return self.attn[i](qh, cache, i, self.n_dev)
+        kh, vh = self._heads(cache.k[i]), self._heads(cache.v[i])
+        if isinstance(cache, PrefixKVCache):
+            return self.attn[i](qh, *cache.prefix_rows(i), kh, vh, self.n_dev)
+        return self.attn[i](qh, kh, vh, self.n_dev)
+
+    def _rope(self, i: int, qkv: torch.Tensor, qh: torch.Tensor, st: int) -> None:
+        """QK-norm + rotary + cache write of the new token, one launch.  ``pos`` counts the cache's own rows; the
+        tables are taken from the position of the first."""
+        m, a = self.model, self.model.layers[i].attn
+        cos, sin = m.rope_cos[self.first:], m.rope_sin[self.first:]
+        if isinstance(self.cache, QuantKVCache):
+            check(lib().skv_qk_rope_quant(self.cache._st[i], qkv.data_ptr(), a.q_norm.weight.data_ptr(),
+                                          a.k_norm.weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), self.pos.data_ptr(),
+                                          int(self.ragged), qh.data_ptr(), self.B, self.H, a.q_norm.eps, st),
+                  "skv_qk_rope_quant")
+            return
+        kc, vc = self.cache.k[i], self.cache.v[i]
+        check(lib().skv_qk_rope_cache(qkv.data_ptr(), a.q_norm.weight.data_ptr(), a.k_norm.weight.data_ptr(),
+                                      cos.data_ptr(), sin.data_ptr(), self.pos.data_ptr(), int(self.ragged), qh.data_ptr(),
+                                      kc.data_ptr(), vc.data_ptr(), self.B, self.H, self.H_kv, self.d, kc.stride(0),
+                                      kc.stride(1), kc.stride(2), a.q_norm.eps, st), "skv_qk_rope_cache")
 
     def _fuse_weights(self) -> None:
         """Lay q/k/v and gate/up weights of every layer out as one matrix each (the modules keep working:
@@ -365,12 +412,9 @@ class GraphDecoder:
                                     layer.norm1.weight.data_ptr(), xn.data_ptr(), B, hidden, eps, st), "skv_add_rmsnorm")
             qkv = F.linear(xn, self._wqkv[i])
             kc, vc = self.cache.k[i], self.cache.v[i]
-            check(L.skv_qk_rope_cache(qkv.data_ptr(), a.q_norm.weight.data_ptr(), a.k_norm.weight.data_ptr(),
-                                      m.rope_cos.data_ptr(), m.rope_sin.data_ptr(), self.pos.data_ptr(),
-                                      int(self.ragged), qh.data_ptr(), kc.data_ptr(), vc.data_ptr(), B, H, H_kv, d,
-                                      kc.stride(0), kc.stride(1), kc.stride(2), a.q_norm.eps, st), "skv_qk_rope_cache")
+            self._rope(i, qkv, qh, st)
             if self.mode == "dense":
-                out = self.attn[i](qh, self._heads(kc), self._heads(vc), self.n_dev)
+                out = self._dense(i, qh)
             else:
                 out = self.attn[i].step(qh, self._heads(kc), self._heads(vc), self.n_dev,
                                         insert=self.insert_all is None)
@@ -488,13 +532,9 @@ class GraphDecoder:
                 out = self.attn[i].step(qh, self._heads(kc), self._heads(vc), self.n_dev,
                                         insert=self.insert_all is None, rope=rope, defer_merge=defer)
             else:
-                check(L.skv_qk_rope_cache(qkv.data_ptr(), a.q_norm.weight.data_ptr(), a.k_norm.weight.data_ptr(),
-                                          m.rope_cos.data_ptr(), m.rope_sin.data_ptr(), self.pos.data_ptr(),
-                                          int(self.ragged), qh.data_ptr(), kc.data_ptr(), vc.data_ptr(), B, H, H_kv, d,
-                                          kc.stride(0), kc.stride(1), kc.stride(2), a.q_norm.eps, st),
-                      "skv_qk_rope_cache")
+                self._rope(i, qkv, qh, st)
                 if self.mode == "dense":
-                    out = self.attn[i](qh, self._heads(kc), self._heads(vc), self.n_dev)
+                    out = self._dense(i, qh)
                 else:
                     out = self.attn[i].step(qh, self._heads(kc), self._heads(vc), self.n_dev,
                                             insert=self.insert_all is None, defer_merge=defer)
@@ -525,13 +565,26 @@ class GraphDecoder:
             self._peer = PeerExchange(tp.group, self.B * hidden, self.tok.device)
         return self._peer
 
+    def _check_place(self, pos) -> None:
+        """A quantised or shared-prefix cache: the new tokens' positions, where the host knows them, lie behind the
+        prefix that ``prepare`` saw and within the cache."""
+        if not isinstance(self.cache, (QuantKVCache, PrefixKVCache)) or (torch.is_tensor(pos) and pos.is_cuda):
+            return
+        if self.first != self.cache.first:
+            raise ValueError("the shared prefix has changed since prepare()")
+        at = [int(pos)] if isinstance(pos, int) or (torch.is_tensor(pos) and pos.dim() == 0) else [int(x) for x in pos]
+        if min(at) < self.first or max(at) >= self.cache.max_seq_len:
+            raise ValueError(f"position {min(at) if min(at) < self.first else max(at)} lies outside the cache's "
+                             f"[{self.first}, {self.cache.max_seq_len})")
+
     def capture(self) -> None:
         """Record one decode step.  Call after ``prepare`` and before the first ``step``; the warm-up
         runs write a placeholder at the current position, which the first real step overwrites."""
+        self._check_place(self.cache.cur_len)
         if self.ragged:
-            self.pos.copy_(torch.tensor(self.cache.cur_len, dtype=torch.long))
+            self.pos.copy_(torch.tensor(self.cache.cur_len, dtype=torch.long) - self.first)
         else:
-            self.pos.fill_(self.cache.cur_len)
+            self.pos.fill_(self.cache.cur_len - self.first)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         self._warming = True                           # (the next step's insert must not run in the warm-up steps)
@@ -556,13 +609,14 @@ class GraphDecoder:
         """Decode ``token [B, 1]`` at position ``pos`` (one position per sequence, a list or tensor ``[B]``, for a
         batch prepared with one length per sequence); returns logits ``[B, 1, vocab]`` (a buffer the next step
         overwrites)."""
+        self._check_place(pos)
         self.tok.copy_(token, non_blocking=True)           # a pinned host tensor goes straight into the step's buffer
         if self.ragged:
             if not torch.is_tensor(pos):
                 pos = torch.tensor([int(x) for x in pos], dtype=torch.long)
-            self.pos.copy_(pos, non_blocking=True)
+            self.pos.copy_(pos - self.first if self.first else pos, non_blocking=True)
         else:
-            self.pos.fill_(pos)
+            self.pos.fill_(pos - self.first)
         if self.graph is not None:
             self.graph.replay()
         else:

@@ -1,0 +1,185 @@
+"""KV cache held in 8 or 4 bits: rows are quantised as they are written, read back for a prefill chunk, and attended over
+in their quantised form by a decode step.
+
+A row (one token of one KV head, 128 values) has one bf16 scale in 8 bits and one for each 32 values in 4 bits, so a cached
+token takes 260 or 144 bytes per KV head where bf16 takes 512.  ``value = (stored - 128) * scale`` or
+``(stored - 8) * scale``, within half a scale of what was written.  In 4 bits a row's 32 runs of four values are stored in
+the order ``(run % 8, run // 8)``, the lower nibble of a byte first.  Values have no gradient: this is a serving cache.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ._lib import SkvQCache, SkvError, check, dtype_code, lib, on_device, stream_ptr
+
+__all__ = ["QuantKVCache", "QuantAttentionGraph"]
+
+
+class QuantKVCache:
+    """Quantised cache of all layers, in place of ``KVCache``: ``k[i], v[i] [B, H_kv, L, 128 * bits / 8]`` uint8 and
+    ``scale[i] [B, H_kv, L, 2, groups]`` bf16 (the key's scales, then the value's)."""
+
+    plain = False
+    first = 0                                              # position of the first row
+
+    def __init__(self, layers: int, batch: int, h_kv: int, max_seq_len: int, d: int, bits: int, device):
+        if bits not in (8, 4):
+            raise ValueError("a quantised cache holds 8 or 4 bits per value")
+        if d != 128:
+            raise ValueError("the kernels are built for head_dim 128")
+        groups, width = (1 if bits == 8 else 4), d * bits // 8
+        # a code of 0 with a scale of 0: rows that were never written read as zeros
+        self._set([torch.zeros(batch, h_kv, max_seq_len, width, dtype=torch.uint8, device=device) for _ in range(layers)],
+                  [torch.zeros(batch, h_kv, max_seq_len, width, dtype=torch.uint8, device=device) for _ in range(layers)],
+                  [torch.zeros(batch, h_kv, max_seq_len, 2, groups, dtype=torch.bfloat16, device=device)
+                   for _ in range(layers)], bits, None)
+
+    @classmethod
+    def from_tensors(cls, k: list, v: list, scale: list, bits: int, status: torch.Tensor | None = None) -> "QuantKVCache":
+        """A cache over tensors that the caller holds (per layer, contiguous, in the layout above)."""
+        if bits not in (8, 4):
+            raise ValueError("a quantised cache holds 8 or 4 bits per value")
+        if not (len(k) == len(v) == len(scale) >= 1):
+            raise ValueError("one tensor of codes of the keys, of the values and of scales is needed per layer")
+        B, H, L, w = k[0].shape
+        want = {"codes": ((B, H, L, 16 * bits), torch.uint8), "scales": ((B, H, L, 2, 1 if bits == 8 else 4), torch.bfloat16)}
+        for name, ts in (("codes", k), ("codes", v), ("scales", scale)):
+            for t in ts:
+                if tuple(t.shape) != want[name][0] or t.dtype != want[name][1] or not t.is_contiguous() \
+                        or t.device != k[0].device:
+                    raise ValueError(f"{name} must be contiguous {want[name][0]} {want[name][1]} on one device")
+        self = cls.__new__(cls)
+        self._set(list(k), list(v), list(scale), bits, status)
+        return self
+
+    def _set(self, k, v, scale, bits, status) -> None:
+        self.k, self.v, self.scale, self.bits = k, v, scale, bits
+        self.batch, self.h_kv, self.max_seq_len, _ = k[0].shape
+        self.d, self.device = 128, k[0].device
+        self.cur_len = 0
+        self.status = torch.zeros(self.batch * self.h_kv, dtype=torch.int32, device=self.device) if status is None else status
+        self._st = [SkvQCache(a.data_ptr(), b.data_ptr(), s.data_ptr(), self.status.data_ptr(), self.batch, self.h_kv,
+                              self.max_seq_len, self.d, bits, 0) for a, b, s in zip(k, v, scale)]
+
+    def sequence(self, b: int) -> "QuantKVCache":
+        """Sequence ``b`` alone, on the same memory."""
+        h = self.h_kv
+        return self.from_tensors([t[b:b + 1] for t in self.k], [t[b:b + 1] for t in self.v],
+                                 [t[b:b + 1] for t in self.scale], self.bits, self.status[b * h:(b + 1) * h])
+
+    def check_status(self) -> int:
+        """Bits of ``SKV_ST_*`` over all heads (a position outside the cache was skipped); synchronises."""
+        bits = 0
+        for s in set(self.status.tolist()):
+            bits |= s
+        return bits
+
+    def _where(self, pos, b: int):
+        """``pos`` as (device address or None, one per sequence, host value)."""
+        if not torch.is_tensor(pos):
+            return None, 0, int(pos)
+        if pos.dtype != torch.long or pos.device != self.device or pos.dim() != 1 or not pos.is_contiguous() \
+                or pos.shape[0] not in (1, b):
+            raise ValueError("positions are an int, or int64 [1] or [sequences] on the cache's device")
+        return pos.data_ptr(), int(pos.shape[0] != 1), 0
+
+    @staticmethod
+    def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
+        per16 = 16 // t.element_size()
+        s0, s1, s2, s3 = t.stride()
+        if s3 != 1 or s0 % per16 or s1 % per16 or s2 % per16 or t.data_ptr() % 16:
+            return t.contiguous()
+        return t
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, pos) -> None:
+        """Quantise ``k, v [b, H_kv, T, 128]`` (bf16 or float32, any strides) into the rows ``[pos, pos + T)`` of the
+        first ``b`` sequences.  ``pos``: an int, or int64 in device memory, one for all or one per sequence; rows of a
+        device position that fall outside the cache are left out and recorded in ``status``."""
+        if k.dim() != 4 or k.shape != v.shape or k.shape[1] != self.h_kv or k.shape[3] != self.d or k.shape[0] > self.batch:
+            raise ValueError(f"keys and values must be [sequences <= {self.batch}, {self.h_kv}, tokens, {self.d}]")
+        if k.dtype != v.dtype or k.device != self.device or v.device != self.device:
+            raise ValueError("keys and values must be of one type, on the cache's device")
+        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+            raise ValueError("a quantised cache has no gradient: write under torch.no_grad()")
+        code = dtype_code(k.dtype)
+        b, T = k.shape[0], k.shape[2]
+        at, per_seq, host = self._where(pos, b)
+        if at is None and not 0 <= host <= self.max_seq_len - T:
+            raise ValueError(f"rows [{host}, {host + T}) lie outside the cache's {self.max_seq_len} positions")
+        if T > self.max_seq_len:
+            raise ValueError(f"{T} rows do not fit the cache's {self.max_seq_len} positions")
+        if b == 0 or T == 0:
+            return
+        k, v = self._rows("k", k), self._rows("v", v)
+        with on_device(self.device):
+            check(lib().skv_quant_write(self._st[layer], k.data_ptr(), v.data_ptr(), code, b, T, *k.stride()[:3],
+                                        *v.stride()[:3], at, per_seq, host, stream_ptr(self.device)), "skv_quant_write")
+
+    def read(self, layer: int, pos, count: int, *, dtype: torch.dtype = torch.bfloat16,
+             batch: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The rows ``[pos, pos + count)`` of the first ``batch`` (all) sequences as ``k, v [b, H_kv, count, 128]`` of
+        ``dtype``; ``pos`` as in ``write`` (rows outside the cache come back as zeros and are recorded)."""
+        b = self.batch if batch is None else batch
+        if not 0 <= b <= self.batch:
+            raise ValueError(f"the cache holds {self.batch} sequences")
+        at, per_seq, host = self._where(pos, b)
+        if not 0 <= count <= self.max_seq_len or (at is None and not 0 <= host <= self.max_seq_len - count):
+            raise ValueError(f"rows [{host}, {host + count}) lie outside the cache's {self.max_seq_len} positions")
+        code = dtype_code(dtype)
+        out = torch.empty(2, b, self.h_kv, count, self.d, dtype=dtype, device=self.device)
+        k, v = out[0], out[1]
+        if b and count:
+            hs = count * self.d
+            bs = self.h_kv * hs
+            with on_device(self.device):
+                check(lib().skv_quant_read(self._st[layer], k.data_ptr(), v.data_ptr(), code, b, count, bs, hs, self.d, bs,
+                                           hs, self.d, at, per_seq, host, stream_ptr(self.device)), "skv_quant_read")
+        return k, v
+
+    def rows(self, layer: int, b: int, n: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows ``[0, n)`` of the first ``b`` sequences, for a prefill chunk's attention."""
+        return self.read(layer, 0, n, dtype=dtype, batch=b)
+
+
+class QuantAttentionGraph:
+    """Exact decode attention over the quantised rows ``[0, n)``, with ``n`` in device memory: ``DenseAttentionGraph``
+    for a ``QuantKVCache``.  The object owns the workspace and the output buffer, which the next call overwrites: calls
+    of one object (and graphs captured from it) must not overlap on the GPU."""
+
+    def __init__(self, *, H: int, H_kv: int, d: int, dtype, device):
+        if H % H_kv:
+            raise ValueError("the query heads must divide into the KV heads")
+        L = lib()
+        self.H, self.H_kv, self.d, self.G = H, H_kv, d, H // H_kv
+        self.n_group = 0                                   # heads per entry of the device-side lengths (0: one length)
+        self.dtype, self.device = dtype, torch.device(device)
+        self._code = dtype_code(dtype)
+        with on_device(self.device):
+            self.num_splits = L.skv_attend_splits(H_kv)
+            size = L.skv_attend_workspace_bytes(H_kv, self.G, d, self.num_splits)
+            if size < 0:
+                raise SkvError(L.skv_error_string(int(size)).decode())
+            self.ws = torch.zeros(size, dtype=torch.uint8, device=device)
+            self.out = torch.empty(H, d, dtype=dtype, device=device)
+        self._scale = 1.0 / math.sqrt(d)
+
+    def __call__(self, q: torch.Tensor, cache: QuantKVCache, layer: int, n_dev: torch.Tensor) -> torch.Tensor:
+        """``q [H, d]`` (all sequences' query heads), ``n_dev`` int32 on the device: one length, or one per ``n_group``
+        heads.  A head without rows gets zeros."""
+        if q.shape != self.out.shape or q.dtype != self.dtype:
+            raise ValueError(f"queries must be {tuple(self.out.shape)} {self.dtype}")
+        if cache.batch * cache.h_kv != self.H_kv or cache.device != q.device or q.device != self.out.device:
+            raise ValueError(f"the cache must hold {self.H_kv} KV heads, on the queries' device")
+        if n_dev.dtype != torch.int32 or n_dev.device != q.device \
+                or n_dev.numel() < (-(-self.H_kv // self.n_group) if self.n_group else 1):
+            raise ValueError("lengths must be int32 on the queries' device: one, or one per n_group heads")
+        if not q.is_contiguous() or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+        with on_device(q.device):
+            check(lib().skv_attend_quant(cache._st[layer], q.data_ptr(), self._code, self.G, n_dev.data_ptr(),
+                                         self.n_group, self.out.data_ptr(), self.ws.data_ptr(), self.num_splits,
+                                         self._scale, stream_ptr(q.device)), "skv_attend_quant")
+        return self.out

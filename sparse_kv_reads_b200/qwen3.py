@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from functools import partial
 
 import torch
 import torch.distributed as dist
@@ -72,11 +73,36 @@ def apply_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.T
 class KVCache:
     """Contiguous cache: ``k[i], v[i] [B, H_kv, L, d]`` per layer."""
 
+    plain = True                                           # rows lie in k[i], v[i] as they were written
+    first = 0                                              # position of the first row
+
     def __init__(self, layers: int, batch: int, h_kv: int, max_seq_len: int, d: int, dtype, device):
         self.k = [torch.zeros(batch, h_kv, max_seq_len, d, dtype=dtype, device=device) for _ in range(layers)]
         self.v = [torch.zeros(batch, h_kv, max_seq_len, d, dtype=dtype, device=device) for _ in range(layers)]
         self.cur_len = 0
         self.max_seq_len = max_seq_len
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, start: int) -> None:
+        """``k, v [b, H_kv, T, d]`` into the rows ``[start, start + T)`` of the first ``b`` sequences."""
+        b, T = k.shape[0], k.shape[2]
+        self.k[layer][:b, :, start:start + T] = k
+        self.v[layer][:b, :, start:start + T] = v
+
+    def rows(self, layer: int, b: int, n: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows ``[0, n)`` of the first ``b`` sequences (views; they have the cache's own type)."""
+        return self.k[layer][:b, :, :n], self.v[layer][:b, :, :n]
+
+    def sequence(self, b: int) -> "KVCache":
+        """Sequence ``b`` alone, on the same memory."""
+        view = KVCache.__new__(KVCache)
+        view.k, view.v = [k[b:b + 1] for k in self.k], [v[b:b + 1] for v in self.v]
+        view.cur_len, view.max_seq_len = 0, self.max_seq_len
+        return view
+
+
+def _cache_op(cache, name: str):
+    """A cache's own operation, or ``KVCache``'s on any object with its attributes."""
+    return getattr(cache, name, None) or partial(getattr(KVCache, name), cache)
 
 
 class _TP:
@@ -102,24 +128,28 @@ class Attention(nn.Module):
         self.decode_attn_op = None            # set by patch.install: op(q, full_k, full_v, *, scale, layer_idx)
         self.layer_idx, self.tp = layer_idx, tp
 
-    def forward(self, x: torch.Tensor, cache: KVCache, start_pos: int, cos: torch.Tensor, sin: torch.Tensor):
+    def forward(self, x: torch.Tensor, cache, start_pos: int, cos: torch.Tensor, sin: torch.Tensor):
         B, T, _ = x.shape
         q = self.q_norm(self.q(x).view(B, T, self.H, self.d)).transpose(1, 2)
         k = self.k_norm(self.k(x).view(B, T, self.H_kv, self.d)).transpose(1, 2)
         v = self.v(x).view(B, T, self.H_kv, self.d).transpose(1, 2)
         q, k = apply_rope(q, k, cos, sin)
-        kc, vc = cache.k[self.layer_idx], cache.v[self.layer_idx]
-        kc[:B, :, start_pos:start_pos + T] = k
-        vc[:B, :, start_pos:start_pos + T] = v
+        _cache_op(cache, "write")(self.layer_idx, k, v, start_pos)
         n = start_pos + T
         scale = 1.0 / math.sqrt(self.d)
         if T == 1 and self.decode_attn_op is not None:
-            out = self.decode_attn_op(q, kc[:B, :, :n], vc[:B, :, :n], scale=scale, layer_idx=self.layer_idx)
-        elif start_pos == 0:
+            if not getattr(cache, "plain", True):
+                raise ValueError("the decode seam reads a plain cache: decode a quantised or shared-prefix cache with "
+                                 "GraphDecoder(mode='dense')")
+            full_k, full_v = _cache_op(cache, "rows")(self.layer_idx, B, n, q.dtype)
+            out = self.decode_attn_op(q, full_k, full_v, scale=scale, layer_idx=self.layer_idx)
+        elif start_pos == 0 and getattr(cache, "plain", True):
             out = F.scaled_dot_product_attention(q, k, v, is_causal=T > 1, enable_gqa=True)
         else:
+            # (a chunk attends over its own keys as the cache holds them, so the result does not depend on the chunks)
             mask = torch.ones(T, n, dtype=torch.bool, device=x.device).tril_(diagonal=start_pos)
-            out = F.scaled_dot_product_attention(q, kc[:B, :, :n], vc[:B, :, :n], attn_mask=mask, enable_gqa=True)
+            full_k, full_v = _cache_op(cache, "rows")(self.layer_idx, B, n, q.dtype)
+            out = F.scaled_dot_product_attention(q, full_k, full_v, attn_mask=mask, enable_gqa=True)
         return self.tp.all_reduce(self.o(out.transpose(1, 2).reshape(B, T, self.H * self.d)))
 
 
@@ -203,10 +233,25 @@ class Qwen3Model(nn.Module):
             f.down.weight.copy_(rows_of(draw(cfg.intermediate_size, cfg.hidden_size), tp.size).t())
         return self
 
-    def alloc_cache(self, max_seq_len: int, max_batch: int = 1, dtype=None) -> KVCache:
+    def alloc_cache(self, max_seq_len: int, max_batch: int = 1, dtype=None, bits: int = 16):
+        """A cache for ``max_batch`` sequences; ``bits`` 8 or 4: one that holds quantised rows (``QuantKVCache``)."""
         p = self.embed.weight
+        if bits in (8, 4):
+            from .quant_cache import QuantKVCache
+            return QuantKVCache(len(self.layers), max_batch, self.cfg.num_key_value_heads, max_seq_len, self.cfg.head_dim,
+                                bits, p.device)
+        if bits != 16:
+            raise ValueError("bits must be 16 (the model's own type), 8 or 4")
         return KVCache(len(self.layers), max_batch, self.cfg.num_key_value_heads, max_seq_len, self.cfg.head_dim,
                        dtype or p.dtype, p.device)
+
+    def alloc_prefix_cache(self, prefix_len: int, own_len: int, max_batch: int, dtype=None):
+        """A cache whose ``max_batch`` sequences share a prefix of up to ``prefix_len`` positions and keep up to
+        ``own_len`` positions each behind it (``PrefixKVCache``): prefill the prompt into its ``.prefix``."""
+        from .prefix_cache import PrefixKVCache
+        p = self.embed.weight
+        return PrefixKVCache(len(self.layers), max_batch, self.cfg.num_key_value_heads, prefix_len, own_len,
+                             self.cfg.head_dim, dtype or p.dtype, p.device)
 
     def logits(self, h: torch.Tensor) -> torch.Tensor:
         """Full-vocabulary logits of hidden states ``h [B, T, hidden]``."""
@@ -219,7 +264,7 @@ class Qwen3Model(nn.Module):
         dist.all_gather(parts, part.contiguous(), group=self.tp.group)
         return torch.cat(parts, dim=-1)
 
-    def forward(self, ids: torch.Tensor, cache: KVCache, start_pos: int = 0, last_only: bool = False) -> torch.Tensor:
+    def forward(self, ids: torch.Tensor, cache, start_pos: int = 0, last_only: bool = False) -> torch.Tensor:
         B, T = ids.shape
         h = self.embed(ids)
         cos, sin = self.rope_cos[start_pos:start_pos + T], self.rope_sin[start_pos:start_pos + T]
@@ -231,23 +276,22 @@ class Qwen3Model(nn.Module):
         return self.logits(h)
 
     @torch.no_grad()
-    def prefill_ragged(self, prompts: list[torch.Tensor], cache: KVCache, chunk: int = 2048) -> list[torch.Tensor]:
+    def prefill_ragged(self, prompts: list[torch.Tensor], cache, chunk: int = 2048) -> list[torch.Tensor]:
         """Prompts of different lengths, one per sequence of the cache: sequence ``b`` is prefilled on its own rows
         of the cache (a view of batch 1).  Returns the last-position logits of each; ``cache.cur_len`` becomes the
         list of lengths."""
         outs = []
         for b, ids in enumerate(prompts):
-            view = KVCache.__new__(KVCache)
-            view.k, view.v = [k[b:b + 1] for k in cache.k], [v[b:b + 1] for v in cache.v]
-            view.cur_len, view.max_seq_len = 0, cache.max_seq_len
-            outs.append(self.prefill(ids.view(1, -1), view, chunk=chunk))
-        cache.cur_len = [int(p.numel()) for p in prompts]
+            outs.append(self.prefill(ids.view(1, -1), _cache_op(cache, "sequence")(b), chunk=chunk))
+        first = getattr(cache, "first", 0)
+        cache.cur_len = [first + int(p.numel()) for p in prompts]
         return outs
 
     @torch.no_grad()
-    def prefill(self, ids: torch.Tensor, cache: KVCache, chunk: int = 2048) -> torch.Tensor:
-        """Run the prompt through the model in chunks; returns the logits of the last position."""
-        out = None
+    def prefill(self, ids: torch.Tensor, cache, chunk: int = 2048) -> torch.Tensor:
+        """Run the prompt through the model in chunks, from the cache's first row (the sequences of a shared-prefix
+        cache begin behind the prefix); returns the logits of the last position."""
+        out, first = None, getattr(cache, "first", 0)
         for s in range(0, ids.shape[1], chunk):
-            out = self.forward(ids[:, s:s + chunk], cache, start_pos=s, last_only=True)
+            out = self.forward(ids[:, s:s + chunk], cache, start_pos=first + s, last_only=True)
         return out

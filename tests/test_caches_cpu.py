@@ -1,0 +1,253 @@
+"""Quantised and shared-prefix caches without a GPU: what the C entry points and the Python classes refuse, the stored
+layout, and the caches' bookkeeping."""
+
+from __future__ import annotations
+
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+from sparse_kv_reads_b200 import (GraphDecoder, PrefixAttentionGraph, PrefixKVCache, QuantAttentionGraph, QuantKVCache,
+                                  Qwen3Config, Qwen3Model)
+from sparse_kv_reads_b200 import _lib
+from sparse_kv_reads_b200.build import build
+from _caches import pack, quantise
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+OK = 0x1000
+CPU = torch.device("cpu")
+
+
+@pytest.fixture(scope="module")
+def L():
+    build()
+    return _lib.lib()
+
+
+def qcache(**o):
+    c = _lib.SkvQCache(OK, OK, OK, None, 2, 4, 64, 128, 8, 0)
+    for name, v in o.items():
+        setattr(c, name, v)
+    return ctypes.byref(c)
+
+
+def test_the_struct_matches_the_header():
+    text = open(os.path.join(ROOT, "include", "skv.h")).read()
+    body = text[text.index("typedef struct skv_qcache {"):text.index("} skv_qcache;")]
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    names = re.findall(r"[\s*]([a-z_0-9]+)(?=[,;])", body)
+    assert names == [f[0] for f in _lib.SkvQCache._fields_]
+    assert ctypes.sizeof(_lib.SkvQCache) == 4 * 8 + 6 * 4
+
+
+BAD_CACHES = [(dict(k=None), -1), (dict(v=None), -1), (dict(scale=None), -1), (dict(d=64), -2), (dict(bits=6), -5),
+              (dict(batch=0), -5), (dict(h_kv=-1), -5), (dict(capacity=0), -5), (dict(batch=70000), -5),
+              (dict(k=0x1008), -4), (dict(scale=0x1004), -4)]
+
+
+@pytest.mark.parametrize("name", ["skv_quant_write", "skv_quant_read"])
+def test_rows_are_refused_on_the_host(L, name):
+    base = dict(k=OK, v=OK, dtype=0, batch=2, tokens=3, kb=4096, kh=1024, kr=128, vb=4096, vh=1024, vr=128, pos=None,
+                per=0, pos0=0)
+
+    def call(c=None, **o):
+        a = {**base, **o}
+        return getattr(L, name)(qcache() if c is None else c, a["k"], a["v"], a["dtype"], a["batch"], a["tokens"], a["kb"],
+                                a["kh"], a["kr"], a["vb"], a["vh"], a["vr"], a["pos"], a["per"], a["pos0"], None)
+
+    for over, code in BAD_CACHES:
+        assert call(qcache(**over)) == code, over
+    assert getattr(L, name)(None, OK, OK, 0, 1, 1, 0, 0, 0, 0, 0, 0, None, 0, 0, None) == -1
+    assert call(k=None) == -1 and call(v=None) == -1 and call(dtype=3) == -3
+    assert call(batch=3) == -5 and call(batch=0) == -5 and call(tokens=-1) == -5 and call(tokens=65) == -5
+    assert call(pos0=62) == -5 and call(pos0=-1) == -5
+    assert call(k=0x1002) == -4 and call(kr=100) == -4 and call(vh=3) == -4 and call(dtype=1, vb=2) == -4
+    assert call(tokens=0) == 0                                                   # nothing to do, nothing launched
+
+
+def test_the_decode_steps_write_is_refused_on_the_host(L):
+    args = dict(qkv=OK, qw=OK, kw=OK, cos=OK, sin=OK, pos=OK, q=OK, batch=2, H=8)
+
+    def call(c=None, **o):
+        a = {**args, **o}
+        return L.skv_qk_rope_quant(qcache() if c is None else c, a["qkv"], a["qw"], a["kw"], a["cos"], a["sin"], a["pos"],
+                                   0, a["q"], a["batch"], a["H"], 1e-6, None)
+
+    for over, code in BAD_CACHES:
+        assert call(qcache(**over)) == code, over
+    for name in ("qkv", "qw", "kw", "cos", "sin", "pos", "q"):
+        assert call(**{name: None}) == -1
+    assert call(H=0) == -5 and call(H=6) == -5 and call(batch=3) == -5 and call(q=0x1004) == -4 and call(qw=0x1004) == -4
+
+
+def test_attention_over_quantised_rows_is_refused_on_the_host(L):
+    args = dict(q=OK, dtype=0, G=2, n=OK, ng=0, out=OK, ws=OK, splits=4)
+
+    def call(c=None, **o):
+        a = {**args, **o}
+        return L.skv_attend_quant(qcache() if c is None else c, a["q"], a["dtype"], a["G"], a["n"], a["ng"], a["out"],
+                                  a["ws"], a["splits"], 0.1, None)
+
+    for over, code in BAD_CACHES:
+        assert call(qcache(**over)) == code, over
+    for name in ("q", "n", "out", "ws"):
+        assert call(**{name: None}) == -1
+    assert call(dtype=2) == -3 and call(G=0) == -2 and call(G=9) == -2 and call(splits=0) == -5 and call(ng=-1) == -5
+    assert call(q=0x1008) == -4 and call(out=0x1002) == -4 and call(ws=0x1008) == -4
+
+
+def test_attention_over_a_shared_prefix_is_refused_on_the_host(L):
+    args = dict(q=OK, kp=OK, vp=OK, P=100, k=OK, v=OK, n=OK, ng=0, out=OK, ws=OK, batch=2, h=4, G=2, d=128, dtype=0,
+                kph=128 * 100, kpr=128, vph=128 * 100, vpr=128, kh=128 * 64, kr=128, vh=128 * 64, vr=128, lim=64, splits=4)
+
+    def call(**o):
+        a = {**args, **o}
+        return L.skv_attend_prefix(a["q"], a["kp"], a["vp"], a["P"], a["k"], a["v"], a["n"], a["ng"], a["out"], a["ws"], None,
+                                   a["batch"], a["h"], a["G"], a["d"], a["dtype"], a["kph"], a["kpr"], a["vph"], a["vpr"],
+                                   a["kh"], a["kr"], a["vh"], a["vr"], a["lim"], a["splits"], 0.1, None)
+
+    for name in ("q", "kp", "vp", "k", "v", "n", "out", "ws"):
+        assert call(**{name: None}) == -1, name
+    assert call(d=64) == -2 and call(G=0) == -2 and call(G=9) == -2 and call(dtype=5) == -3
+    assert call(batch=0) == -5 and call(h=0) == -5 and call(batch=20000) == -5 and call(P=-1) == -5 and call(lim=-1) == -5
+    assert call(P=2 ** 31 - 2) == -5 and call(splits=0) == -5 and call(ng=-1) == -5
+    assert call(q=0x1008) == -4 and call(kp=0x1004) == -4 and call(kpr=132) == -4 and call(kpr=64) == -4
+    assert call(vr=100) == -4 and call(kh=4) == -4
+    assert L.skv_prefix_splits(0, 8, 2, 0) == -5 and L.skv_prefix_splits(2, 8, 9, 0) == -2
+    assert L.skv_prefix_splits(2, 8, 2, 9) == -3 and L.skv_prefix_splits(2, 8, 2, 0) >= 1
+    assert L.skv_prefix_workspace_bytes(0, 8, 2, 128, 4) == -5 and L.skv_prefix_workspace_bytes(2, 8, 2, 64, 4) == -5
+
+
+def test_quantised_cache_checks_its_arguments():
+    with pytest.raises(ValueError, match="8 or 4 bits"):
+        QuantKVCache(1, 1, 2, 16, 128, 6, CPU)
+    with pytest.raises(ValueError, match="head_dim"):
+        QuantKVCache(1, 1, 2, 16, 64, 8, CPU)
+    c = QuantKVCache(2, 3, 2, 16, 128, 4, CPU)
+    assert c.k[0].shape == (3, 2, 16, 64) and c.scale[1].shape == (3, 2, 16, 2, 4) and c.check_status() == 0
+    x = torch.zeros(3, 2, 4, 128, dtype=torch.bfloat16)
+    for bad in (x[..., :64], x[:, :1], torch.zeros(4, 2, 4, 128, dtype=torch.bfloat16), x[0]):
+        with pytest.raises(ValueError, match="must be"):
+            c.write(0, bad, bad, 0)
+    with pytest.raises(ValueError, match="one type"):
+        c.write(0, x, x.float(), 0)
+    with pytest.raises(ValueError, match="unsupported"):
+        c.write(0, x.half(), x.half(), 0)
+    for pos in (-1, 13):
+        with pytest.raises(ValueError, match="outside"):
+            c.write(0, x, x, pos)
+        with pytest.raises(ValueError, match="outside"):
+            c.read(0, pos, 4)
+    for pos in (torch.tensor([0, 1]), torch.tensor([0], dtype=torch.int32), torch.tensor(3)):
+        with pytest.raises(ValueError, match="positions are"):
+            c.write(0, x, x, pos)
+    with pytest.raises(ValueError, match="3 sequences"):
+        c.read(0, 0, 1, batch=4)
+    with pytest.raises(ValueError, match="no gradient"):
+        y = x.clone().requires_grad_()
+        c.write(0, y, y, 0)
+    c.write(0, x[:, :, :0], x[:, :, :0], 16)                                     # nothing to write: no launch
+    assert c.read(0, 3, 0)[0].shape == (3, 2, 0, 128)
+    with pytest.raises(ValueError, match="codes must be"):
+        QuantKVCache.from_tensors(c.k, c.v, c.scale, 8)
+    with pytest.raises(ValueError, match="scales must be"):
+        QuantKVCache.from_tensors(c.k, c.v, [s.float() for s in c.scale], 4)
+    one = c.sequence(2)
+    assert one.batch == 1 and one.k[1].data_ptr() == c.k[1][2].data_ptr() and one.status.data_ptr() == c.status[4:].data_ptr()
+
+
+def test_attention_objects_check_their_arguments(L):
+    with pytest.raises(ValueError, match="divide"):
+        QuantAttentionGraph(H=5, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
+    with pytest.raises(ValueError, match="divide"):
+        PrefixAttentionGraph(B=1, H=5, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
+    with pytest.raises(_lib.SkvError):
+        PrefixAttentionGraph(B=1, H=18, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
+    with pytest.raises(ValueError, match="unsupported"):
+        QuantAttentionGraph(H=4, H_kv=2, d=128, dtype=torch.float16, device=CPU)
+    q, n = torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    c = QuantKVCache(1, 1, 2, 16, 128, 8, CPU)
+    a = QuantAttentionGraph(H=4, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
+    with pytest.raises(ValueError, match="queries must be"):
+        a(q[:3], c, 0, n)
+    with pytest.raises(ValueError, match="queries must be"):
+        a(q.float(), c, 0, n)
+    with pytest.raises(ValueError, match="KV heads"):
+        a(q, QuantKVCache(1, 1, 4, 16, 128, 8, CPU), 0, n)
+    with pytest.raises(ValueError, match="lengths must be"):
+        a(q, c, 0, n.long())
+    a.n_group = 1
+    with pytest.raises(ValueError, match="lengths must be"):
+        a(q, c, 0, n)
+    p = PrefixAttentionGraph(B=2, H=4, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
+    q8, kp, k = torch.zeros(8, 128, dtype=torch.bfloat16), torch.zeros(2, 9, 128, dtype=torch.bfloat16), \
+        torch.zeros(4, 5, 128, dtype=torch.bfloat16)
+    for args, word in (((q, kp, kp, k, k, n), "queries must be"), ((q8, kp[:1], kp[:1], k, k, n), "prefix must be"),
+                       ((q8, kp, kp[:, :3], k, k, n), "prefix must be"), ((q8, kp, kp, k[:3], k[:3], n), "rows must be"),
+                       ((q8, kp.float(), kp.float(), k, k, n), "type and device"),
+                       ((q8, kp, kp, k, k, n.long()), "lengths must be"),
+                       ((q8, kp, kp, k.transpose(1, 2).contiguous().transpose(1, 2), k, n), "unit last stride")):
+        with pytest.raises(ValueError, match=word):
+            p(*args)
+
+
+def test_four_bit_layout_puts_one_run_of_each_group_side_by_side():
+    code = torch.arange(128).view(1, 128) // 32 - 2                              # the group's number, less two
+    stored = pack(code, 4)
+    assert stored.view(8, 8).tolist() == [[0x66, 0x66, 0x77, 0x77, 0x88, 0x88, 0x99, 0x99]] * 8
+    code, scale = quantise(torch.zeros(1, 128), 4)
+    assert int(pack(code, 4).sum()) == 64 * 0x88 and scale.tolist() == [[0.0] * 4]
+
+
+TINY = dict(hidden_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=128,
+            intermediate_size=96, vocab_size=200, max_position_embeddings=256)
+
+
+def test_shared_prefix_prefill_equals_whole_prompts():
+    m = Qwen3Model(Qwen3Config(**TINY)).eval().init_random(seed=3, std=0.1)
+    g = torch.Generator().manual_seed(0)
+    doc = torch.randint(0, 200, (1, 30), generator=g)
+    asks = [torch.randint(0, 200, (n,), generator=g) for n in (5, 12)]
+    cache = m.alloc_prefix_cache(40, 16, 2)
+    with torch.no_grad():
+        m.prefill(doc, cache.prefix, chunk=8)
+        assert cache.first == 30 and cache.max_seq_len == 46 and cache.cur_len == 30
+        got = m.prefill_ragged(asks, cache, chunk=4)
+        for b, a in enumerate(asks):
+            want = m.prefill(torch.cat((doc[0], a)).view(1, -1), m.alloc_cache(64), chunk=16)
+            torch.testing.assert_close(got[b], want, rtol=1e-4, atol=1e-4)       # float32, sums in another order
+        assert cache.cur_len == [35, 42]
+        # both sequences at once
+        cache.cur_len = 30
+        two = m(torch.stack([a[:5] for a in asks]), cache, start_pos=30, last_only=True)
+        torch.testing.assert_close(two[:1], got[0], rtol=1e-4, atol=1e-4)
+    with pytest.raises(ValueError, match="behind the prefix"):
+        m(doc, cache, start_pos=3)
+    with pytest.raises(ValueError, match="behind the prefix"):
+        cache.cur_len = 29
+    m.layers[0].attn.decode_attn_op = lambda *a, **k: None
+    with pytest.raises(ValueError, match="plain cache"):
+        m(doc[:, :1], cache, start_pos=30)
+    with pytest.raises(ValueError, match="bits must be"):
+        m.alloc_cache(16, bits=5)
+
+
+def test_the_clustered_mode_refuses_the_new_caches_and_steps_are_checked():
+    m = Qwen3Model(Qwen3Config(**TINY)).eval()
+    for cache in (m.alloc_cache(16, bits=8), m.alloc_prefix_cache(8, 8, 2)):
+        with pytest.raises(ValueError, match="mode='dense'"):
+            GraphDecoder(m, cache, mode="cluster")
+    cache = m.alloc_prefix_cache(8, 4, 2)
+    assert isinstance(cache, PrefixKVCache)
+    cache.prefix.cur_len = 6
+    dec = GraphDecoder(m, cache, mode="dense")
+    dec.prepare(6)
+    for pos in (5, 10):
+        with pytest.raises(ValueError, match="outside the cache"):
+            dec.step(torch.zeros(2, 1, dtype=torch.long), pos)
+    cache.prefix.cur_len = 7
+    with pytest.raises(ValueError, match="prefix has changed"):
+        dec.step(torch.zeros(2, 1, dtype=torch.long), 8)

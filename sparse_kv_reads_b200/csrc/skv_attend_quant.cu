@@ -1,6 +1,21 @@
 // Attention of one new token per sequence over a quantised KV cache, split over CTAs, merged by the last CTA of a head.
 //
-// Simple kernel: half a warp per row, float32 arithmetic on the CUDA cores.
+// bf16 queries: tensor-core kernel.  Both products take half-float operands, because a code turns into a half float with
+// one byte permutation or one logic operation: 0x6400 | c is 1024 + c, 0x6400 | c << 4 is 1024 + 16 c.
+//   S^T = K Q^T (16 keys on M, up to 8 query heads on N).  The order of the 128 components is free as long as both sides
+//     agree on it, so a lane takes the bytes it needs straight from global memory, 16 at a time, and the queries are
+//     fetched in the matching order; nothing goes through shared memory.  The offsets (1152 = 1024 + 128 in 8 bits) stay
+//     in the codes: the accumulators start at minus the offset times the sum of the query.  Queries are scaled by a power
+//     of two to a largest component in [1, 2), which half floats hold to 2^-25 of that.
+//   O^T = V^T (P vs): component d of the values on M, keys on K.  A lane reads the same bytes of the value rows of its
+//     four keys and pairs them up by permutation.  The value's scale goes into the weights (per scale group in 4 bits).
+// Two running references per head, in base 2: m for the sum of weights (largest score) and r for the accumulators (largest
+// score + log2 of the value's scale), so that the half floats 2^(z - r) vs keep their precision whatever the scales.  A
+// reference is only raised when something passes it by 8: products up to 256 cost a half float nothing, and most tiles
+// then need no shuffles.  A weight is rounded to 11 bits; sums and accumulators are float32.
+// float32 queries: half a warp per row, float32 arithmetic on the CUDA cores.
+#include <cuda_fp16.h>
+
 #include "skv_attend_finish.cuh"
 #include "skv_quant.cuh"
 
@@ -83,6 +98,368 @@ __global__ void __launch_bounds__(128) attend_quant_simple_kernel(const AttendQu
     finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, &s_flag, red, 2 * WARPS * GP);
 }
 
+// ---------------------------------------------------------------------------------------------
+// tensor-core path
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+    return y;
+}
+__device__ __forceinline__ uint32_t hsub(uint32_t x, float by) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&x), __float2half2_rn(by));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t hfma(uint32_t x, float mul, float add) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&x), __float2half2_rn(mul), __float2half2_rn(add));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+constexpr uint32_t F16_1024 = 0x64006400u;                // two half floats of 1024, whose last place counts 1
+
+// What one lane holds of 16 cached positions: lane = 4 g + t.  Keys: rows g and g + 8; values: rows 2t, 2t+1, 2t+8, 2t+9.
+template <int BITS>
+struct RawTile;
+template <>
+struct RawTile<8> {
+    uint4 k[2][2];                                        // [row g, g + 8][16-byte chunk t, t + 4]
+    uint4 v[4];                                           // chunk g of the four rows
+    uint32_t s[2];                                        // (key scale, value scale) of rows g, g + 8
+};
+template <>
+struct RawTile<4> {
+    uint4 k[2];                                           // chunk t: runs 2t and 2t + 1 of every scale group
+    uint2 v[4];                                           // bytes 8g .. 8g+7: run g of every scale group
+    uint4 s[2];                                           // four key scales, four value scales
+};
+
+template <int BITS>
+struct WarpAttendQuant {
+    using Q = Quant<BITS>;
+    static constexpr int GR = Q::GROUPS;
+    uint32_t qb[8][2];                 // Q^T fragments in the order of the codes, column = head g
+    float off[GR][2];                  // what the accumulators of heads 2t, 2t + 1 start from, per scale group
+    float acc[8][4];                   // O^T: 8-bit tile j: components 16 g + 2 j, + 1; 4-bit tile (group, i): 32 group + 4 g + 2 i, + 1
+    float mA, mB, lA, lB;              // reference of the weights / partial sum of heads 2t, 2t + 1
+    float rA, rB, fA, fB;              // reference of the accumulators, and 2^(m - r)
+    float qsA, qsB;                    // score scale of the two heads, with the query's power of two
+    int g, t;
+
+    __device__ __forceinline__ void init(const __nv_bfloat16 *q, int G, float scale_log2) {
+        const int lane = threadIdx.x & 31;
+        g = lane >> 2; t = lane & 3;
+        // component index of the eight 4-component runs this lane owns of head g's query
+        float x[8][4];
+        float top = 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const int d = BITS == 8 ? (s < 4 ? t * 16 + 4 * s : 64 + t * 16 + 4 * (s - 4)) : 32 * (s >> 1) + 8 * t + 4 * (s & 1);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (g < G) v = load4(q + g * HEAD_DIM + d);
+            x[s][0] = v.x; x[s][1] = v.y; x[s][2] = v.z; x[s][3] = v.w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[s][i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // exponent of the largest component, kept where its inverse is a normal number too
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        if (!(top > 0.f) || e > 127) e = 0;
+        e = max(e, -120);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+        float sum[GR];
+#pragma unroll
+        for (int i = 0; i < GR; ++i) sum[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            if constexpr (BITS == 8) {                    // one k-step per run
+                qb[s][0] = pack_f16(x[s][0] * down, x[s][1] * down);
+                qb[s][1] = pack_f16(x[s][2] * down, x[s][3] * down);
+                const float2 a = unpack_f16(qb[s][0]), b = unpack_f16(qb[s][1]);
+                sum[0] -= 1152.f * ((a.x + a.y) + (b.x + b.y));
+            } else {                                      // k-steps (group, 0) and (group, 1) of runs 2t, 2t + 1
+                const int gr = s >> 1, i = (s & 1) * 2;   // components i and i + 1 of both runs
+                qb[s][0] = pack_f16(x[2 * gr][i] * down, x[2 * gr + 1][i] * down);
+                qb[s][1] = pack_f16(x[2 * gr][i + 1] * down * 0.0625f, x[2 * gr + 1][i + 1] * down * 0.0625f);
+                const float2 a = unpack_f16(qb[s][0]), b = unpack_f16(qb[s][1]);
+                sum[gr] -= 1032.f * (a.x + a.y) + 1152.f * (b.x + b.y);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+            off[i][0] = __shfl_sync(0xffffffffu, sum[i], 8 * t);          // head 2t: lanes 4 (2t) ..
+            off[i][1] = __shfl_sync(0xffffffffu, sum[i], 8 * t + 4);
+        }
+        const float qs = up * scale_log2;
+        qsA = __shfl_sync(0xffffffffu, qs, 8 * t);
+        qsB = __shfl_sync(0xffffffffu, qs, 8 * t + 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        mA = mB = NEG_BIG;
+        rA = rB = NEG_BIG;
+        lA = lB = fA = fB = 0.f;
+    }
+
+    // scores of keys g, g + 8 for heads 2t, 2t + 1: z = (A, g), (B, g), (A, g + 8), (B, g + 8), in base 2
+    __device__ __forceinline__ void scores(const RawTile<BITS> &r, float (&z)[4]) const {
+        if constexpr (BITS == 8) {
+            float c[4] = {off[0][0], off[0][1], off[0][0], off[0][1]}, c2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const uint4 &q0 = r.k[0][s >> 2], &q1 = r.k[1][s >> 2];
+                const uint32_t w0 = (s & 3) == 0 ? q0.x : (s & 3) == 1 ? q0.y : (s & 3) == 2 ? q0.z : q0.w;
+                const uint32_t w1 = (s & 3) == 0 ? q1.x : (s & 3) == 1 ? q1.y : (s & 3) == 2 ? q1.z : q1.w;
+                mma_f16_16816(s & 1 ? c2 : c, __byte_perm(w0, F16_1024, 0x5150), __byte_perm(w1, F16_1024, 0x5150),
+                              __byte_perm(w0, F16_1024, 0x5352), __byte_perm(w1, F16_1024, 0x5352), qb[s][0], qb[s][1]);
+            }
+            const float k0 = bf16_low(r.s[0]), k1 = bf16_low(r.s[1]);
+            z[0] = (c[0] + c2[0]) * qsA * k0; z[1] = (c[1] + c2[1]) * qsB * k0;
+            z[2] = (c[2] + c2[2]) * qsA * k1; z[3] = (c[3] + c2[3]) * qsB * k1;
+        } else {
+            z[0] = z[1] = z[2] = z[3] = 0.f;
+#pragma unroll
+            for (int gr = 0; gr < 4; ++gr) {
+                const uint32_t sel = gr & 1 ? 0x7632 : 0x5410;
+                uint32_t a = gr < 2 ? __byte_perm(r.k[0].x, r.k[0].z, sel) : __byte_perm(r.k[0].y, r.k[0].w, sel);
+                uint32_t b = gr < 2 ? __byte_perm(r.k[1].x, r.k[1].z, sel) : __byte_perm(r.k[1].y, r.k[1].w, sel);
+                float c[4] = {off[gr][0], off[gr][1], off[gr][0], off[gr][1]};
+                mma_f16_16816(c, and_or(a, 0x000f000fu, F16_1024), and_or(b, 0x000f000fu, F16_1024),
+                              and_or(a, 0x00f000f0u, F16_1024), and_or(b, 0x00f000f0u, F16_1024), qb[2 * gr][0], qb[2 * gr][1]);
+                a >>= 8; b >>= 8;
+                mma_f16_16816(c, and_or(a, 0x000f000fu, F16_1024), and_or(b, 0x000f000fu, F16_1024),
+                              and_or(a, 0x00f000f0u, F16_1024), and_or(b, 0x00f000f0u, F16_1024), qb[2 * gr + 1][0],
+                              qb[2 * gr + 1][1]);
+                const uint32_t s0 = gr < 2 ? r.s[0].x : r.s[0].y, s1 = gr < 2 ? r.s[1].x : r.s[1].y;
+                const float k0 = gr & 1 ? bf16_high(s0) : bf16_low(s0), k1 = gr & 1 ? bf16_high(s1) : bf16_low(s1);
+                z[0] = fmaf(c[0], k0, z[0]); z[1] = fmaf(c[1], k0, z[1]);
+                z[2] = fmaf(c[2], k1, z[2]); z[3] = fmaf(c[3], k1, z[3]);
+            }
+            z[0] *= qsA; z[1] *= qsB; z[2] *= qsA; z[3] *= qsB;
+        }
+    }
+
+    // value scale of a row's group
+    static __device__ __forceinline__ float value_scale(const RawTile<BITS> &r, int row, int gr) {
+        if constexpr (BITS == 8) return bf16_high(r.s[row]);
+        else {
+            const uint32_t w = gr < 2 ? r.s[row].z : r.s[row].w;
+            return gr & 1 ? bf16_high(w) : bf16_low(w);
+        }
+    }
+
+    // A fragment pair of one m-tile from the codes of two keys x, y: components (row g, row g + 8)
+    __device__ __forceinline__ void pair8(uint32_t x, uint32_t y, bool high, uint32_t &a, uint32_t &b) const {
+        const uint32_t p = __byte_perm(x, y, high ? 0x7362 : 0x5140);     // x_i, y_i, x_i+1, y_i+1
+        a = hsub(__byte_perm(p, F16_1024, 0x5150), 1152.f);
+        b = hsub(__byte_perm(p, F16_1024, 0x5352), 1152.f);
+    }
+
+    // one tile of 16 positions, `left` of them cached (16 or more: all)
+    __device__ __forceinline__ void consume(const RawTile<BITS> &r, float (&z)[4], int left) {
+        const bool ok0 = g < left, ok1 = g + 8 < left;
+        if (left < 16) {
+            if (!ok0) z[0] = z[1] = NEG_BIG;
+            if (!ok1) z[2] = z[3] = NEG_BIG;
+        }
+        float v0 = 0.f, v1 = 0.f;                          // largest value scale of the lane's two keys
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) { v0 = fmaxf(v0, value_scale(r, 0, gr)); v1 = fmaxf(v1, value_scale(r, 1, gr)); }
+        v0 = __log2f(v0); v1 = __log2f(v1);                // (-inf for values of zero: they never raise r)
+        float tA = fmaxf(z[0], z[2]), tB = fmaxf(z[1], z[3]);
+        float yA = fmaxf(z[0] + v0, z[2] + v1), yB = fmaxf(z[1] + v0, z[3] + v1);
+        if (__any_sync(0xffffffffu, tA > mA + 8.f || tB > mB + 8.f || yA > rA + 8.f || yB > rB + 8.f)) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                tA = fmaxf(tA, __shfl_xor_sync(0xffffffffu, tA, o)); tB = fmaxf(tB, __shfl_xor_sync(0xffffffffu, tB, o));
+                yA = fmaxf(yA, __shfl_xor_sync(0xffffffffu, yA, o)); yB = fmaxf(yB, __shfl_xor_sync(0xffffffffu, yB, o));
+            }
+            const float nA = fmaxf(mA, tA), nB = fmaxf(mB, tB);
+            lA *= fast_exp2(mA - nA); lB *= fast_exp2(mB - nB);
+            mA = nA; mB = nB;
+            // (r no further below m than a float's exponent reaches)
+            const float sA = fmaxf(fmaxf(rA, yA), mA - 120.f), sB = fmaxf(fmaxf(rB, yB), mB - 120.f);
+            const float alA = fast_exp2(rA - sA), alB = fast_exp2(rB - sB);
+            rA = sA; rB = sB;
+            fA = fast_exp2(mA - rA); fB = fast_exp2(mB - rB);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                acc[j][0] *= alA; acc[j][1] *= alB;
+                acc[j][2] *= alA; acc[j][3] *= alB;
+            }
+        }
+        float p0 = fast_exp2(z[0] - mA), p1 = fast_exp2(z[1] - mB), p2 = fast_exp2(z[2] - mA), p3 = fast_exp2(z[3] - mB);
+        if (left < 16) {
+            if (!ok0) p0 = p1 = 0.f;
+            if (!ok1) p2 = p3 = 0.f;
+        }
+        lA += p0 + p2; lB += p1 + p3;
+        p0 *= fA; p1 *= fB; p2 *= fA; p3 *= fB;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            const float w0 = value_scale(r, 0, gr), w1 = value_scale(r, 1, gr);
+            const uint32_t b0 = movmatrix_trans(pack_f16(p0 * w0, p1 * w0)), b1 = movmatrix_trans(pack_f16(p2 * w1, p3 * w1));
+            if constexpr (BITS == 8) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t a0, a1, a2, a3;
+                    const int i = j >> 1;
+                    pair8(i == 0 ? r.v[0].x : i == 1 ? r.v[0].y : i == 2 ? r.v[0].z : r.v[0].w,
+                          i == 0 ? r.v[1].x : i == 1 ? r.v[1].y : i == 2 ? r.v[1].z : r.v[1].w, j & 1, a0, a1);
+                    pair8(i == 0 ? r.v[2].x : i == 1 ? r.v[2].y : i == 2 ? r.v[2].z : r.v[2].w,
+                          i == 0 ? r.v[3].x : i == 1 ? r.v[3].y : i == 2 ? r.v[3].z : r.v[3].w, j & 1, a2, a3);
+                    mma_f16_16816(acc[j], a0, a1, a2, a3, b0, b1);
+                }
+            } else {
+                const uint32_t sel = gr & 1 ? 0x7632 : 0x5410;
+                uint32_t x = gr < 2 ? __byte_perm(r.v[0].x, r.v[1].x, sel) : __byte_perm(r.v[0].y, r.v[1].y, sel);
+                uint32_t y = gr < 2 ? __byte_perm(r.v[2].x, r.v[3].x, sel) : __byte_perm(r.v[2].y, r.v[3].y, sel);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    mma_f16_16816(acc[2 * gr + i], hsub(and_or(x, 0x000f000fu, F16_1024), 1032.f),
+                                  hfma(and_or(x, 0x00f000f0u, F16_1024), 0.0625f, -72.f),
+                                  hsub(and_or(y, 0x000f000fu, F16_1024), 1032.f),
+                                  hfma(and_or(y, 0x00f000f0u, F16_1024), 0.0625f, -72.f), b0, b1);
+                    x >>= 8; y >>= 8;
+                }
+            }
+        }
+    }
+
+    // leave this warp's (sums, maximum, sum of weights) of heads < G in red[(warp * G + head) * 132 ..]
+    __device__ __forceinline__ void store_partial(float *red, int warp, int G) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            lA += __shfl_xor_sync(0xffffffffu, lA, o);
+            lB += __shfl_xor_sync(0xffffffffu, lB, o);
+        }
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const int head = 2 * t + which;
+            if (head >= G) continue;
+            float *o = red + (warp * G + head) * 132;
+            // back to weights relative to m, in two steps: values near the largest numbers have 2^(r - m) beyond them
+            const float up = fast_exp2(0.5f * (which ? rB - mB : rA - mA));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int d = BITS == 8 ? 16 * g + 2 * j : 32 * (j >> 1) + 4 * g + 2 * (j & 1);
+                *reinterpret_cast<float2 *>(o + d) = make_float2(acc[j][which] * up * up, acc[j][2 + which] * up * up);
+            }
+            if (g == 0) { o[128] = which ? mB : mA; o[129] = which ? lB : lA; }
+        }
+    }
+};
+
+template <int BITS>
+__device__ __forceinline__ void load_keys(RawTile<BITS> &r, const unsigned char *k, int left, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const bool ok = g + 8 * h < left;
+        if constexpr (BITS == 8) {
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            r.k[h][0] = ok ? __ldcs(reinterpret_cast<const uint4 *>(k + h * 1024)) : zero;
+            r.k[h][1] = ok ? __ldcs(reinterpret_cast<const uint4 *>(k + h * 1024 + 64)) : zero;
+        } else {
+            r.k[h] = ok ? __ldcs(reinterpret_cast<const uint4 *>(k + h * 512)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+}
+template <int BITS>
+__device__ __forceinline__ void load_scales(RawTile<BITS> &r, const unsigned char *s, int left, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const bool ok = g + 8 * h < left;
+        if constexpr (BITS == 8) r.s[h] = ok ? __ldcs(reinterpret_cast<const uint32_t *>(s + h * 32)) : 0u;
+        else r.s[h] = ok ? __ldcs(reinterpret_cast<const uint4 *>(s + h * 128)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+template <int BITS>
+__device__ __forceinline__ void load_values(RawTile<BITS> &r, const unsigned char *v, int left, int t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = (i & 1) + (i >> 1) * 8;           // beside row 2t
+        const bool ok = 2 * t + row < left;
+        if constexpr (BITS == 8) r.v[i] = ok ? __ldcs(reinterpret_cast<const uint4 *>(v + row * 128)) : make_uint4(0u, 0u, 0u, 0u);
+        else r.v[i] = ok ? __ldcs(reinterpret_cast<const uint2 *>(v + row * 64)) : make_uint2(0u, 0u);
+    }
+}
+
+constexpr int QUANT_STAGE_ROWS = 80;   // partial rows the merging CTA stages: 40 splits of two query heads in one trip
+
+template <int BITS, int U, int CTAS>
+__global__ void __launch_bounds__(128, CTAS) attend_quant_mma_kernel(const AttendQuantParams p) {
+    using Q = Quant<BITS>;
+    constexpr int WARPS = 4, ROWS = 16 * U;
+    __shared__ __align__(16) float red[QUANT_STAGE_ROWS * 132];
+    __shared__ int s_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int head = blockIdx.y, split = blockIdx.x;
+    const int n = min(max(positions_of(p.n_dev, p.n_group, head), 0), p.capacity);
+    const int tiles = (n + ROWS - 1) / ROWS;
+    const int s_eff = min(p.splits, max(1, (tiles + WARPS - 1) / WARPS));
+    if (split >= s_eff) return;
+    const int slots = s_eff * WARPS, per = (tiles + slots - 1) / slots;
+    const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
+    const int64_t row0 = (int64_t)head * p.capacity + (int64_t)t0 * ROWS;
+    const unsigned char *k = p.kc + (row0 + g) * Q::ROW_BYTES + t * 16;
+    const unsigned char *v = p.vc + (row0 + 2 * t) * Q::ROW_BYTES + g * (Q::ROW_BYTES / 8);
+    const unsigned char *s = reinterpret_cast<const unsigned char *>(p.scale) + (row0 + g) * Q::SCALES * 2;
+    int left = n - t0 * ROWS;
+    RawTile<BITS> r[U];
+    if (t0 < t1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, left - 16 * u, g);
+            load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, left - 16 * u, g);
+            load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, left - 16 * u, t);
+        }
+    }
+    WarpAttendQuant<BITS> wa;
+    wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * p.G * HEAD_DIM, p.G, p.scale_log2);
+    for (int i = t0; i < t1; ++i) {
+        // a part's registers take the next tile's as soon as they are used up: a whole tile is always in flight
+        const int next = i + 1 < t1 ? left - ROWS : 0;
+        k += ROWS * Q::ROW_BYTES; v += ROWS * Q::ROW_BYTES; s += ROWS * Q::SCALES * 2;
+        float z[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            wa.scores(r[u], z[u]);
+            load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, next - 16 * u, g);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (U == 1 || left > 16 * u) wa.consume(r[u], z[u], left - 16 * u);
+            load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, next - 16 * u, g);
+            load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, next - 16 * u, t);
+        }
+        left -= ROWS;
+    }
+    wa.store_partial(red, warp, p.G);
+    __syncthreads();
+    finish_head<__nv_bfloat16>(p, red, WARPS, head, split, s_eff, &s_flag, red, QUANT_STAGE_ROWS);
+}
+
+template <int BITS, int U, int CTAS>
+static int launch_quant_mma(const AttendQuantParams &p, cudaStream_t st) {
+    attend_quant_mma_kernel<BITS, U, CTAS><<<dim3(p.splits, p.heads), 128, 0, st>>>(p);
+    SKV_CUDA_OK(cudaGetLastError());
+    return SKV_OK;
+}
+
 template <typename T, int BITS>
 static int launch_quant_simple(const AttendQuantParams &p, cudaStream_t st) {
     const dim3 grid(p.splits, p.heads);
@@ -117,5 +494,5 @@ extern "C" int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, i
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_F32) return c->bits == 8 ? launch_quant_simple<float, 8>(p, st) : launch_quant_simple<float, 4>(p, st);
-    return c->bits == 8 ? launch_quant_simple<__nv_bfloat16, 8>(p, st) : launch_quant_simple<__nv_bfloat16, 4>(p, st);
+    return c->bits == 8 ? launch_quant_mma<8, 2, 3>(p, st) : launch_quant_mma<4, 2, 3>(p, st);
 }

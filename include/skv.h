@@ -466,10 +466,13 @@ int skv_qk_rope_quant(const skv_qcache *c, const void *qkv, const void *q_norm_w
                       int batch, int H, float eps, void *stream);
 /* Softmax attention of one query per query head over the quantised rows [0, n): skv_attend's dense mode
  * (ssa/kernels/graph_kernels.py:27-59) for a quantised cache.  q, out [batch * h_kv * G, 128] dtype, G <= 8; n_dev and
- * n_group as everywhere (a length beyond the capacity counts as the capacity); workspace of
- * skv_attend_workspace_bytes(batch * h_kv, G, 128, splits), zero-initialised once; a head without rows gets zeros. */
+ * n_group as everywhere (a length beyond the capacity counts as the capacity).  `ctas` CTAs share all heads' rows evenly
+ * (skv_quant_ctas: as many as the current device runs at once); workspace of skv_quant_workspace_bytes(batch * h_kv, G, 128,
+ * ctas), zero-initialised once.  A head without rows gets zeros. */
+int skv_quant_ctas(void);
+int64_t skv_quant_workspace_bytes(int heads, int G, int d, int ctas);
 int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, int G, const int32_t *n_dev, int n_group, void *out,
-                     void *workspace, int splits, float scale, void *stream);
+                     void *workspace, int ctas, float scale, void *stream);
 
 /* Attention of a batch whose sequences share a prefix: query row of (sequence b, KV head h) attends over the prefix's
  * rows [0, prefix) of head h, which exist once, and over its own rows [0, n) of cache head b * h_kv + h.  The reference

@@ -22,7 +22,7 @@ EXPORTS = ("skv_version", "skv_error_string", "skv_last_cuda_error", "skv_attend
            "skv_insert_max_members", "skv_fit_tensor_cores", "skv_fit_workspace_bytes", "skv_fit", "skv_rebin",
            "skv_add_rmsnorm", "skv_qk_rope_cache", "skv_silu_mul", "skv_gemv", "skv_gemv_attended", "skv_gemv_supported", "skv_gemv_tp", "skv_comm_bytes", "skv_comm_alloc",
            "skv_comm_export", "skv_comm_open", "skv_comm_close", "skv_comm_free", "skv_comm_view", "skv_comm_tick", "skv_comm_push", "skv_comm_reduce", "skv_comm_status",
-           "skv_quant_write", "skv_quant_read", "skv_qk_rope_quant", "skv_attend_quant", "skv_prefix_splits",
+           "skv_quant_write", "skv_quant_read", "skv_qk_rope_quant", "skv_quant_ctas", "skv_quant_workspace_bytes", "skv_attend_quant", "skv_prefix_splits",
            "skv_prefix_workspace_bytes", "skv_attend_prefix")
 
 
@@ -164,6 +164,10 @@ def _declare(lib) -> None:
     lib.skv_quant_read.argtypes = lib.skv_quant_write.argtypes
     lib.skv_qk_rope_quant.restype = i32
     lib.skv_qk_rope_quant.argtypes = [qc, vp, vp, vp, vp, vp, vp, i32, vp, i32, i32, f32, vp]
+    lib.skv_quant_ctas.restype = i32
+    lib.skv_quant_ctas.argtypes = []
+    lib.skv_quant_workspace_bytes.restype = i64
+    lib.skv_quant_workspace_bytes.argtypes = [i32, i32, i32, i32]
     lib.skv_attend_quant.restype = i32
     lib.skv_attend_quant.argtypes = [qc, vp, i32, i32, vp, i32, vp, vp, i32, f32, vp]
     lib.skv_prefix_splits.restype = i32

@@ -109,7 +109,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attend_mma_kernel(const AttendP
     float *red = reinterpret_cast<float *>(smem);
     wa.store_partial(red, warp, G);
     __syncthreads();
-    finish_head<__nv_bfloat16>(p, red, WARPS, head, split, sh.s_eff, &s_flag, red, WARPS * STAGES * 8192 / (PART_LD * 4));
+    finish_head<__nv_bfloat16>(p, red, WARPS, head, split, sh.s_eff, (int64_t)head * p.splits,
+                               &s_flag, red, WARPS * STAGES * 8192 / (PART_LD * 4));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -201,7 +202,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attend_labels_kernel(const Atte
     wa.store_partial(red, warp, G);
     __syncthreads();
     stamp(p, 4);
-    finish_head<__nv_bfloat16>(p, red, WARPS, head, split, s_eff, &s_flag, red, WARPS * STAGES * 8192 / (PART_LD * 4));
+    finish_head<__nv_bfloat16>(p, red, WARPS, head, split, s_eff, (int64_t)head * p.splits,
+                               &s_flag, red, WARPS * STAGES * 8192 / (PART_LD * 4));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(128) attend_simple_kernel(const AttendParams p
         if (sub == 0) { r[128] = m[g]; r[129] = l[g]; }
     }
     __syncthreads();
-    finish_head<T>(p, red, 2 * WARPS, head, split, sh.s_eff, &s_flag, red, 2 * WARPS * GP);
+    finish_head<T>(p, red, 2 * WARPS, head, split, sh.s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
 }
 
 // natural-log merge of caller-provided partials

@@ -12,16 +12,18 @@ constexpr int PART_LD = 132;               // floats per partial row: 128 sums, 
 template <typename Params>
 __device__ __forceinline__ void stamp(const Params &, int) {}
 
-// `p` needs: out, part [heads, splits, G, 132], ticket [heads], G, splits.
-// Combine the partial (max, sum, acc) sets that the warps of this CTA left in shared memory
-// (red[set][g][132]: 128 acc, then max, sum), publish the CTA's partial, and let the last CTA of the
-// head merge all partials into `out`.  blockDim.x must be 128 (one thread per output column).
+// `p` needs: out, part [slots, G, 132], ticket [heads], G.  The head's s_eff partials lie in the slots from slot0 on; this
+// CTA's is number `split` of them.
+// blockDim.x is 128: one thread per output column.
+
+// Combine the partial (max, sum, acc) sets that the warps of this CTA left in shared memory (red[set][g][132]: 128 acc,
+// then max, sum): into the output where this CTA alone served the head, else into the CTA's slot.
 template <typename T, typename Params>
-__device__ __forceinline__ void finish_head(const Params &p, const float *red, int sets, int head, int split,
-                                            int s_eff, int *sh_flag, float *stage, int stage_rows) {
+__device__ __forceinline__ void publish_head(const Params &p, const float *red, int sets, int head, int split, int s_eff,
+                                             int64_t slot0) {
     const int G = p.G, tid = threadIdx.x;
     T *out = static_cast<T *>(p.out);
-    float *pa = p.part + ((int64_t)head * p.splits + split) * G * PART_LD;
+    float *pa = p.part + (slot0 + split) * G * PART_LD;
 #pragma unroll 1
     for (int g = 0; g < G; ++g) {
         float M = NEG_BIG;
@@ -40,26 +42,20 @@ __device__ __forceinline__ void finish_head(const Params &p, const float *red, i
             if (tid == 0) __stcg(reinterpret_cast<float2 *>(pa + g * PART_LD + HEAD_DIM), make_float2(M, dn));
         }
     }
-    if (s_eff == 1) return;
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        int t = atomicAdd(p.ticket + head, 1);
-        *sh_flag = (t == s_eff - 1);
-    }
-    __syncthreads();
-    stamp(p, 5);
-    if (!*sh_flag) return;
-    __threadfence();
-    // Merge of the head's partials by this (last) CTA.  The partial rows are copied into the shared memory
-    // the CTA no longer needs with asynchronous 16-byte copies, all requested before any is used: one round
-    // trip to L2 where they fit (stage_rows rows), chunks of one query head's splits with a running maximum
-    // otherwise.  Up to four query heads are then folded at once, each by 4 / (their number) warps that share
-    // its rows; a lane owns four columns.
-    float *stg = stage;
+}
+
+// Merge of the head's partials by the CTA that published last.  The partial rows are copied into the shared memory
+// the CTA no longer needs with asynchronous 16-byte copies, all requested before any is used: one round
+// trip to L2 where they fit (stage_rows rows), chunks of one query head's splits with a running maximum
+// otherwise.  Up to four query heads are then folded at once, each by 4 / (their number) warps that share
+// its rows; a lane owns four columns.
+template <typename T, typename Params>
+__device__ __forceinline__ void merge_head(const Params &p, int head, int s_eff, int64_t slot0, float *stg, int stage_rows) {
+    const int G = p.G, tid = threadIdx.x;
+    T *out = static_cast<T *>(p.out);
     __shared__ __align__(16) float s_sum[4][PART_LD];
     const int lane = tid & 31, wid = tid >> 5;
-    const float *src = p.part + (int64_t)head * p.splits * G * PART_LD;
+    const float *src = p.part + slot0 * G * PART_LD;
     const int gc = max(1, min(G, stage_rows / s_eff));        // query heads staged together
     const int cs = gc > 1 ? s_eff : min(s_eff, stage_rows);   // splits per chunk
     for (int g0 = 0; g0 < G; g0 += gc) {
@@ -127,6 +123,26 @@ __device__ __forceinline__ void finish_head(const Params &p, const float *red, i
         }
     }
     if (tid == 0) p.ticket[head] = 0;     // ready for the next call on this stream
+}
+
+// Both, with the ticket between them: the last CTA of the head to publish merges.
+template <typename T, typename Params>
+__device__ __forceinline__ void finish_head(const Params &p, const float *red, int sets, int head, int split,
+                                            int s_eff, int64_t slot0, int *sh_flag, float *stage,
+                                            int stage_rows) {
+    publish_head<T>(p, red, sets, head, split, s_eff, slot0);
+    if (s_eff == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int t = atomicAdd(p.ticket + head, 1);
+        *sh_flag = (t == s_eff - 1);
+    }
+    __syncthreads();
+    stamp(p, 5);
+    if (!*sh_flag) return;
+    __threadfence();
+    merge_head<T>(p, head, s_eff, slot0, stage, stage_rows);
     stamp(p, 6);
 }
 

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
         if (sub == 0) { r[128] = m[g]; r[129] = l[g]; }
     }
     __syncthreads();
-    finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, &s_flag, red, 2 * WARPS * GP);
+    finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
 }
 
 template <typename T>

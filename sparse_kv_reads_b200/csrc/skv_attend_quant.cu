@@ -27,9 +27,12 @@ struct AttendQuantParams {
     const __nv_bfloat16 *scale;
     const int32_t *n_dev;
     void *out;
-    float *part;       // [heads, splits, G, 132]
+    float *part;       // [ctas + heads, G, 132]
     int32_t *ticket;   // [heads]
-    int heads, G, n_group, capacity, splits;
+    int heads, G, n_group, capacity;
+    int ctas;          // CTAs that share the rows
+    int splits;        // CTAs per head of the float32 kernel
+    int stage_rows;    // rows of 132 floats of shared memory
     float scale_log2;
 };
 
@@ -95,7 +98,7 @@ __global__ void __launch_bounds__(128) attend_quant_simple_kernel(const AttendQu
         if (sub == 0) { r[128] = m[g]; r[129] = l[g]; }
     }
     __syncthreads();
-    finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, &s_flag, red, 2 * WARPS * GP);
+    finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -128,6 +131,7 @@ __device__ __forceinline__ uint32_t hfma(uint32_t x, float mul, float add) {
 }
 __device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 constexpr uint32_t F16_1024 = 0x64006400u;                // two half floats of 1024, whose last place counts 1
 
 // What one lane holds of 16 cached positions: lane = 4 g + t.  Keys: rows g and g + 8; values: rows 2t, 2t+1, 2t+8, 2t+9.
@@ -221,9 +225,7 @@ struct WarpAttendQuant {
             float c[4] = {off[0][0], off[0][1], off[0][0], off[0][1]}, c2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                const uint4 &q0 = r.k[0][s >> 2], &q1 = r.k[1][s >> 2];
-                const uint32_t w0 = (s & 3) == 0 ? q0.x : (s & 3) == 1 ? q0.y : (s & 3) == 2 ? q0.z : q0.w;
-                const uint32_t w1 = (s & 3) == 0 ? q1.x : (s & 3) == 1 ? q1.y : (s & 3) == 2 ? q1.z : q1.w;
+                const uint32_t w0 = word(r.k[0][s >> 2], s & 3), w1 = word(r.k[1][s >> 2], s & 3);
                 mma_f16_16816(s & 1 ? c2 : c, __byte_perm(w0, F16_1024, 0x5150), __byte_perm(w1, F16_1024, 0x5150),
                               __byte_perm(w0, F16_1024, 0x5352), __byte_perm(w1, F16_1024, 0x5352), qb[s][0], qb[s][1]);
             }
@@ -269,20 +271,30 @@ struct WarpAttendQuant {
         b = hsub(__byte_perm(p, F16_1024, 0x5352), 1152.f);
     }
 
-    // one tile of 16 positions, `left` of them cached (16 or more: all)
-    __device__ __forceinline__ void consume(const RawTile<BITS> &r, float (&z)[4], int left) {
-        const bool ok0 = g < left, ok1 = g + 8 < left;
-        if (left < 16) {
-            if (!ok0) z[0] = z[1] = NEG_BIG;
-            if (!ok1) z[2] = z[3] = NEG_BIG;
-        }
-        float v0 = 0.f, v1 = 0.f;                          // largest value scale of the lane's two keys
+    // U blocks of 16 positions, `left` positions cached (16 U or more: all)
+    template <int U>
+    __device__ __forceinline__ void consume(const RawTile<BITS> (&r)[U], float (&z)[U][4], int left) {
+        if (left < 16 * U) {
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) { v0 = fmaxf(v0, value_scale(r, 0, gr)); v1 = fmaxf(v1, value_scale(r, 1, gr)); }
-        v0 = __log2f(v0); v1 = __log2f(v1);                // (-inf for values of zero: they never raise r)
-        float tA = fmaxf(z[0], z[2]), tB = fmaxf(z[1], z[3]);
-        float yA = fmaxf(z[0] + v0, z[2] + v1), yB = fmaxf(z[1] + v0, z[3] + v1);
-        if (__any_sync(0xffffffffu, tA > mA + 8.f || tB > mB + 8.f || yA > rA + 8.f || yB > rB + 8.f)) {
+            for (int u = 0; u < U; ++u) {
+                if (g + 16 * u >= left) z[u][0] = z[u][1] = NEG_BIG;
+                if (g + 8 + 16 * u >= left) z[u][2] = z[u][3] = NEG_BIG;
+            }
+        }
+        float tA = NEG_BIG, tB = NEG_BIG, yA = NEG_BIG, yB = NEG_BIG;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float v0 = 0.f, v1 = 0.f;                      // largest value scale of the lane's two keys
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) {
+                v0 = fmaxf(v0, value_scale(r[u], 0, gr));
+                v1 = fmaxf(v1, value_scale(r[u], 1, gr));
+            }
+            v0 = __log2f(v0); v1 = __log2f(v1);            // (-inf for values of zero: they never raise r)
+            tA = fmaxf(tA, fmaxf(z[u][0], z[u][2])); tB = fmaxf(tB, fmaxf(z[u][1], z[u][3]));
+            yA = fmaxf(yA, fmaxf(z[u][0] + v0, z[u][2] + v1)); yB = fmaxf(yB, fmaxf(z[u][1] + v0, z[u][3] + v1));
+        }
+        if (__any_sync(0xffffffffu, fmaxf(tA - mA, yA - rA) > 8.f || fmaxf(tB - mB, yB - rB) > 8.f)) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 tA = fmaxf(tA, __shfl_xor_sync(0xffffffffu, tA, o)); tB = fmaxf(tB, __shfl_xor_sync(0xffffffffu, tB, o));
@@ -302,42 +314,46 @@ struct WarpAttendQuant {
                 acc[j][2] *= alA; acc[j][3] *= alB;
             }
         }
-        float p0 = fast_exp2(z[0] - mA), p1 = fast_exp2(z[1] - mB), p2 = fast_exp2(z[2] - mA), p3 = fast_exp2(z[3] - mB);
-        if (left < 16) {
-            if (!ok0) p0 = p1 = 0.f;
-            if (!ok1) p2 = p3 = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            z[u][0] = fast_exp2(z[u][0] - mA); z[u][1] = fast_exp2(z[u][1] - mB);
+            z[u][2] = fast_exp2(z[u][2] - mA); z[u][3] = fast_exp2(z[u][3] - mB);
+            if (left < 16 * U) {
+                if (g + 16 * u >= left) z[u][0] = z[u][1] = 0.f;
+                if (g + 8 + 16 * u >= left) z[u][2] = z[u][3] = 0.f;
+            }
+            lA += z[u][0] + z[u][2]; lB += z[u][1] + z[u][3];
+            z[u][0] *= fA; z[u][1] *= fB; z[u][2] *= fA; z[u][3] *= fB;
         }
-        lA += p0 + p2; lB += p1 + p3;
-        p0 *= fA; p1 *= fB; p2 *= fA; p3 *= fB;
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) {
-            const float w0 = value_scale(r, 0, gr), w1 = value_scale(r, 1, gr);
-            const uint32_t b0 = movmatrix_trans(pack_f16(p0 * w0, p1 * w0)), b1 = movmatrix_trans(pack_f16(p2 * w1, p3 * w1));
-            if constexpr (BITS == 8) {
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t a0, a1, a2, a3;
-                    const int i = j >> 1;
-                    pair8(i == 0 ? r.v[0].x : i == 1 ? r.v[0].y : i == 2 ? r.v[0].z : r.v[0].w,
-                          i == 0 ? r.v[1].x : i == 1 ? r.v[1].y : i == 2 ? r.v[1].z : r.v[1].w, j & 1, a0, a1);
-                    pair8(i == 0 ? r.v[2].x : i == 1 ? r.v[2].y : i == 2 ? r.v[2].z : r.v[2].w,
-                          i == 0 ? r.v[3].x : i == 1 ? r.v[3].y : i == 2 ? r.v[3].z : r.v[3].w, j & 1, a2, a3);
-                    mma_f16_16816(acc[j], a0, a1, a2, a3, b0, b1);
-                }
-            } else {
-                const uint32_t sel = gr & 1 ? 0x7632 : 0x5410;
-                uint32_t x = gr < 2 ? __byte_perm(r.v[0].x, r.v[1].x, sel) : __byte_perm(r.v[0].y, r.v[1].y, sel);
-                uint32_t y = gr < 2 ? __byte_perm(r.v[2].x, r.v[3].x, sel) : __byte_perm(r.v[2].y, r.v[3].y, sel);
+            for (int gr = 0; gr < GR; ++gr) {
+                const float w0 = value_scale(r[u], 0, gr), w1 = value_scale(r[u], 1, gr);
+                const uint32_t b0 = movmatrix_trans(pack_f16(z[u][0] * w0, z[u][1] * w0));
+                const uint32_t b1 = movmatrix_trans(pack_f16(z[u][2] * w1, z[u][3] * w1));
+                if constexpr (BITS == 8) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    mma_f16_16816(acc[2 * gr + i], hsub(and_or(x, 0x000f000fu, F16_1024), 1032.f),
-                                  hfma(and_or(x, 0x00f000f0u, F16_1024), 0.0625f, -72.f),
-                                  hsub(and_or(y, 0x000f000fu, F16_1024), 1032.f),
-                                  hfma(and_or(y, 0x00f000f0u, F16_1024), 0.0625f, -72.f), b0, b1);
-                    x >>= 8; y >>= 8;
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t a0, a1, a2, a3;
+                        pair8(word(r[u].v[0], j >> 1), word(r[u].v[1], j >> 1), j & 1, a0, a1);
+                        pair8(word(r[u].v[2], j >> 1), word(r[u].v[3], j >> 1), j & 1, a2, a3);
+                        mma_f16_16816(acc[j], a0, a1, a2, a3, b0, b1);
+                    }
+                } else {
+                    const uint32_t sel = gr & 1 ? 0x7632 : 0x5410;
+                    uint32_t x = gr < 2 ? __byte_perm(r[u].v[0].x, r[u].v[1].x, sel) : __byte_perm(r[u].v[0].y, r[u].v[1].y, sel);
+                    uint32_t y = gr < 2 ? __byte_perm(r[u].v[2].x, r[u].v[3].x, sel) : __byte_perm(r[u].v[2].y, r[u].v[3].y, sel);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        mma_f16_16816(acc[2 * gr + i], hsub(and_or(x, 0x000f000fu, F16_1024), 1032.f),
+                                      hfma(and_or(x, 0x00f000f0u, F16_1024), 0.0625f, -72.f),
+                                      hsub(and_or(y, 0x000f000fu, F16_1024), 1032.f),
+                                      hfma(and_or(y, 0x00f000f0u, F16_1024), 0.0625f, -72.f), b0, b1);
+                        x >>= 8; y >>= 8;
+                    }
                 }
             }
-        }
     }
 
     // leave this warp's (sums, maximum, sum of weights) of heads < G in red[(warp * G + head) * 132 ..]
@@ -398,64 +414,213 @@ __device__ __forceinline__ void load_values(RawTile<BITS> &r, const unsigned cha
     }
 }
 
-constexpr int QUANT_STAGE_ROWS = 80;   // partial rows the merging CTA stages: 40 splits of two query heads in one trip
-
-template <int BITS, int U, int CTAS>
-__global__ void __launch_bounds__(128, CTAS) attend_quant_mma_kernel(const AttendQuantParams p) {
-    using Q = Quant<BITS>;
-    constexpr int WARPS = 4, ROWS = 16 * U;
-    __shared__ __align__(16) float red[QUANT_STAGE_ROWS * 132];
-    __shared__ int s_flag;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int head = blockIdx.y, split = blockIdx.x;
-    const int n = min(max(positions_of(p.n_dev, p.n_group, head), 0), p.capacity);
-    const int tiles = (n + ROWS - 1) / ROWS;
-    const int s_eff = min(p.splits, max(1, (tiles + WARPS - 1) / WARPS));
-    if (split >= s_eff) return;
-    const int slots = s_eff * WARPS, per = (tiles + slots - 1) / slots;
-    const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
-    const int64_t row0 = (int64_t)head * p.capacity + (int64_t)t0 * ROWS;
-    const unsigned char *k = p.kc + (row0 + g) * Q::ROW_BYTES + t * 16;
-    const unsigned char *v = p.vc + (row0 + 2 * t) * Q::ROW_BYTES + g * (Q::ROW_BYTES / 8);
-    const unsigned char *s = reinterpret_cast<const unsigned char *>(p.scale) + (row0 + g) * Q::SCALES * 2;
-    int left = n - t0 * ROWS;
-    RawTile<BITS> r[U];
-    if (t0 < t1) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, left - 16 * u, g);
-            load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, left - 16 * u, g);
-            load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, left - 16 * u, t);
-        }
-    }
-    WarpAttendQuant<BITS> wa;
-    wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * p.G * HEAD_DIM, p.G, p.scale_log2);
-    for (int i = t0; i < t1; ++i) {
-        // a part's registers take the next tile's as soon as they are used up: a whole tile is always in flight
-        const int next = i + 1 < t1 ? left - ROWS : 0;
-        k += ROWS * Q::ROW_BYTES; v += ROWS * Q::ROW_BYTES; s += ROWS * Q::SCALES * 2;
-        float z[U][4];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            wa.scores(r[u], z[u]);
-            load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, next - 16 * u, g);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (U == 1 || left > 16 * u) wa.consume(r[u], z[u], left - 16 * u);
-            load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, next - 16 * u, g);
-            load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, next - 16 * u, t);
-        }
-        left -= ROWS;
-    }
-    wa.store_partial(red, warp, p.G);
-    __syncthreads();
-    finish_head<__nv_bfloat16>(p, red, WARPS, head, split, s_eff, &s_flag, red, QUANT_STAGE_ROWS);
+constexpr int QUANT_CTAS_PER_SM = 3;   // 168 registers a thread
+// Rows of 132 floats of shared memory: the warps' partials of two heads at least, and what the merging CTA stages of a head
+// in one trip.  No more than that: the first-level cache, which the loads in flight pass through, gets the rest (128 heads
+// of 8,191 rows and fewer, four query heads: 46 us with 32 rows per CTA, 53 us with 128).
+constexpr int QUANT_MAX_ROWS = 128;
+static int quant_stage_rows(int heads, int G, int ctas) {
+    const int merge = (ctas / heads + 1) * G;
+    return merge < 8 * G ? 8 * G : merge > QUANT_MAX_ROWS ? QUANT_MAX_ROWS : merge;
 }
 
-template <int BITS, int U, int CTAS>
+// The ways of sharing the work out, below, in blocks of 16 rows.  Measured on B200 (8-bit rows, two query heads, us):
+// ALONE: a head up to this long is left to one CTA, without a merge (32 blocks: 8.2, in two parts 9.7; 63 blocks: 10.2 and
+//   8.6 in ten parts).  LEAST: blocks of a CTA at least, where a head is split.  HOP: what the longest run of an even
+//   sharing may be beyond the average (64 heads of 512 blocks: even 35.8, line 36.9; of 2,048: 116 and 109; 8 heads of
+//   2,048: 21.8 and 25.6).
+constexpr int QUANT_ALONE = 32, QUANT_LEAST = 8, QUANT_HOP = 24;
+
+// (a * b - less) / c where the result fits 31 bits: a 32-bit quotient where the product allows it (all but billions of rows)
+__device__ __forceinline__ int64_t mul_div(int64_t a, int64_t b, int64_t c, int less = 0) {
+    const uint64_t ab = (uint64_t)a * (uint64_t)b - less;
+    if ((ab >> 32) == 0 && (c >> 32) == 0) return (uint32_t)ab / (uint32_t)c;
+    return (int64_t)(ab / (uint64_t)c);
+}
+
+// The rows of all heads, cut into blocks of 16, are shared out over the CTAs in one of two ways.
+// Even: every head gets the same number of CTAs, each a run of its blocks.  It costs least where it leaves no CTA much more
+//   than the average: no CTA serves two heads.
+// Line: the blocks of all heads form one line and every CTA takes an equal run of it, whatever the lengths.  A head may be
+//   met by several CTAs and a CTA may meet several heads; the partials of the pair (CTA c, head h) have slot c + h, which
+//   no two pairs share (both only grow along the line), and a head's slots lie side by side.
+// A CTA's warps take a quarter each of what the CTA has of a head and go on to the next head without waiting for one
+// another; partials are combined, published and merged at the end (or when the shared memory for them is full).
+// A head without rows counts one block, so that it gets its zeros.
+struct QuantSegment {
+    int head, split, parts;
+    int64_t slot0;
+};
+
+template <int BITS, int U>
+__global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kernel(const AttendQuantParams p) {
+    using Q = Quant<BITS>;
+    constexpr int WARPS = 4, ROWS = 16 * U, MAX_SEG = QUANT_MAX_ROWS / WARPS;
+    extern __shared__ __align__(16) float red[];          // stage_rows x 132
+    __shared__ int s_scan[40];
+    __shared__ float s_max[32];
+    // (kept here, the tile loop needs the registers)
+    __shared__ int64_t s_line, s_end, s_place[WARPS];     // where a warp's next head begins, and its first block there
+    __shared__ int s_ctas, s_even, s_head[WARPS], s_b0[WARPS];
+    __shared__ QuantSegment s_seg[MAX_SEG];
+    __shared__ int s_last[MAX_SEG];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    pdl_wait();
+    pdl_trigger();
+    const int group = p.n_group > 0 ? min(p.n_group, p.heads) : p.heads;
+    const int groups = (p.heads + group - 1) / group;     // of heads that share one length
+    auto blocks_of = [&](int i) {
+        const int n = min(max(p.n_dev[i], 0), p.capacity);
+        return max(1, (n + 15) >> 4);
+    };
+    auto heads_of = [&](int i) { return min(group, p.heads - i * group); };
+    // Sums of the groups' blocks ahead of this thread's contiguous share of them (they pass 31 bits beyond 34 billion
+    // rows: the lower 20 bits and the rest are scanned apart), and the longest head.
+    const int share = (groups + 127) / 128;
+    const int i0 = min(tid * share, groups), i1 = min(i0 + share, groups);
+    int64_t before = 0, mine = 0, line;
+    int longest = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int b = blocks_of(i);
+        mine += (int64_t)b * heads_of(i);
+        longest = max(longest, b);
+    }
+    if (groups == 1) {
+        longest = blocks_of(0);
+        line = (int64_t)longest * p.heads;
+    } else {
+        int low, high;
+        const int64_t lo = block_excl_scan((int)(mine & 0xfffff), s_scan, low);
+        const int64_t hi = block_excl_scan((int)(mine >> 20), s_scan, high);
+        before = (hi << 20) + lo;
+        line = ((int64_t)high << 20) + low;
+        longest = (int)block_max((float)longest, s_max);  // (to 24 bits: it only chooses the way of sharing)
+    }
+    // CTAs per head, shared out evenly, and CTAs on the line
+    const int each = longest <= QUANT_ALONE ? 1 : max(1, min(longest / QUANT_LEAST, (int)gridDim.x / p.heads));
+    const int on_line = (int)max((int64_t)1, min((int64_t)gridDim.x, line / (2 * QUANT_LEAST)));
+    const bool even = (int)gridDim.x >= p.heads && (longest + each - 1) / each <= line / on_line + QUANT_HOP;
+    const int ctas = even ? each * p.heads : on_line;
+    if (blockIdx.x >= ctas) return;
+    if (even) {
+        const int head = blockIdx.x / each, part = blockIdx.x - head * each, b = blocks_of(head / group);
+        const int parts = min(each, b);
+        if (part >= parts) return;
+        if (tid < WARPS) {
+            s_head[tid] = head; s_place[tid] = 0;
+            s_b0[tid] = (int)((int64_t)b * part / parts);
+            if (tid == 0) {
+                s_end = (int64_t)b * (part + 1) / parts;
+                s_seg[0] = {head, part, parts, (int64_t)head * each};
+            }
+        }
+    } else {
+        const int64_t at = mul_div(line, blockIdx.x, ctas);
+        if (groups == 1 ? tid == 0 : (at >= before && at < before + mine)) {            // exactly one thread
+            int i = groups == 1 ? 0 : i0;
+            int64_t one = (int64_t)blocks_of(i) * heads_of(i);
+            while (at >= before + one) { before += one; ++i; one = (int64_t)blocks_of(i) * heads_of(i); }
+            const int h = (int)mul_div(at - before, 1, blocks_of(i));
+            const int64_t place = before + (int64_t)h * blocks_of(i);
+            s_end = mul_div(line, blockIdx.x + 1, ctas);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) { s_head[w] = i * group + h; s_place[w] = place; s_b0[w] = (int)(at - place); }
+        }
+        if (tid == 0) { s_line = line; s_ctas = ctas; }
+    }
+    if (tid == 0) s_even = even;
+    __syncthreads();
+    const int seg_cap = p.stage_rows / (WARPS * p.G), seg_floats = WARPS * p.G * PART_LD;
+    for (bool more = true; more;) {
+        int segs = 0;
+        while (segs < seg_cap) {
+            const int head = s_head[warp], b0 = s_b0[warp];
+            const int64_t place = s_place[warp];
+            more = place + b0 < s_end;
+            if (!more) break;
+            const int n = min(max(positions_of(p.n_dev, p.n_group, head), 0), p.capacity);
+            const int blocks = max(1, (n + 15) >> 4), b1 = (int)min(s_end - place, (int64_t)blocks);
+            __syncwarp();
+            if (lane == 0) {
+                s_head[warp] = head + 1; s_place[warp] = place + blocks; s_b0[warp] = 0;
+                if (warp == 0 && !s_even) {               // CTAs that meet this head: from its first block's to its last's
+                    const int c0 = (int)mul_div(place + 1, s_ctas, s_line, 1), c1 = (int)mul_div(place + blocks, s_ctas, s_line, 1);
+                    s_seg[segs] = {head, (int)blockIdx.x - c0, c1 - c0 + 1, (int64_t)c0 + head};
+                }
+            }
+            __syncwarp();
+            // this warp's rows [r0, r1)
+            const int per = (b1 - b0 + WARPS - 1) / WARPS;
+            const int r0 = min((b0 + warp * per) * 16, n), r1 = min((b0 + min((warp + 1) * per, b1 - b0)) * 16, n);
+            const int64_t row0 = (int64_t)head * p.capacity + r0;
+            const unsigned char *k = p.kc + (row0 + g) * Q::ROW_BYTES + t * 16;
+            const unsigned char *v = p.vc + (row0 + 2 * t) * Q::ROW_BYTES + g * (Q::ROW_BYTES / 8);
+            const unsigned char *s = reinterpret_cast<const unsigned char *>(p.scale) + (row0 + g) * Q::SCALES * 2;
+            RawTile<BITS> r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, r1 - r0 - 16 * u, g);
+                load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, r1 - r0 - 16 * u, g);
+                load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, r1 - r0 - 16 * u, t);
+            }
+            WarpAttendQuant<BITS> wa;
+            wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * p.G * HEAD_DIM, p.G, p.scale_log2);
+            for (int left = r1 - r0; left > 0; left -= ROWS) {
+                // a part's registers take the next tile's as soon as they are used up: a whole tile is always in flight
+                const int next = left - ROWS;
+                k += ROWS * Q::ROW_BYTES; v += ROWS * Q::ROW_BYTES; s += ROWS * Q::SCALES * 2;
+                float z[U][4];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    wa.scores(r[u], z[u]);
+                    load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, next - 16 * u, g);
+                }
+                wa.consume(r, z, left);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, next - 16 * u, g);
+                    load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, next - 16 * u, t);
+                }
+            }
+            wa.store_partial(red + segs * seg_floats, warp, p.G);
+            ++segs;
+        }
+        __syncthreads();
+        bool shared = false;
+        for (int i = 0; i < segs; ++i) {
+            publish_head<__nv_bfloat16>(p, red + i * seg_floats, WARPS, s_seg[i].head, s_seg[i].split, s_seg[i].parts,
+                                        s_seg[i].slot0);
+            shared |= s_seg[i].parts > 1;
+        }
+        if (shared) {
+            __threadfence();
+            __syncthreads();
+            if (tid < segs) {
+                const int parts = s_seg[tid].parts;
+                s_last[tid] = parts > 1 && atomicAdd(p.ticket + s_seg[tid].head, 1) == parts - 1;
+            }
+            __syncthreads();
+            __threadfence();
+            for (int i = 0; i < segs; ++i)
+                if (s_last[i]) merge_head<__nv_bfloat16>(p, s_seg[i].head, s_seg[i].parts, s_seg[i].slot0, red, p.stage_rows);
+        }
+        __syncthreads();                                  // the next heads' partials go where these were
+    }
+}
+
+template <int BITS, int U>
 static int launch_quant_mma(const AttendQuantParams &p, cudaStream_t st) {
-    attend_quant_mma_kernel<BITS, U, CTAS><<<dim3(p.splits, p.heads), 128, 0, st>>>(p);
+    auto kern = attend_quant_mma_kernel<BITS, U>;
+    constexpr int SMEM = QUANT_MAX_ROWS * PART_LD * 4;
+    static bool configured[64] = {};       // the attribute is kept per device
+    int dev = 0;
+    SKV_CUDA_OK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return SKV_E_RANGE;
+    if (!configured[dev]) {
+        SKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        configured[dev] = true;
+    }
+    SKV_CUDA_OK(launch_pdl(kern, dim3(p.ctas), dim3(128), (size_t)p.stage_rows * PART_LD * 4, st, p));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -475,24 +640,34 @@ static int launch_quant_simple(const AttendQuantParams &p, cudaStream_t st) {
 
 using namespace skv;
 
+extern "C" int skv_quant_ctas(void) { return QUANT_CTAS_PER_SM * device_sm_count(); }
+
+extern "C" int64_t skv_quant_workspace_bytes(int heads, int G, int d, int ctas) {
+    if (heads <= 0 || heads > 65535 || ctas <= 0 || ctas > 65535) return SKV_E_RANGE;
+    if (d != HEAD_DIM || G < 1 || G > 8) return SKV_E_DIM;
+    return ((int64_t)ctas + heads) * G * PART_LD * 4 + ((int64_t)heads * 4 + 255) / 256 * 256;
+}
+
 extern "C" int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, int G, const int32_t *n_dev, int n_group,
-                                void *out, void *workspace, int splits, float scale, void *stream) {
+                                void *out, void *workspace, int ctas, float scale, void *stream) {
     const int rc = qcache_check(c);
     if (rc) return rc;
     if (!q || !n_dev || !out || !workspace) return SKV_E_NULL;
     if (dtype != SKV_BF16 && dtype != SKV_F32) return SKV_E_DTYPE;
     if (G < 1 || G > 8) return SKV_E_DIM;
-    if (splits <= 0 || splits > 65535 || n_group < 0) return SKV_E_RANGE;
+    if (ctas <= 0 || ctas > 65535 || n_group < 0) return SKV_E_RANGE;
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return SKV_E_ALIGN;
     AttendQuantParams p;
-    p.heads = c->batch * c->h_kv; p.G = G; p.n_group = n_group; p.capacity = c->capacity; p.splits = splits;
+    p.heads = c->batch * c->h_kv; p.G = G; p.n_group = n_group; p.capacity = c->capacity;
+    p.ctas = ctas; p.splits = (ctas + p.heads) / p.heads;
+    p.stage_rows = quant_stage_rows(p.heads, G, ctas);
     p.q = q; p.out = out; p.n_dev = n_dev;
     p.kc = static_cast<const unsigned char *>(c->k); p.vc = static_cast<const unsigned char *>(c->v);
     p.scale = static_cast<const __nv_bfloat16 *>(c->scale);
     p.part = static_cast<float *>(workspace);
-    p.ticket = reinterpret_cast<int32_t *>(p.part + (int64_t)p.heads * splits * G * PART_LD);
+    p.ticket = reinterpret_cast<int32_t *>(p.part + ((int64_t)ctas + p.heads) * G * PART_LD);
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_F32) return c->bits == 8 ? launch_quant_simple<float, 8>(p, st) : launch_quant_simple<float, 4>(p, st);
-    return c->bits == 8 ? launch_quant_mma<8, 2, 3>(p, st) : launch_quant_mma<4, 2, 3>(p, st);
+    return c->bits == 8 ? launch_quant_mma<8, 2>(p, st) : launch_quant_mma<4, 2>(p, st);
 }

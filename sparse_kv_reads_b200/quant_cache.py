@@ -158,8 +158,8 @@ class QuantAttentionGraph:
         self.dtype, self.device = dtype, torch.device(device)
         self._code = dtype_code(dtype)
         with on_device(self.device):
-            self.num_splits = L.skv_attend_splits(H_kv)
-            size = L.skv_attend_workspace_bytes(H_kv, self.G, d, self.num_splits)
+            self.ctas = L.skv_quant_ctas()
+            size = L.skv_quant_workspace_bytes(H_kv, self.G, d, self.ctas)
             if size < 0:
                 raise SkvError(L.skv_error_string(int(size)).decode())
             self.ws = torch.zeros(size, dtype=torch.uint8, device=device)
@@ -180,6 +180,6 @@ class QuantAttentionGraph:
             q = q.clone(memory_format=torch.contiguous_format)
         with on_device(q.device):
             check(lib().skv_attend_quant(cache._st[layer], q.data_ptr(), self._code, self.G, n_dev.data_ptr(),
-                                         self.n_group, self.out.data_ptr(), self.ws.data_ptr(), self.num_splits,
+                                         self.n_group, self.out.data_ptr(), self.ws.data_ptr(), self.ctas,
                                          self._scale, stream_ptr(q.device)), "skv_attend_quant")
         return self.out

@@ -84,19 +84,21 @@ def test_the_decode_steps_write_is_refused_on_the_host(L):
 
 
 def test_attention_over_quantised_rows_is_refused_on_the_host(L):
-    args = dict(q=OK, dtype=0, G=2, n=OK, ng=0, out=OK, ws=OK, splits=4)
+    args = dict(q=OK, dtype=0, G=2, n=OK, ng=0, out=OK, ws=OK, ctas=4)
 
     def call(c=None, **o):
         a = {**args, **o}
         return L.skv_attend_quant(qcache() if c is None else c, a["q"], a["dtype"], a["G"], a["n"], a["ng"], a["out"],
-                                  a["ws"], a["splits"], 0.1, None)
+                                  a["ws"], a["ctas"], 0.1, None)
 
     for over, code in BAD_CACHES:
         assert call(qcache(**over)) == code, over
     for name in ("q", "n", "out", "ws"):
         assert call(**{name: None}) == -1
-    assert call(dtype=2) == -3 and call(G=0) == -2 and call(G=9) == -2 and call(splits=0) == -5 and call(ng=-1) == -5
+    assert call(dtype=2) == -3 and call(G=0) == -2 and call(G=9) == -2 and call(ctas=0) == -5 and call(ng=-1) == -5
     assert call(q=0x1008) == -4 and call(out=0x1002) == -4 and call(ws=0x1008) == -4
+    assert L.skv_quant_ctas() == 3 * 148 and L.skv_quant_workspace_bytes(8, 2, 128, 444) == 452 * 2 * 528 + 256
+    assert L.skv_quant_workspace_bytes(0, 2, 128, 4) == -5 and L.skv_quant_workspace_bytes(8, 9, 128, 4) == -2
 
 
 def test_attention_over_a_shared_prefix_is_refused_on_the_host(L):
@@ -164,6 +166,8 @@ def test_attention_objects_check_their_arguments(L):
         QuantAttentionGraph(H=5, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
     with pytest.raises(ValueError, match="divide"):
         PrefixAttentionGraph(B=1, H=5, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
+    with pytest.raises(_lib.SkvError):
+        QuantAttentionGraph(H=18, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
     with pytest.raises(_lib.SkvError):
         PrefixAttentionGraph(B=1, H=18, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
     with pytest.raises(ValueError, match="unsupported"):

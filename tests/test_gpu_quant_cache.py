@@ -417,9 +417,7 @@ def test_refused_on_the_gpu_too():
     with pytest.raises(ValueError, match="plain cache"):
         GraphDecoder(model, model.alloc_cache(64, bits=8), mode="cluster")
     with pytest.raises(SkvError):
-        QuantAttentionGraph(H=18, H_kv=2, d=128, dtype=torch.bfloat16, device=DEV)(
-            torch.zeros(18, 128, dtype=torch.bfloat16, device=DEV), QuantKVCache(1, 1, 2, 8, 128, 8, DEV), 0,
-            torch.zeros(1, dtype=torch.int32, device=DEV))
+        QuantAttentionGraph(H=18, H_kv=2, d=128, dtype=torch.bfloat16, device=DEV)
     cache = QuantKVCache(1, 1, 2, 8, 128, 8, DEV)
     x = torch.zeros(1, 2, 1, 128, dtype=torch.bfloat16, device=DEV, requires_grad=True)
     with pytest.raises(ValueError, match="no gradient"):

@@ -1,10 +1,15 @@
 // Attention of one new token per sequence over a prefix that all sequences share (its cache rows exist once) and over
 // each sequence's own rows behind it.
 //
-// Simple kernel: a (sequence, KV head) pair walks the prefix and its own rows as one list, half a warp per row, float32
+// bf16, two launches.  The first reads the prefix once per KV head for all sequences together: their batch x G query rows
+// are the M side of tcgen05 products over 128-key tiles (prefix_mma_kernel, below).  The second attends over the own rows,
+// one CTA per (split, sequence, KV head), and its last CTA per head merges everything.
+// float32: a (sequence, KV head) pair walks the prefix and its own rows as one list, half a warp per row, float32
 // arithmetic on the CUDA cores.
+#include <cuda.h>
+
 #include "skv_attend_finish.cuh"
-#include "skv_common.cuh"
+#include "skv_tcgen05.cuh"
 
 namespace skv {
 
@@ -12,10 +17,11 @@ struct PrefixParams {
     const void *q, *kp, *vp, *k, *v;
     const int32_t *n_dev;
     void *out;
-    float *part;       // [batch * h_kv, splits, G, 132]
+    float *part;       // [batch * h_kv, splits, G, 132]: the prefix's partials, then the own rows'
     int32_t *ticket;   // [batch * h_kv]
     int32_t *status;
     int batch, h_kv, G, n_group, prefix, rows_limit, splits;
+    int prefix_splits, own_splits;      // bf16: prefix_splits + own_splits <= splits
     int64_t kph, kpr, vph, vpr, ksh, ksr, vsh, vsr;
     float scale_log2;
 };
@@ -94,6 +100,328 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
     finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
 }
 
+// ---------------------------------------------------------------------------------------------
+// The prefix, bf16: rows of all sequences together on the tensor cores
+// ---------------------------------------------------------------------------------------------
+// A CTA (one per SM) serves one KV head, a run of 128-key tiles and up to 256 query rows.  Two warpgroups of softmax threads
+// have an accumulator each (slot 0 and 1): with more than 128 query rows they take 128 rows each of every tile, else both
+// have the same rows and take the tiles in turn, and are merged at the end.  A thread owns one row: it reads its 128 scores
+// from tensor memory, so that no maximum needs a shuffle, and writes the weights back over them in bf16 as the A operand of
+// the second product.  One thread feeds the ring of K and V tiles by TMA (rows beyond the prefix read as zeros), one issues
+//   S = Q K^T  (both K-major in shared memory)        O += P V  (P in tensor memory, V MN-major)
+// with S of the next tile issued before O of this one has to wait for its weights: the slots' softmax and products overlap.
+// Accumulators are rescaled only when a row's maximum rises by more than 8 (base 2).
+constexpr int PT = 128;                                   // keys of a tile, rows of a slot
+constexpr int PSTAGES = 2;
+constexpr uint32_t P_TILE = PT * 256;                     // bytes of a 128 x 128 bf16 tile: two halves of 64 components
+constexpr uint32_t P_OUT = PT * PART_LD * 4;              // bytes of a slot's float32 rows on their way out
+constexpr uint32_t P_SMEM = 2 * P_TILE + PSTAGES * 2 * P_TILE + 1024;
+static_assert(2 * P_OUT <= 2 * P_TILE + PSTAGES * 2 * P_TILE, "the rows on their way out lie over the tiles");
+
+struct PrefixBars {
+    uint64_t kfull[PSTAGES], vfull[PSTAGES], kempty[PSTAGES], vempty[PSTAGES];
+    uint64_t sfull[2], pfull[2], done[2], drain;
+};
+
+__global__ void __launch_bounds__(320, 1)
+prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ unsigned char raw[];
+    __shared__ PrefixBars bars;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_fail;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char *const smem = raw + (base - smem_u32(raw));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x, h = blockIdx.z;
+    const int rows = p.batch * p.G, row0 = blockIdx.y * 2 * PT;
+    const bool both = rows - row0 <= PT;                  // one set of rows: the slots take the tiles in turn
+    const int tiles = (p.prefix + PT - 1) / PT;
+    const int t0 = (int)((int64_t)tiles * split / p.prefix_splits), t1 = (int)((int64_t)tiles * (split + 1) / p.prefix_splits);
+    const int n = t1 - t0;
+    const uint32_t kbase = base + 2 * P_TILE;
+    const uint32_t b_kfull = smem_u32(bars.kfull), b_vfull = smem_u32(bars.vfull), b_kempty = smem_u32(bars.kempty),
+                   b_vempty = smem_u32(bars.vempty), b_sfull = smem_u32(bars.sfull), b_pfull = smem_u32(bars.pfull),
+                   b_done = smem_u32(bars.done), b_drain = smem_u32(&bars.drain);
+    if (tid == 256) {
+        for (int i = 0; i < PSTAGES; ++i) {
+            mbar_init(b_kfull + 8 * i, 1); mbar_init(b_vfull + 8 * i, 1);
+            mbar_init(b_kempty + 8 * i, 1); mbar_init(b_vempty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(b_sfull + 8 * i, 1); mbar_init(b_pfull + 8 * i, PT); mbar_init(b_done + 8 * i, 1);
+        }
+        mbar_init(b_drain, 1);
+        s_fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_proxy();
+    }
+    if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
+    pdl_wait();
+    pdl_trigger();
+    // Queries into the 128-byte swizzle, 16 bytes at a time; rows beyond the last are zero.  A negative softmax scale goes
+    // into their sign: the running maximum is one of scaled scores.
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+    const int qrows = both ? PT : 2 * PT;
+    for (int i = tid; i < qrows * 16; i += 320) {
+        const int r = i >> 4, c = i & 15, row = row0 + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows) {
+            const int b = row / p.G, g = row - b * p.G;
+            v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.q) +
+                                                 (((int64_t)b * p.h_kv + h) * p.G + g) * HEAD_DIM + c * 8);
+            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        }
+        const int rr = r & (PT - 1);
+        *reinterpret_cast<uint4 *>(smem + (r >> 7) * P_TILE + (c >> 3) * (P_TILE / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+    }
+    fence_async_proxy();
+    tcgen05_before_sync();
+    __syncthreads();
+    tcgen05_after_sync();
+    const uint32_t tmem = s_tmem;
+
+    if (warp == 8) {
+        // ---- tiles, by TMA ----
+        if (lane == 0) {
+            int i = 0;
+            bool ok = true;
+            for (; i < n; ++i) {
+                const int s = i % PSTAGES;
+                const uint32_t kt = kbase + s * 2 * P_TILE, vt = kt + P_TILE, turn = (i / PSTAGES - 1) & 1;
+                if (i >= PSTAGES && !(ok = mbar_wait(b_kempty + 8 * s, turn))) break;
+                mbar_expect(b_kfull + 8 * s, P_TILE);
+                tma_load_3d(kt, &kmap, b_kfull + 8 * s, 0, (t0 + i) * PT, h);
+                tma_load_3d(kt + P_TILE / 2, &kmap, b_kfull + 8 * s, 64, (t0 + i) * PT, h);
+                if (i >= PSTAGES && !(ok = mbar_wait(b_vempty + 8 * s, turn))) {
+                    mbar_wait(b_kfull + 8 * s, (i / PSTAGES) & 1);
+                    break;
+                }
+                mbar_expect(b_vfull + 8 * s, P_TILE);
+                tma_load_3d(vt, &vmap, b_vfull + 8 * s, 0, (t0 + i) * PT, h);
+                tma_load_3d(vt + P_TILE / 2, &vmap, b_vfull + 8 * s, 64, (t0 + i) * PT, h);
+            }
+            if (!ok) s_fail = 1;
+            for (int j = max(0, i - PSTAGES); j < i; ++j) {            // no copy is in flight when the CTA ends
+                mbar_wait(b_kfull + 8 * (j % PSTAGES), (j / PSTAGES) & 1);
+                mbar_wait(b_vfull + 8 * (j % PSTAGES), (j / PSTAGES) & 1);
+            }
+        }
+    } else if (warp == 9) {
+        // ---- products ----
+        if (lane == 0) {
+            constexpr uint32_t ID_S = idesc_bf16(PT, PT, false), ID_O = idesc_bf16(PT, HEAD_DIM, true);
+            bool ok = true;
+            // slot w's scores of tile i; `free_k`: nothing reads the key tile afterwards
+            auto scores = [&](int i, int w, bool free_k) {
+                const int s = i % PSTAGES;
+                if (!ok || !(ok = mbar_wait(b_kfull + 8 * s, (i / PSTAGES) & 1))) return;
+                tcgen05_after_sync();
+                const uint32_t qt = base + (both ? 0 : w) * P_TILE, kt = kbase + s * 2 * P_TILE;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t at = (k >> 2) * (P_TILE / 2) + (k & 3) * 32;
+                    mma_ss(tmem + w * PT, smem_desc(qt + at, 1024), smem_desc(kt + at, 1024), ID_S, k > 0);
+                }
+                tcgen05_commit(b_sfull + 8 * w);
+                if (free_k) tcgen05_commit(b_kempty + 8 * s);
+            };
+            // slot w's weighted values of tile i, its turn number j
+            auto values = [&](int i, int w, int j, bool free_v, bool last) {
+                const int s = i % PSTAGES;
+                if (!ok || !(ok = mbar_wait(b_pfull + 8 * w, j & 1)) || !(ok = mbar_wait(b_vfull + 8 * s, (i / PSTAGES) & 1)))
+                    return;
+                tcgen05_after_sync();
+                const uint32_t vt = kbase + s * 2 * P_TILE + P_TILE;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    mma_ts(tmem + 256 + w * PT, tmem + w * PT + k * 8, smem_desc(vt + k * 2048, 1024, P_TILE / 2), ID_O,
+                           j > 0 || k > 0);
+                if (free_v) tcgen05_commit(b_vempty + 8 * s);
+                if (last) tcgen05_commit(b_done + 8 * w);
+            };
+            if (both) {
+                scores(0, 0, true);
+                if (n > 1) scores(1, 1, true);
+                for (int i = 0; i < n; ++i) {
+                    values(i, i & 1, i >> 1, true, i + 2 >= n);
+                    if (i + 2 < n) scores(i + 2, i & 1, true);
+                }
+            } else {
+                scores(0, 0, false);
+                scores(0, 1, true);
+                for (int i = 0; i < n; ++i)
+                    for (int w = 0; w < 2; ++w) {
+                        values(i, w, i, w == 1, i + 1 == n);
+                        if (i + 1 < n) scores(i + 1, w, w == 1);
+                    }
+            }
+            if (!ok) s_fail = 1;
+            tcgen05_commit(b_drain);                      // no product is in flight when the CTA ends
+            mbar_wait(b_drain, 0);
+        }
+    } else {
+        // ---- softmax: one row per thread ----
+        const int w = warp >> 2, r = tid & (PT - 1);
+        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);        // this warp's 32 lanes
+        const uint32_t sc = mine + w * PT, oc = mine + 256 + w * PT;
+        const float scale = fabsf(p.scale_log2);
+        const int turns = both ? (n - w + 1) / 2 : n;
+        float m = NEG_BIG, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < turns; ++j) {
+            const int i = both ? 2 * j + w : j;
+            if (!(ok = mbar_wait_warp(b_sfull + 8 * w, j & 1))) break;
+            tcgen05_after_sync();
+            uint32_t x[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(sc + c * 32, x[c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld_done(x[c]);
+            const int left = p.prefix - (t0 + i) * PT;    // keys of this tile
+            if (left < PT) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (c * 32 + e >= left) x[c][e] = 0xff800000u;
+            }
+            float top[4] = {NEG_BIG, NEG_BIG, NEG_BIG, NEG_BIG};
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][e]));
+            const float z = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+            if (__any_sync(0xffffffffu, z > m + 8.f)) {
+                const float nm = fmaxf(m, z), al = fast_exp2(m - nm);
+                m = nm;
+                l *= al;
+                if (j > 0) {                              // (the products up to the tile before have ended: S came after them)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(oc + c * 32, o);
+                        tmem_ld_done(o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+                        tmem_st32(oc + c * 32, o);
+                    }
+                }
+            }
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float a = fast_exp2(fmaf(__uint_as_float(x[c][e]), scale, -m));
+                    const float b = fast_exp2(fmaf(__uint_as_float(x[c][e + 1]), scale, -m));
+                    sum[(e >> 1) & 3] += a + b;
+                    pk[e >> 1] = pack_bf16(a, b);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[c >> 1][(c & 1) * 16 + e] = pk[e];
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st32(sc, x[0]);
+            tmem_st32(sc + 32, x[1]);
+            tcgen05_wait_st();
+            tcgen05_before_sync();
+            mbar_arrive(b_pfull + 8 * w);
+        }
+        if (ok && turns > 0) ok = mbar_wait_warp(b_done + 8 * w, 0);
+        if (!ok) s_fail = 1;
+        tcgen05_after_sync();
+        asm volatile("bar.sync 1, 256;" ::: "memory");    // both slots' products have ended: the tiles' memory is free
+        float *out = reinterpret_cast<float *>(smem + w * P_OUT) + r * PART_LD;
+        const bool fold = both && n > 1;                  // slot 1's rows are folded into slot 0's
+        if (turns > 0 && !(fold && w == 0)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                tmem_ld32(oc + c * 32, o);
+                tmem_ld_done(o);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<uint4 *>(out + c * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+            *reinterpret_cast<float4 *>(out + HEAD_DIM) = make_float4(m, l, 0.f, 0.f);
+        }
+        if (fold) {
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (w == 0) {
+                const float *other = reinterpret_cast<const float *>(smem + P_OUT) + r * PART_LD;
+                const float4 ml = *reinterpret_cast<const float4 *>(other + HEAD_DIM);
+                const float M = fmaxf(m, ml.x), f0 = fast_exp2(m - M), f1 = fast_exp2(ml.x - M);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(oc + c * 32, o);
+                    tmem_ld_done(o);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 a = *reinterpret_cast<const float4 *>(other + c * 32 + e);
+                        *reinterpret_cast<float4 *>(out + c * 32 + e) =
+                            make_float4(fmaf(f1, a.x, f0 * __uint_as_float(o[e])), fmaf(f1, a.y, f0 * __uint_as_float(o[e + 1])),
+                                        fmaf(f1, a.z, f0 * __uint_as_float(o[e + 2])), fmaf(f1, a.w, f0 * __uint_as_float(o[e + 3])));
+                    }
+                }
+                *reinterpret_cast<float4 *>(out + HEAD_DIM) = make_float4(M, fmaf(f1, ml.y, f0 * l), 0.f, 0.f);
+            }
+        }
+        const int row = row0 + (both ? 0 : w * PT) + r;
+        if (row < rows && turns > 0 && !(both && w == 1)) {
+            const int b = row / p.G, g = row - b * p.G;
+            fence_async_proxy();
+            bulk_store(p.part + ((((int64_t)b * p.h_kv + h) * p.splits + split) * p.G + g) * PART_LD, smem_u32(out), PART_LD * 4);
+            bulk_store_wait();
+        }
+        tcgen05_before_sync();
+    }
+    __syncwarp();
+    __syncthreads();
+    if (s_fail && p.status && tid < p.batch) atomicOr(p.status + tid * p.h_kv + h, SKV_ST_WAIT_TIMEOUT);
+    if (warp == 9) {
+        tcgen05_after_sync();
+        tmem_free(tmem, 512);
+    }
+}
+
+// The sequences' own rows, and everything merged by the head's last CTA: grid (own splits, sequence x KV head).
+template <int STAGES>
+__global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p) {
+    constexpr int WARPS = 4;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint32_t s_vmask[WARPS][STAGES];
+    __shared__ int s_flag;
+    const int warp = threadIdx.x >> 5, head = blockIdx.y, split = blockIdx.x;
+    const int n = own_rows(p, head);
+    const int tiles = (n + TILE_ROWS - 1) / TILE_ROWS;
+    const int s_eff = min(p.own_splits, max(1, (tiles + WARPS - 1) / WARPS));
+    if (split >= s_eff) return;
+    const int slots = s_eff * WARPS, per = (tiles + slots - 1) / slots;
+    const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
+    WarpAttendT<STAGES> wa;
+    wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * p.G * HEAD_DIM, p.G, smem + warp * (STAGES * 8192),
+            s_vmask[warp], static_cast<const char *>(p.k) + (int64_t)head * p.ksh * 2,
+            static_cast<const char *>(p.v) + (int64_t)head * p.vsh * 2, p.ksr * 2, p.vsr * 2, p.scale_log2);
+    wa.run(t0, t1, [&](int row) { return row < n ? row : -1; });
+    __syncthreads();
+    float *red = reinterpret_cast<float *>(smem);
+    wa.store_partial(red, warp, p.G);
+    __syncthreads();
+    const int parts = p.prefix_splits + s_eff;
+    const int64_t slot0 = (int64_t)head * p.splits;
+    publish_head<__nv_bfloat16>(p, red, WARPS, head, p.prefix_splits + split, parts, slot0);
+    if (parts == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) s_flag = s_eff == 1 || atomicAdd(p.ticket + head, 1) == s_eff - 1;
+    __syncthreads();
+    if (!s_flag) return;
+    __threadfence();
+    merge_head<__nv_bfloat16>(p, head, parts, slot0, red, WARPS * STAGES * 8192 / (PART_LD * 4));
+}
+
 template <typename T>
 static int launch_prefix_simple(const PrefixParams &p, cudaStream_t st) {
     const dim3 grid(p.splits, p.batch * p.h_kv);
@@ -101,6 +429,72 @@ static int launch_prefix_simple(const PrefixParams &p, cudaStream_t st) {
     else if (p.G <= 2) attend_prefix_simple_kernel<T, 2><<<grid, 128, 0, st>>>(p);
     else if (p.G <= 4) attend_prefix_simple_kernel<T, 4><<<grid, 128, 0, st>>>(p);
     else attend_prefix_simple_kernel<T, 8><<<grid, 128, 0, st>>>(p);
+    SKV_CUDA_OK(cudaGetLastError());
+    return SKV_OK;
+}
+
+constexpr int OWN_STAGES = 2, OWN_SMEM = 4 * OWN_STAGES * 8192;
+
+// Most CTAs the prefix of a KV head is split over: one per SM over all heads and row groups.
+static int prefix_splits_of(int batch, int h_kv, int G) {
+    const int groups = (batch * G + 2 * PT - 1) / (2 * PT), s = device_sm_count() / (h_kv * groups);
+    return s < 1 ? 1 : s;
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Map of [h_kv, prefix, 128] bf16 rows in boxes of 128 rows x 64 components, 128-byte swizzle; false where the strides or the
+// address do not allow one.
+static bool prefix_map(CUtensorMap *map, const void *x, int h_kv, int prefix, int64_t head_stride, int64_t row_stride) {
+    static EncodeTiled encode = nullptr;
+    if (!encode) {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            return false;
+        encode = reinterpret_cast<EncodeTiled>(fn);
+    }
+    if (prefix == 1) row_stride = HEAD_DIM;               // (a stride that no address uses may be anything)
+    if (h_kv == 1) head_stride = row_stride;
+    if (row_stride < HEAD_DIM || head_stride <= 0) return false;
+    const cuuint64_t dims[3] = {HEAD_DIM, (cuuint64_t)prefix, (cuuint64_t)h_kv};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_stride * 2, (cuuint64_t)head_stride * 2};
+    const cuuint32_t box[3] = {64, PT, 1}, unit[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(x), dims, strides, box, unit,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
+    const int tiles = (p.prefix + PT - 1) / PT;
+    int ps = prefix_splits_of(p.batch, p.h_kv, p.G);
+    ps = ps < tiles ? ps : tiles;
+    if (ps > p.splits - 1) ps = p.splits - 1;
+    int own = skv_attend_splits(p.batch * p.h_kv);
+    if (own > p.splits - ps) own = p.splits - ps;
+    p.prefix_splits = ps;
+    p.own_splits = own;
+    CUtensorMap kmap, vmap;
+    if (ps > 0 && (!prefix_map(&kmap, p.kp, p.h_kv, p.prefix, p.kph, p.kpr) ||
+                   !prefix_map(&vmap, p.vp, p.h_kv, p.prefix, p.vph, p.vpr)))
+        return launch_prefix_simple<__nv_bfloat16>(p, st);
+    static bool configured[64] = {};       // the attributes are kept per device
+    int dev = 0;
+    SKV_CUDA_OK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return SKV_E_RANGE;
+    if (!configured[dev]) {
+        SKV_CUDA_OK(cudaFuncSetAttribute(prefix_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM));
+        SKV_CUDA_OK(cudaFuncSetAttribute(prefix_own_kernel<OWN_STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, OWN_SMEM));
+        configured[dev] = true;
+    }
+    if (ps > 0) {
+        const int groups = (p.batch * p.G + 2 * PT - 1) / (2 * PT);
+        SKV_CUDA_OK(launch_pdl(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(320), P_SMEM, st, p, kmap, vmap));
+    }
+    prefix_own_kernel<OWN_STAGES><<<dim3(own, p.batch * p.h_kv), 128, OWN_SMEM, st>>>(p);
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -113,7 +507,8 @@ extern "C" int skv_prefix_splits(int batch, int h_kv, int G, int dtype) {
     if (batch <= 0 || h_kv <= 0 || (int64_t)batch * h_kv > 65535) return SKV_E_RANGE;
     if (G < 1 || G > 8) return SKV_E_DIM;
     if (dtype != SKV_BF16 && dtype != SKV_F32) return SKV_E_DTYPE;
-    return skv_attend_splits(batch * h_kv);
+    const int own = skv_attend_splits(batch * h_kv);
+    return dtype == SKV_F32 ? own : own + prefix_splits_of(batch, h_kv, G);
 }
 
 extern "C" int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d, int splits) {
@@ -154,5 +549,7 @@ extern "C" int skv_attend_prefix(const void *q, const void *k_prefix, const void
     p.ksh = k_head_stride; p.ksr = k_row_stride; p.vsh = v_head_stride; p.vsr = v_row_stride;
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == SKV_F32 ? launch_prefix_simple<float>(p, st) : launch_prefix_simple<__nv_bfloat16>(p, st);
+    p.prefix_splits = p.own_splits = 0;
+    if (dtype == SKV_F32) return launch_prefix_simple<float>(p, st);
+    return splits > 1 ? launch_prefix_mma(p, st) : launch_prefix_simple<__nv_bfloat16>(p, st);
 }

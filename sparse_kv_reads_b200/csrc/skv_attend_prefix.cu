@@ -123,7 +123,11 @@ struct PrefixBars {
     uint64_t sfull[2], pfull[2], done[2], drain;
 };
 
-__global__ void __launch_bounds__(320, 1)
+// 384 threads at 168 registers: the softmax warpgroups take 232 each, the third (tiles, products, two idle warps) keeps 40:
+// 128 x (2 x 232 + 40) = 384 x 168.
+constexpr int P_THREADS = 384;
+
+__global__ void __launch_bounds__(P_THREADS, 1)
 prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ unsigned char raw[];
     __shared__ PrefixBars bars;
@@ -142,6 +146,12 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
     const uint32_t b_kfull = smem_u32(bars.kfull), b_vfull = smem_u32(bars.vfull), b_kempty = smem_u32(bars.kempty),
                    b_vempty = smem_u32(bars.vempty), b_sfull = smem_u32(bars.sfull), b_pfull = smem_u32(bars.pfull),
                    b_done = smem_u32(bars.done), b_drain = smem_u32(&bars.drain);
+    // one tile's K or V, two boxes of 64 components
+    auto load = [&](const CUtensorMap &map, uint32_t dst, uint32_t bar, int tile) {
+        mbar_expect(bar, P_TILE);
+        tma_load_3d(dst, &map, bar, 0, tile * PT, h);
+        tma_load_3d(dst + P_TILE / 2, &map, bar, 64, tile * PT, h);
+    };
     if (tid == 256) {
         for (int i = 0; i < PSTAGES; ++i) {
             mbar_init(b_kfull + 8 * i, 1); mbar_init(b_vfull + 8 * i, 1);
@@ -154,6 +164,11 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
         s_fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_proxy();
+        // the first tiles are on their way before anything else: no earlier kernel of the same step writes the prefix
+        for (int i = 0; i < min(n, PSTAGES); ++i) {
+            load(kmap, kbase + i * 2 * P_TILE, b_kfull + 8 * i, t0 + i);
+            load(vmap, kbase + i * 2 * P_TILE + P_TILE, b_vfull + 8 * i, t0 + i);
+        }
     }
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
     pdl_wait();
@@ -162,7 +177,8 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
     // into their sign: the running maximum is one of scaled scores.
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
     const int qrows = both ? PT : 2 * PT;
-    for (int i = tid; i < qrows * 16; i += 320) {
+    #pragma unroll 4
+    for (int i = tid; i < qrows * 16; i += P_THREADS) {
         const int r = i >> 4, c = i & 15, row = row0 + r;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (row < rows) {
@@ -180,87 +196,87 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
     tcgen05_after_sync();
     const uint32_t tmem = s_tmem;
 
-    if (warp == 8) {
-        // ---- tiles, by TMA ----
-        if (lane == 0) {
-            int i = 0;
-            bool ok = true;
-            for (; i < n; ++i) {
-                const int s = i % PSTAGES;
-                const uint32_t kt = kbase + s * 2 * P_TILE, vt = kt + P_TILE, turn = (i / PSTAGES - 1) & 1;
-                if (i >= PSTAGES && !(ok = mbar_wait(b_kempty + 8 * s, turn))) break;
-                mbar_expect(b_kfull + 8 * s, P_TILE);
-                tma_load_3d(kt, &kmap, b_kfull + 8 * s, 0, (t0 + i) * PT, h);
-                tma_load_3d(kt + P_TILE / 2, &kmap, b_kfull + 8 * s, 64, (t0 + i) * PT, h);
-                if (i >= PSTAGES && !(ok = mbar_wait(b_vempty + 8 * s, turn))) {
-                    mbar_wait(b_kfull + 8 * s, (i / PSTAGES) & 1);
-                    break;
-                }
-                mbar_expect(b_vfull + 8 * s, P_TILE);
-                tma_load_3d(vt, &vmap, b_vfull + 8 * s, 0, (t0 + i) * PT, h);
-                tma_load_3d(vt + P_TILE / 2, &vmap, b_vfull + 8 * s, 64, (t0 + i) * PT, h);
-            }
-            if (!ok) s_fail = 1;
-            for (int j = max(0, i - PSTAGES); j < i; ++j) {            // no copy is in flight when the CTA ends
-                mbar_wait(b_kfull + 8 * (j % PSTAGES), (j / PSTAGES) & 1);
-                mbar_wait(b_vfull + 8 * (j % PSTAGES), (j / PSTAGES) & 1);
-            }
-        }
-    } else if (warp == 9) {
-        // ---- products ----
-        if (lane == 0) {
-            constexpr uint32_t ID_S = idesc_bf16(PT, PT, false), ID_O = idesc_bf16(PT, HEAD_DIM, true);
-            bool ok = true;
-            // slot w's scores of tile i; `free_k`: nothing reads the key tile afterwards
-            auto scores = [&](int i, int w, bool free_k) {
-                const int s = i % PSTAGES;
-                if (!ok || !(ok = mbar_wait(b_kfull + 8 * s, (i / PSTAGES) & 1))) return;
-                tcgen05_after_sync();
-                const uint32_t qt = base + (both ? 0 : w) * P_TILE, kt = kbase + s * 2 * P_TILE;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t at = (k >> 2) * (P_TILE / 2) + (k & 3) * 32;
-                    mma_ss(tmem + w * PT, smem_desc(qt + at, 1024), smem_desc(kt + at, 1024), ID_S, k > 0);
-                }
-                tcgen05_commit(b_sfull + 8 * w);
-                if (free_k) tcgen05_commit(b_kempty + 8 * s);
-            };
-            // slot w's weighted values of tile i, its turn number j
-            auto values = [&](int i, int w, int j, bool free_v, bool last) {
-                const int s = i % PSTAGES;
-                if (!ok || !(ok = mbar_wait(b_pfull + 8 * w, j & 1)) || !(ok = mbar_wait(b_vfull + 8 * s, (i / PSTAGES) & 1)))
-                    return;
-                tcgen05_after_sync();
-                const uint32_t vt = kbase + s * 2 * P_TILE + P_TILE;
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    mma_ts(tmem + 256 + w * PT, tmem + w * PT + k * 8, smem_desc(vt + k * 2048, 1024, P_TILE / 2), ID_O,
-                           j > 0 || k > 0);
-                if (free_v) tcgen05_commit(b_vempty + 8 * s);
-                if (last) tcgen05_commit(b_done + 8 * w);
-            };
-            if (both) {
-                scores(0, 0, true);
-                if (n > 1) scores(1, 1, true);
-                for (int i = 0; i < n; ++i) {
-                    values(i, i & 1, i >> 1, true, i + 2 >= n);
-                    if (i + 2 < n) scores(i + 2, i & 1, true);
-                }
-            } else {
-                scores(0, 0, false);
-                scores(0, 1, true);
-                for (int i = 0; i < n; ++i)
-                    for (int w = 0; w < 2; ++w) {
-                        values(i, w, i, w == 1, i + 1 == n);
-                        if (i + 1 < n) scores(i + 1, w, w == 1);
+    if (warp >= 8) {
+        fewer_registers<40>();
+        if (warp == 8) {
+            // ---- tiles, by TMA ----
+            if (lane == 0) {
+                int i = min(n, PSTAGES);
+                bool ok = true;
+                for (; i < n; ++i) {
+                    const int s = i % PSTAGES;
+                    const uint32_t kt = kbase + s * 2 * P_TILE, turn = (i / PSTAGES - 1) & 1;
+                    if (!(ok = mbar_wait(b_kempty + 8 * s, turn))) break;
+                    load(kmap, kt, b_kfull + 8 * s, t0 + i);
+                    if (!(ok = mbar_wait(b_vempty + 8 * s, turn))) {
+                        mbar_wait(b_kfull + 8 * s, (i / PSTAGES) & 1);
+                        break;
                     }
+                    load(vmap, kt + P_TILE, b_vfull + 8 * s, t0 + i);
+                }
+                if (!ok) s_fail = 1;
+                for (int j = max(0, i - PSTAGES); j < i; ++j) {            // no copy is in flight when the CTA ends
+                    mbar_wait(b_kfull + 8 * (j % PSTAGES), (j / PSTAGES) & 1);
+                    mbar_wait(b_vfull + 8 * (j % PSTAGES), (j / PSTAGES) & 1);
+                }
             }
-            if (!ok) s_fail = 1;
-            tcgen05_commit(b_drain);                      // no product is in flight when the CTA ends
-            mbar_wait(b_drain, 0);
+        } else if (warp == 9) {
+            // ---- products ----
+            if (lane == 0) {
+                constexpr uint32_t ID_S = idesc_bf16(PT, PT, false), ID_O = idesc_bf16(PT, HEAD_DIM, true);
+                bool ok = true;
+                // slot w's scores of tile i; `free_k`: nothing reads the key tile afterwards
+                auto scores = [&](int i, int w, bool free_k) {
+                    const int s = i % PSTAGES;
+                    if (!ok || !(ok = mbar_wait(b_kfull + 8 * s, (i / PSTAGES) & 1))) return;
+                    tcgen05_after_sync();
+                    const uint32_t qt = base + (both ? 0 : w) * P_TILE, kt = kbase + s * 2 * P_TILE;
+    #pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t at = (k >> 2) * (P_TILE / 2) + (k & 3) * 32;
+                        mma_ss(tmem + w * PT, smem_desc(qt + at, 1024), smem_desc(kt + at, 1024), ID_S, k > 0);
+                    }
+                    tcgen05_commit(b_sfull + 8 * w);
+                    if (free_k) tcgen05_commit(b_kempty + 8 * s);
+                };
+                // slot w's weighted values of tile i, its turn number j
+                auto values = [&](int i, int w, int j, bool free_v, bool last) {
+                    const int s = i % PSTAGES;
+                    if (!ok || !(ok = mbar_wait(b_pfull + 8 * w, j & 1)) || !(ok = mbar_wait(b_vfull + 8 * s, (i / PSTAGES) & 1)))
+                        return;
+                    tcgen05_after_sync();
+                    const uint32_t vt = kbase + s * 2 * P_TILE + P_TILE;
+    #pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        mma_ts(tmem + 256 + w * PT, tmem + w * PT + k * 8, smem_desc(vt + k * 2048, 1024, P_TILE / 2), ID_O,
+                               j > 0 || k > 0);
+                    if (free_v) tcgen05_commit(b_vempty + 8 * s);
+                    if (last) tcgen05_commit(b_done + 8 * w);
+                };
+                if (both) {
+                    scores(0, 0, true);
+                    if (n > 1) scores(1, 1, true);
+                    for (int i = 0; i < n; ++i) {
+                        values(i, i & 1, i >> 1, true, i + 2 >= n);
+                        if (i + 2 < n) scores(i + 2, i & 1, true);
+                    }
+                } else {
+                    scores(0, 0, false);
+                    scores(0, 1, true);
+                    for (int i = 0; i < n; ++i)
+                        for (int w = 0; w < 2; ++w) {
+                            values(i, w, i, w == 1, i + 1 == n);
+                            if (i + 1 < n) scores(i + 1, w, w == 1);
+                        }
+                }
+                if (!ok) s_fail = 1;
+                tcgen05_commit(b_drain);                      // no product is in flight when the CTA ends
+                mbar_wait(b_drain, 0);
+            }
         }
     } else {
         // ---- softmax: one row per thread ----
+        more_registers<232>();
         const int w = warp >> 2, r = tid & (PT - 1);
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);        // this warp's 32 lanes
         const uint32_t sc = mine + w * PT, oc = mine + 256 + w * PT;
@@ -287,43 +303,44 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
             }
             float top[4] = {NEG_BIG, NEG_BIG, NEG_BIG, NEG_BIG};
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][e]));
+                for (int c = 0; c < 4; ++c)
+                    top[c] = fmaxf(fmaxf(top[c], __uint_as_float(x[c][e])), __uint_as_float(x[c][e + 1]));
             const float z = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
             if (__any_sync(0xffffffffu, z > m + 8.f)) {
                 const float nm = fmaxf(m, z), al = fast_exp2(m - nm);
                 m = nm;
                 l *= al;
                 if (j > 0) {                              // (the products up to the tile before have ended: S came after them)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(oc + c * 32, o);
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(oc + c * 16, o);
                         tmem_ld_done(o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
-                        tmem_st32(oc + c * 32, o);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+                        tmem_st16(oc + c * 16, o);
                     }
                 }
             }
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 sum[4] = {};
+            const float2 mul = make_float2(scale, scale), sub = make_float2(-m, -m);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
-                    const float a = fast_exp2(fmaf(__uint_as_float(x[c][e]), scale, -m));
-                    const float b = fast_exp2(fmaf(__uint_as_float(x[c][e + 1]), scale, -m));
-                    sum[(e >> 1) & 3] += a + b;
-                    pk[e >> 1] = pack_bf16(a, b);
+                    float2 a = fma2(make_float2(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), mul, sub);
+                    a.x = fast_exp2(a.x);
+                    a.y = fast_exp2(a.y);
+                    sum[(e >> 1) & 3] = add2(sum[(e >> 1) & 3], a);
+                    pk[e >> 1] = pack_bf16(a.x, a.y);
                 }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[c >> 1][(c & 1) * 16 + e] = pk[e];
+                tmem_st16(sc + c * 16, pk);               // over scores that are in registers by now
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st32(sc, x[0]);
-            tmem_st32(sc + 32, x[1]);
+            const float2 all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+            l += all.x + all.y;
             tcgen05_wait_st();
             tcgen05_before_sync();
             mbar_arrive(b_pfull + 8 * w);
@@ -397,7 +414,10 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
     const int n = own_rows(p, head);
     const int tiles = (n + TILE_ROWS - 1) / TILE_ROWS;
     const int s_eff = min(p.own_splits, max(1, (tiles + WARPS - 1) / WARPS));
-    if (split >= s_eff) return;
+    if (split >= s_eff) {
+        pdl_wait();
+        return;
+    }
     const int slots = s_eff * WARPS, per = (tiles + slots - 1) / slots;
     const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
     WarpAttendT<STAGES> wa;
@@ -411,6 +431,7 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
     __syncthreads();
     const int parts = p.prefix_splits + s_eff;
     const int64_t slot0 = (int64_t)head * p.splits;
+    pdl_wait();                            // the prefix's partials, and whoever read the output before
     publish_head<__nv_bfloat16>(p, red, WARPS, head, p.prefix_splits + split, parts, slot0);
     if (parts == 1) return;
     __threadfence();
@@ -492,9 +513,18 @@ static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
     }
     if (ps > 0) {
         const int groups = (p.batch * p.G + 2 * PT - 1) / (2 * PT);
-        SKV_CUDA_OK(launch_pdl(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(320), P_SMEM, st, p, kmap, vmap));
+        SKV_CUDA_OK(launch_pdl(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(P_THREADS), P_SMEM, st, p, kmap, vmap));
     }
-    prefix_own_kernel<OWN_STAGES><<<dim3(own, p.batch * p.h_kv), 128, OWN_SMEM, st>>>(p);
+    // The second launch may always start early behind the first, which waits for everything before it: its own rows are
+    // read while the last tiles of the prefix are multiplied.
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(own, p.batch * p.h_kv); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = OWN_SMEM; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ps > 0 ? 1 : 0;
+    SKV_CUDA_OK(cudaLaunchKernelEx(&cfg, prefix_own_kernel<OWN_STAGES>, p));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }

@@ -22,6 +22,7 @@ struct PrefixParams {
     int32_t *status;
     int batch, h_kv, G, n_group, prefix, rows_limit, splits;
     int prefix_splits, own_splits;      // bf16: prefix_splits + own_splits <= splits
+    int listed;                         // bf16: rows of the prefix that the second launch reads itself
     int64_t kph, kpr, vph, vpr, ksh, ksr, vsh, vsr;
     float scale_log2;
 };
@@ -158,7 +159,7 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
             mbar_init(b_kempty + 8 * i, 1); mbar_init(b_vempty + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(b_sfull + 8 * i, 1); mbar_init(b_pfull + 8 * i, PT); mbar_init(b_done + 8 * i, 1);
+            mbar_init(b_sfull + 8 * i, 1); mbar_init(b_pfull + 8 * i, PT / 32); mbar_init(b_done + 8 * i, 1);
         }
         mbar_init(b_drain, 1);
         s_fail = 0;
@@ -343,7 +344,8 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
             l += all.x + all.y;
             tcgen05_wait_st();
             tcgen05_before_sync();
-            mbar_arrive(b_pfull + 8 * w);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_pfull + 8 * w);
         }
         if (ok && turns > 0) ok = mbar_wait_warp(b_done + 8 * w, 0);
         if (!ok) s_fail = 1;
@@ -403,16 +405,18 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
     }
 }
 
-// The sequences' own rows, and everything merged by the head's last CTA: grid (own splits, sequence x KV head).
+// The sequences' own rows, and everything merged: grid (own splits, sequence x KV head).  With `listed`, the prefix's rows
+// too, as one list ahead of the own ones (short prefixes and small batches, which the second-level cache serves).
+// STAGES tiles of 16 rows per warp: as many as the shared memory allows at the CTAs per SM that the grid makes.
 template <int STAGES>
 __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p) {
     constexpr int WARPS = 4;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t s_vmask[WARPS][STAGES];
     __shared__ int s_flag;
-    const int warp = threadIdx.x >> 5, head = blockIdx.y, split = blockIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, head = blockIdx.y, split = blockIdx.x, h = head % p.h_kv, G = p.G;
     const int n = own_rows(p, head);
-    const int tiles = (n + TILE_ROWS - 1) / TILE_ROWS;
+    const int shared_tiles = (p.listed + TILE_ROWS - 1) / TILE_ROWS, tiles = shared_tiles + (n + TILE_ROWS - 1) / TILE_ROWS;
     const int s_eff = min(p.own_splits, max(1, (tiles + WARPS - 1) / WARPS));
     if (split >= s_eff) {
         pdl_wait();
@@ -420,23 +424,86 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
     }
     const int slots = s_eff * WARPS, per = (tiles + slots - 1) / slots;
     const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
+    const char *ko = static_cast<const char *>(p.k) + (int64_t)head * p.ksh * 2, *vo = static_cast<const char *>(p.v) + (int64_t)head * p.vsh * 2;
     WarpAttendT<STAGES> wa;
-    wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * p.G * HEAD_DIM, p.G, smem + warp * (STAGES * 8192),
-            s_vmask[warp], static_cast<const char *>(p.k) + (int64_t)head * p.ksh * 2,
-            static_cast<const char *>(p.v) + (int64_t)head * p.vsh * 2, p.ksr * 2, p.vsr * 2, p.scale_log2);
-    wa.run(t0, t1, [&](int row) { return row < n ? row : -1; });
+    wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * G * HEAD_DIM, G, smem + warp * (STAGES * 8192),
+            s_vmask[warp], static_cast<const char *>(p.kp) + (int64_t)h * p.kph * 2,
+            static_cast<const char *>(p.vp) + (int64_t)h * p.vph * 2, p.kpr * 2, p.vpr * 2, p.scale_log2);
+    if (t0 < shared_tiles) wa.run(t0, min(t1, shared_tiles), [&](int row) { return row < p.listed ? row : -1; });
+    wa.Kb = ko; wa.Vb = vo; wa.krow = p.ksr * 2; wa.vrow = p.vsr * 2;
+    if (t1 > shared_tiles)
+        wa.run(max(t0, shared_tiles) - shared_tiles, t1 - shared_tiles, [&](int row) { return row < n ? row : -1; });
     __syncthreads();
     float *red = reinterpret_cast<float *>(smem);
-    wa.store_partial(red, warp, p.G);
+    wa.store_partial(red, warp, G);
     __syncthreads();
     const int parts = p.prefix_splits + s_eff;
     const int64_t slot0 = (int64_t)head * p.splits;
     pdl_wait();                            // the prefix's partials, and whoever read the output before
+    if (s_eff == 1) {
+        // Alone: the prefix's partials straight from where they lie.  Every warp folds a quarter of each row's into its own
+        // partial (a lane has four columns; the loads of two query heads are in flight together), then the four are joined.
+        constexpr int AT_ONCE = 5;
+        const int lane = tid & 31;
+        for (int g0 = 0; g0 < G; g0 += 2) {
+            float M[2], dn[2];
+            float4 nm[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float *r = red + (warp * G + min(g0 + e, G - 1)) * PART_LD;
+                M[e] = r[128]; dn[e] = r[129];
+                nm[e] = *reinterpret_cast<const float4 *>(r + lane * 4);
+            }
+            for (int i0 = warp; i0 < p.prefix_splits; i0 += WARPS * AT_ONCE) {
+                float2 ml[2][AT_ONCE];
+                float4 a[2][AT_ONCE];
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        ml[e][i] = make_float2(NEG_BIG, 0.f);
+                        a[e][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (i0 + i * WARPS < p.prefix_splits) {
+                            const float *r = p.part + ((slot0 + i0 + i * WARPS) * G + min(g0 + e, G - 1)) * PART_LD;
+                            ml[e][i] = __ldcg(reinterpret_cast<const float2 *>(r + 128));
+                            a[e][i] = __ldcg(reinterpret_cast<const float4 *>(r + lane * 4));
+                        }
+                    }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = M[e];
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, ml[e][i].x);
+                    const float al = fast_exp2(M[e] - top);
+                    M[e] = top;
+                    dn[e] *= al;
+                    nm[e].x *= al; nm[e].y *= al; nm[e].z *= al; nm[e].w *= al;
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; ++i) {
+                        const float f = fast_exp2(ml[e][i].x - top);
+                        dn[e] = fmaf(f, ml[e][i].y, dn[e]);
+                        nm[e].x = fmaf(f, a[e][i].x, nm[e].x); nm[e].y = fmaf(f, a[e][i].y, nm[e].y);
+                        nm[e].z = fmaf(f, a[e][i].z, nm[e].z); nm[e].w = fmaf(f, a[e][i].w, nm[e].w);
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (g0 + e >= G) continue;
+                float *r = red + (warp * G + g0 + e) * PART_LD;
+                __syncwarp();
+                *reinterpret_cast<float4 *>(r + lane * 4) = nm[e];
+                if (lane == 0) { r[128] = M[e]; r[129] = dn[e]; }
+            }
+        }
+        __syncthreads();
+        publish_head<__nv_bfloat16>(p, red, WARPS, head, 0, 1, 0);
+        return;
+    }
     publish_head<__nv_bfloat16>(p, red, WARPS, head, p.prefix_splits + split, parts, slot0);
-    if (parts == 1) return;
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) s_flag = s_eff == 1 || atomicAdd(p.ticket + head, 1) == s_eff - 1;
+    if (tid == 0) s_flag = atomicAdd(p.ticket + head, 1) == s_eff - 1;
     __syncthreads();
     if (!s_flag) return;
     __threadfence();
@@ -454,9 +521,36 @@ static int launch_prefix_simple(const PrefixParams &p, cudaStream_t st) {
     return SKV_OK;
 }
 
-constexpr int OWN_STAGES = 2, OWN_SMEM = 4 * OWN_STAGES * 8192;
+template <int STAGES>
+static int launch_own(const PrefixParams &p, cudaStream_t st) {
+    constexpr int SMEM = 4 * STAGES * 8192;
+    static bool configured[64] = {};       // the attribute is kept per device
+    int dev = 0;
+    SKV_CUDA_OK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return SKV_E_RANGE;
+    if (!configured[dev]) {
+        SKV_CUDA_OK(cudaFuncSetAttribute(prefix_own_kernel<STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        configured[dev] = true;
+    }
+    // Behind the prefix's launch, which waits for everything before it, this one may always start early: its own rows are
+    // read while the last tiles of the prefix are multiplied.
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.own_splits, p.batch * p.h_kv); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = SMEM; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.prefix_splits > 0 ? 1 : 0;
+    SKV_CUDA_OK(cudaLaunchKernelEx(&cfg, prefix_own_kernel<STAGES>, p));
+    SKV_CUDA_OK(cudaGetLastError());
+    return SKV_OK;
+}
 
-// Most CTAs the prefix of a KV head is split over: one per SM over all heads and row groups.
+// The prefix's rows go through the list where reading them once per sequence moves at most this much.
+constexpr int64_t LIST_BYTES = 64 << 20;
+
+// Most CTAs the prefix of a KV head is split over: one per SM over all heads and row groups.  (A call uses at most a third
+// of the prefix's tiles: a partial costs the merge as much as a tile costs its CTA.)
 static int prefix_splits_of(int batch, int h_kv, int G) {
     const int groups = (batch * G + 2 * PT - 1) / (2 * PT), s = device_sm_count() / (h_kv * groups);
     return s < 1 ? 1 : s;
@@ -490,43 +584,34 @@ static bool prefix_map(CUtensorMap *map, const void *x, int h_kv, int prefix, in
 }
 
 static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
-    const int tiles = (p.prefix + PT - 1) / PT;
-    int ps = prefix_splits_of(p.batch, p.h_kv, p.G);
-    ps = ps < tiles ? ps : tiles;
+    const int heads = p.batch * p.h_kv, tiles = (p.prefix + PT - 1) / PT;
+    const bool list = (int64_t)heads * p.prefix * 2 * HEAD_DIM * 2 <= LIST_BYTES;
+    int ps = list ? 0 : prefix_splits_of(p.batch, p.h_kv, p.G);
+    if (ps > (tiles + 2) / 3) ps = (tiles + 2) / 3;
     if (ps > p.splits - 1) ps = p.splits - 1;
-    int own = skv_attend_splits(p.batch * p.h_kv);
-    if (own > p.splits - ps) own = p.splits - ps;
-    p.prefix_splits = ps;
-    p.own_splits = own;
     CUtensorMap kmap, vmap;
     if (ps > 0 && (!prefix_map(&kmap, p.kp, p.h_kv, p.prefix, p.kph, p.kpr) ||
                    !prefix_map(&vmap, p.vp, p.h_kv, p.prefix, p.vph, p.vpr)))
-        return launch_prefix_simple<__nv_bfloat16>(p, st);
-    static bool configured[64] = {};       // the attributes are kept per device
-    int dev = 0;
-    SKV_CUDA_OK(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return SKV_E_RANGE;
-    if (!configured[dev]) {
-        SKV_CUDA_OK(cudaFuncSetAttribute(prefix_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM));
-        SKV_CUDA_OK(cudaFuncSetAttribute(prefix_own_kernel<OWN_STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, OWN_SMEM));
-        configured[dev] = true;
-    }
+        ps = 0;                            // (strides that no map can have)
+    int own = skv_attend_splits(heads);
+    if (own > p.splits - ps) own = p.splits - ps;
+    p.prefix_splits = ps;
+    p.own_splits = own;
+    p.listed = ps > 0 ? 0 : p.prefix;
     if (ps > 0) {
+        static bool configured[64] = {};   // the attribute is kept per device
+        int dev = 0;
+        SKV_CUDA_OK(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= 64) return SKV_E_RANGE;
+        if (!configured[dev]) {
+            SKV_CUDA_OK(cudaFuncSetAttribute(prefix_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM));
+            configured[dev] = true;
+        }
         const int groups = (p.batch * p.G + 2 * PT - 1) / (2 * PT);
         SKV_CUDA_OK(launch_pdl(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(P_THREADS), P_SMEM, st, p, kmap, vmap));
     }
-    // The second launch may always start early behind the first, which waits for everything before it: its own rows are
-    // read while the last tiles of the prefix are multiplied.
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(own, p.batch * p.h_kv); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = OWN_SMEM; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = ps > 0 ? 1 : 0;
-    SKV_CUDA_OK(cudaLaunchKernelEx(&cfg, prefix_own_kernel<OWN_STAGES>, p));
-    SKV_CUDA_OK(cudaGetLastError());
-    return SKV_OK;
+    const int ctas = heads * own, sms = device_sm_count();
+    return ctas <= sms ? launch_own<6>(p, st) : ctas <= 2 * sms ? launch_own<3>(p, st) : launch_own<2>(p, st);
 }
 
 }  // namespace skv
@@ -579,7 +664,7 @@ extern "C" int skv_attend_prefix(const void *q, const void *k_prefix, const void
     p.ksh = k_head_stride; p.ksr = k_row_stride; p.vsh = v_head_stride; p.vsr = v_row_stride;
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    p.prefix_splits = p.own_splits = 0;
+    p.prefix_splits = p.own_splits = p.listed = 0;
     if (dtype == SKV_F32) return launch_prefix_simple<float>(p, st);
     return splits > 1 ? launch_prefix_mma(p, st) : launch_prefix_simple<__nv_bfloat16>(p, st);
 }

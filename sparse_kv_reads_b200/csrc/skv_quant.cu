@@ -1,8 +1,8 @@
 // Writing rows into a quantised KV cache and reading them back.
 //
 // Both move a few bytes per value and compute little: HBM-bound for a prefill chunk, launch-bound for a decode step.
-// Half a warp serves one cached position of one KV head, key and value together, so that a lane's two 16-byte loads (8
-// values each) are requested before either is used and the position's scales are written by one place.
+// Half a warp serves one cached position of one KV head, key and value together (a lane has 8 values of each), and two
+// positions at once, so that a lane's four loads are requested before any is used.
 #include "skv_quant.cuh"
 #include "skv_rope.cuh"
 
@@ -17,7 +17,11 @@ struct RowsParams {
     const int64_t *pos;          // first position: pos[0], or pos[sequence] with pos_per_seq; null: pos0
     int64_t pos0;
     int pos_per_seq, batch, h_kv, capacity, tokens;
+    uint32_t items;              // positions x heads x sequences
 };
+
+constexpr int AT_ONCE = 2;       // positions of a half warp
+constexpr int PER_CTA = 16 * AT_ONCE;
 
 // Position of token `t` of sequence `b`; -1 (recorded in the head's status) when it lies outside the cache.
 __device__ __forceinline__ int64_t row_position(const RowsParams &p, int b, int head, int t) {
@@ -30,60 +34,166 @@ __device__ __forceinline__ int64_t row_position(const RowsParams &p, int b, int 
     return at;
 }
 
+// A lane's eight values and the magnitude bits of the largest.  bf16: compared two at a time as they lie in memory.
+__device__ __forceinline__ uint32_t largest_of(const uint4 &raw, float (&x)[8]) {
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&raw);
+    __nv_bfloat162 top = __habs2(h[0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(h[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+        if (i) top = __hmax2_nan(top, __habs2(h[i]));
+    }
+    const uint32_t t = *reinterpret_cast<const uint32_t *>(&top);
+    return max(t << 16, t & 0xffff0000u);
+}
+
+template <typename T> struct Eight;
+template <> struct Eight<__nv_bfloat16> {
+    uint4 v;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { v = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ uint32_t values(float (&x)[8]) const { return largest_of(v, x); }
+};
+template <> struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = __ldcs(reinterpret_cast<const float4 *>(p));
+        b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+    }
+    __device__ __forceinline__ uint32_t values(float (&x)[8]) const {
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(x[i]));
+        return top;
+    }
+};
+
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256) quant_write_kernel(const RowsParams p) {
     using Q = Quant<BITS>;
+    constexpr bool EXACT = sizeof(T) == 4;
     const int sub = threadIdx.x & 15;
     const unsigned hmask = (threadIdx.x & 16) ? 0xffff0000u : 0x0000ffffu;
-    const int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (item >= (int64_t)p.batch * p.h_kv * p.tokens) return;         // uniform within the half warp
-    const int t = (int)(item % p.tokens), head = (int)(item / p.tokens);
-    const int b = head / p.h_kv, h = head % p.h_kv;
-    const int64_t at = row_position(p, b, head, t);
-    if (at < 0) return;
-    float k[8], v[8];
-    load8(static_cast<const T *>(p.k) + b * p.kb + h * p.kh + t * p.kr + sub * 8, k);
-    load8(static_cast<const T *>(p.v) + b * p.vb + h * p.vh + t * p.vr + sub * 8, v);
-    const int64_t row = (int64_t)head * p.capacity + at;
-    const float ks = quantise_row8<BITS>(k, sub, hmask, p.kc + row * Q::ROW_BYTES, true);
-    const float vs = quantise_row8<BITS>(v, sub, hmask, p.vc + row * Q::ROW_BYTES, true);
-    if (sub % (16 / Q::GROUPS) == 0) {
-        __nv_bfloat16 *s = p.scale + row * Q::SCALES + group_of<BITS>(sub);
-        s[0] = __float2bfloat16(ks);
-        s[Q::GROUPS] = __float2bfloat16(vs);
+    Eight<T> k[AT_ONCE], v[AT_ONCE];
+    int64_t row[AT_ONCE];
+#pragma unroll
+    for (int r = 0; r < AT_ONCE; ++r) {                    // (everything about a position is uniform within its half warp)
+        const uint32_t item = blockIdx.x * PER_CTA + r * 16 + (threadIdx.x >> 4);
+        row[r] = -1;
+        if (item >= p.items) continue;
+        const uint32_t head = item / (uint32_t)p.tokens;
+        const int t = (int)(item - head * p.tokens), b = (int)(head / (uint32_t)p.h_kv), h = (int)head - b * p.h_kv;
+        const int64_t at = row_position(p, b, (int)head, t);
+        if (at < 0) continue;
+        row[r] = (int64_t)head * p.capacity + at;
+        k[r].load(static_cast<const T *>(p.k) + b * p.kb + h * p.kh + t * p.kr + sub * 8);
+        v[r].load(static_cast<const T *>(p.v) + b * p.vb + h * p.vh + t * p.vr + sub * 8);
+    }
+#pragma unroll
+    for (int r = 0; r < AT_ONCE; ++r) {
+        if (row[r] < 0) continue;
+        float x[8];
+        uint32_t top = k[r].values(x);
+        const float ks = quantise_row8<BITS, EXACT>(x, top, sub, hmask, p.kc + row[r] * Q::ROW_BYTES);
+        top = v[r].values(x);
+        const float vs = quantise_row8<BITS, EXACT>(x, top, sub, hmask, p.vc + row[r] * Q::ROW_BYTES);
+        if (sub % (16 / Q::GROUPS) == 0) {
+            __nv_bfloat16 *s = p.scale + row[r] * Q::SCALES + group_of<BITS>(sub);
+            s[0] = __float2bfloat16(ks);
+            s[Q::GROUPS] = __float2bfloat16(vs);
+        }
     }
 }
 
-__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
-    __align__(16) __nv_bfloat162 o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(o);
-}
-__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
-    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-}
+__device__ __forceinline__ uint32_t bf2(__nv_bfloat162 x) { return *reinterpret_cast<const uint32_t *>(&x); }
+__device__ __forceinline__ __nv_bfloat162 bf2(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162 *>(&x); }
 
-// code * scale has at most 15 significant bits: exact in float32, rounded once where the destination is bf16.
+// A lane's eight stored codes -> values.  bf16: code and scale are both bf16 numbers, so one packed product rounds the value
+// once; codes become bf16 by bytes and masks (0x4300 | c is 128 + c for c < 128; the sign of an 8-bit code is taken off it).
+// float32: the product has at most 15 significant bits and is exact.
+template <int BITS> struct Stored;
+template <> struct Stored<8> {
+    uint2 w;
+    __device__ __forceinline__ void load(const unsigned char *row, int sub) { w = __ldcs(reinterpret_cast<const uint2 *>(row + sub * 8)); }
+    __device__ __forceinline__ void store(__nv_bfloat16 *out, __nv_bfloat16 scale) const {
+        const __nv_bfloat162 s = __halves2bfloat162(scale, scale);
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = __byte_perm((i < 2 ? w.x : w.y) ^ 0x80808080u, 0x43434343u, i & 1 ? 0x4342 : 0x4140);
+            o[i] = bf2(__hmul2(__hsub2(bf2(u & 0xff7fff7fu), bf2(u & 0xff80ff80u)), s));
+        }
+        *reinterpret_cast<uint4 *>(out) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    __device__ __forceinline__ float code(int i) const { return (float)((int)(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255u) - 128); }
+};
+template <> struct Stored<4> {
+    uint32_t r0, r1;
+    __device__ __forceinline__ void load(const unsigned char *row, int sub) {
+        const int unit = 8 * (sub & 3) + (sub >> 2);       // runs 2 sub and 2 sub + 1: places 2 (sub % 4), + 1 of the group
+        r0 = __ldcs(reinterpret_cast<const unsigned short *>(row + unit * 2));
+        r1 = __ldcs(reinterpret_cast<const unsigned short *>(row + unit * 2 + 8));
+    }
+    __device__ __forceinline__ void store(__nv_bfloat16 *out, __nv_bfloat16 scale) const {
+        const __nv_bfloat162 s = __halves2bfloat162(scale, scale), bias = __float2bfloat162_rn(136.f);
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t r = i < 2 ? r0 : r1, two = i & 1 ? (r >> 8) | (r << 4) : r | (r << 12);
+            o[i] = bf2(__hmul2(__hsub2(bf2((two & 0x000f000fu) | 0x43004300u), bias), s));
+        }
+        *reinterpret_cast<uint4 *>(out) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    __device__ __forceinline__ float code(int i) const { return (float)((int)(((i < 4 ? r0 : r1) >> (4 * (i & 3))) & 15u) - 8); }
+};
+template <int BITS>
+__device__ __forceinline__ void store_values(float *out, const Stored<BITS> &c, __nv_bfloat16 scale) {
+    const float s = __bfloat162float(scale);
+    *reinterpret_cast<float4 *>(out) = make_float4(c.code(0) * s, c.code(1) * s, c.code(2) * s, c.code(3) * s);
+    *reinterpret_cast<float4 *>(out + 4) = make_float4(c.code(4) * s, c.code(5) * s, c.code(6) * s, c.code(7) * s);
+}
+template <int BITS>
+__device__ __forceinline__ void store_values(__nv_bfloat16 *out, const Stored<BITS> &c, __nv_bfloat16 scale) { c.store(out, scale); }
+
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256) quant_read_kernel(const RowsParams p) {
     using Q = Quant<BITS>;
     const int sub = threadIdx.x & 15;
-    const int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (item >= (int64_t)p.batch * p.h_kv * p.tokens) return;
-    const int t = (int)(item % p.tokens), head = (int)(item / p.tokens);
-    const int b = head / p.h_kv, h = head % p.h_kv;
-    const int64_t at = row_position(p, b, head, t);
-    float k[8] = {}, v[8] = {};
-    if (at >= 0) {
+    Stored<BITS> k[AT_ONCE], v[AT_ONCE];
+    __nv_bfloat16 ks[AT_ONCE], vs[AT_ONCE];
+    T *ko[AT_ONCE], *vo[AT_ONCE];
+#pragma unroll
+    for (int r = 0; r < AT_ONCE; ++r) {
+        const uint32_t item = blockIdx.x * PER_CTA + r * 16 + (threadIdx.x >> 4);
+        ko[r] = nullptr;
+        if (item >= p.items) continue;
+        const uint32_t head = item / (uint32_t)p.tokens;
+        const int t = (int)(item - head * p.tokens), b = (int)(head / (uint32_t)p.h_kv), h = (int)head - b * p.h_kv;
+        ko[r] = static_cast<T *>(p.k) + b * p.kb + h * p.kh + t * p.kr + sub * 8;
+        vo[r] = static_cast<T *>(p.v) + b * p.vb + h * p.vh + t * p.vr + sub * 8;
+        const int64_t at = row_position(p, b, (int)head, t);
+        if (at < 0) {
+            float4 *o[2] = {reinterpret_cast<float4 *>(ko[r]), reinterpret_cast<float4 *>(vo[r])};
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) o[0][i] = o[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            ko[r] = nullptr;
+            continue;
+        }
         const int64_t row = (int64_t)head * p.capacity + at;
+        k[r].load(p.kc + row * Q::ROW_BYTES, sub);
+        v[r].load(p.vc + row * Q::ROW_BYTES, sub);
         const __nv_bfloat16 *s = p.scale + row * Q::SCALES + group_of<BITS>(sub);
-        restore_row8<BITS>(p.kc + row * Q::ROW_BYTES, sub, __bfloat162float(s[0]), k);
-        restore_row8<BITS>(p.vc + row * Q::ROW_BYTES, sub, __bfloat162float(s[Q::GROUPS]), v);
+        ks[r] = s[0];
+        vs[r] = s[Q::GROUPS];
     }
-    store8(static_cast<T *>(p.k) + b * p.kb + h * p.kh + t * p.kr + sub * 8, k);
-    store8(static_cast<T *>(p.v) + b * p.vb + h * p.vh + t * p.vr + sub * 8, v);
+#pragma unroll
+    for (int r = 0; r < AT_ONCE; ++r)
+        if (ko[r]) {
+            store_values<BITS>(ko[r], k[r], ks[r]);
+            store_values<BITS>(vo[r], v[r], vs[r]);
+        }
 }
 
 // The decode step's QK-norm + rotary (qk_rope_cache_kernel's arithmetic and roundings) with the new key and value rows
@@ -118,8 +228,11 @@ __global__ void __launch_bounds__(128) qk_rope_quant_kernel(const __nv_bfloat16 
 #pragma unroll
     for (int o = 1; o < (BITS == 8 ? 32 : 8); o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float s = group_scale<BITS>(top);
-    const uint32_t c0 = stored_code<BITS>(r.x, s), c1 = stored_code<BITS>(r.y, s), c2 = stored_code<BITS>(r.z, s),
-                   c3 = stored_code<BITS>(r.w, s);
+    const float x[8] = {r.x, r.y, r.z, r.w, 0.f, 0.f, 0.f, 0.f};
+    uint32_t c[8];
+    stored_codes<BITS, false>(x, s, c);
+    constexpr uint32_t MASK = BITS == 8 ? 255u : 15u;
+    const uint32_t c0 = c[0] & MASK, c1 = c[1] & MASK, c2 = c[2] & MASK, c3 = c[3] & MASK;
     unsigned char *dst = (is_v ? p.vc : p.kc) + row * Q::ROW_BYTES;
     if (BITS == 8) *reinterpret_cast<uint32_t *>(dst + lane * 4) = c0 | c1 << 8 | c2 << 16 | c3 << 24;
     else *reinterpret_cast<uint16_t *>(dst + ((lane & 7) * 4 + (lane >> 3)) * 2) = (uint16_t)(c0 | c1 << 4 | c2 << 8 | c3 << 12);
@@ -134,7 +247,9 @@ static int rows_check(const skv_qcache *c, const void *k, const void *v, int dty
     if (rc) return rc;
     if (!k || !v) return SKV_E_NULL;
     if (dtype != SKV_BF16 && dtype != SKV_F32) return SKV_E_DTYPE;
-    if (batch <= 0 || batch > c->batch || tokens < 0 || tokens > c->capacity) return SKV_E_RANGE;
+    if (batch <= 0 || batch > c->batch || tokens < 0 || tokens > c->capacity ||
+        (int64_t)batch * c->h_kv * tokens > 0x7fffffff)
+        return SKV_E_RANGE;
     if (!pos && (pos0 < 0 || pos0 + tokens > c->capacity)) return SKV_E_RANGE;
     const int per16 = dtype == SKV_BF16 ? 8 : 4;
     if (!aligned16(k) || !aligned16(v) || kb % per16 || kh % per16 || kr % per16 || vb % per16 || vh % per16 || vr % per16)
@@ -145,6 +260,7 @@ static int rows_check(const skv_qcache *c, const void *k, const void *v, int dty
     p.scale = static_cast<__nv_bfloat16 *>(c->scale); p.status = c->status;
     p.pos = pos; p.pos0 = pos0;
     p.batch = batch; p.h_kv = c->h_kv; p.capacity = c->capacity; p.tokens = tokens;
+    p.items = (uint32_t)batch * c->h_kv * tokens;
     return SKV_OK;
 }
 
@@ -162,8 +278,7 @@ extern "C" int skv_quant_write(const skv_qcache *c, const void *k, const void *v
     if (rc) return rc;
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
-    const int64_t items = (int64_t)batch * c->h_kv * tokens;
-    const dim3 grid((unsigned)((items + 15) / 16));
+    const dim3 grid((p.items + PER_CTA - 1) / PER_CTA);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_BF16 && c->bits == 8) quant_write_kernel<__nv_bfloat16, 8><<<grid, 256, 0, st>>>(p);
     else if (dtype == SKV_BF16) quant_write_kernel<__nv_bfloat16, 4><<<grid, 256, 0, st>>>(p);
@@ -183,8 +298,7 @@ extern "C" int skv_quant_read(const skv_qcache *c, void *k, void *v, int dtype, 
     if (rc) return rc;
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
-    const int64_t items = (int64_t)batch * c->h_kv * tokens;
-    const dim3 grid((unsigned)((items + 15) / 16));
+    const dim3 grid((p.items + PER_CTA - 1) / PER_CTA);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_BF16 && c->bits == 8) quant_read_kernel<__nv_bfloat16, 8><<<grid, 256, 0, st>>>(p);
     else if (dtype == SKV_BF16) quant_read_kernel<__nv_bfloat16, 4><<<grid, 256, 0, st>>>(p);

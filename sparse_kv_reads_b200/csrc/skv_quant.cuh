@@ -34,44 +34,59 @@ __device__ __forceinline__ float group_scale(uint32_t largest) {
     return s < 1.17549435e-38f ? 0.f : s;
 }
 
-// An IEEE quotient: for a bf16 value and a bf16 scale it is exact wherever the true quotient lies half-way between two
-// codes and far enough from there otherwise, so the code is the nearest one (ties to even) of the true quotient.
-template <int BITS>
-__device__ __forceinline__ uint32_t stored_code(float x, float scale) {
-    constexpr float M = (float)Quant<BITS>::MOST;
-    const float c = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -M), M) : 0.f;
-    return (uint32_t)((int)c + Quant<BITS>::BIAS);
+// The stored codes of eight values, as the low bits of the results.  Adding 1.5 * 2^23 rounds a quotient to an integer, ties
+// to even, and leaves it, biased, in the low bits; no clamp is needed, since the scale is at most 2^-9 of itself too small.
+// EXACT: an IEEE quotient.  Else the values are bf16, like the scale: a quotient from the rounded reciprocal y with one
+// correction by its exact remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).
+// Where the true quotient lies half-way between two codes it is a float32 number t, the first quotient is t + d, its
+// remainder -s d, and the corrected one t - d (1 - s y) rounds to t; everywhere else two 8-bit significands keep the
+// quotient 2^-16 of itself away from there.  So the code is the nearest one (ties to even) of the true quotient.
+// (Remainders of scales below 2^-90 could leave the numbers: those take the IEEE quotient as well.)
+template <int BITS, bool EXACT>
+__device__ __forceinline__ void stored_codes(const float (&x)[8], float scale, uint32_t (&c)[8]) {
+    constexpr float ROUND = 12582912.f + (float)Quant<BITS>::BIAS;
+    if (!(scale > 0.f)) {                                  // zeros, or a group that has no scale
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = Quant<BITS>::BIAS;
+    } else if (EXACT || scale < 8.077936e-28f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(__fdiv_rn(x[i], scale) + ROUND);
+    } else {
+        const float y = __frcp_rn(scale);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = x[i] * y;
+            c[i] = __float_as_uint(fmaf(fmaf(-q, scale, x[i]), y, q) + ROUND);
+        }
+    }
 }
 
-// Eight consecutive values (lane `sub` of 16 owns components 8 sub .. 8 sub + 7) -> their place in the stored row.
-// The lanes of a half warp call this together.  Returns the scale of the lane's group.
-template <int BITS>
-__device__ __forceinline__ float quantise_row8(const float (&x)[8], int sub, unsigned hmask, unsigned char *row,
-                                               bool store) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(x[i]));
+// Eight consecutive values (lane `sub` of 16 owns components 8 sub .. 8 sub + 7), whose largest magnitude has the bits
+// `top`, -> their place in the stored row.  The lanes of a half warp call this together.  Returns the lane's group's scale.
+template <int BITS, bool EXACT>
+__device__ __forceinline__ float quantise_row8(const float (&x)[8], uint32_t top, int sub, unsigned hmask,
+                                               unsigned char *row) {
 #pragma unroll
     for (int o = 1; o < (BITS == 8 ? 16 : 4); o <<= 1) top = max(top, __shfl_xor_sync(hmask, top, o, 16));
     const float s = group_scale<BITS>(top);
     uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = stored_code<BITS>(x[i], s);
+    stored_codes<BITS, EXACT>(x, s, c);
     if (BITS == 8) {
         uint2 w;
-        w.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-        w.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-        if (store) *reinterpret_cast<uint2 *>(row + sub * 8) = w;
+        w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+        *reinterpret_cast<uint2 *>(row + sub * 8) = w;
     } else {
         // runs 2 sub and 2 sub + 1: group sub / 4, places j = 2 (sub % 4) and j + 1; the neighbouring group's lane
         // (sub ^ 4) has the run that lies beside either of them
-        const uint32_t r0 = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12, r1 = c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12;
+        const uint32_t r0 = (c[0] & 15u) | (c[1] & 15u) << 4 | (c[2] & 15u) << 8 | (c[3] & 15u) << 12;
+        const uint32_t r1 = (c[4] & 15u) | (c[5] & 15u) << 4 | (c[6] & 15u) << 8 | (c[7] & 15u) << 12;
         const int grp = sub >> 2, j = 2 * (sub & 3);
         const bool odd = grp & 1;
         const uint32_t other = __shfl_xor_sync(hmask, odd ? r0 : r1, 4, 16);
         const uint32_t w = odd ? (other | r1 << 16) : (r0 | other << 16);
         const int unit = odd ? (j + 1) * 4 + grp - 1 : j * 4 + grp;
-        if (store) *reinterpret_cast<uint32_t *>(row + unit * 2) = w;
+        *reinterpret_cast<uint32_t *>(row + unit * 2) = w;
     }
     return s;
 }

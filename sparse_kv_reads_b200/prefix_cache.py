@@ -79,9 +79,9 @@ class PrefixAttentionGraph:
         L = lib()
         self.B, self.H, self.H_kv, self.d, self.G = B, H, H_kv, d, H // H_kv
         self.n_group = 0                                   # KV heads per entry of the device-side lengths (0: one length)
-        self.dtype, self.device = dtype, torch.device(device)
+        self.dtype = dtype
         self._code = dtype_code(dtype)
-        with on_device(self.device):
+        with on_device(torch.device(device)):
             self.num_splits = L.skv_prefix_splits(B, H_kv, self.G, self._code)
             size = L.skv_prefix_workspace_bytes(B, H_kv, self.G, d, self.num_splits) if self.num_splits > 0 \
                 else self.num_splits
@@ -90,33 +90,44 @@ class PrefixAttentionGraph:
             self.ws = torch.zeros(size, dtype=torch.uint8, device=device)
             self.out = torch.empty(B * H, d, dtype=dtype, device=device)
             self.status = torch.zeros(B * H_kv, dtype=torch.int32, device=device)
-        self._scale = 1.0 / math.sqrt(d)
+        self.device = self.out.device                      # (with its index)
+        self._shape, self._scale = self.out.shape, 1.0 / math.sqrt(d)
+        self._checked = None
+
+    def _check_layout(self, Kp, Vp, K, V) -> None:
+        heads = self.B * self.H_kv
+        if Kp.dim() != 3 or Kp.shape != Vp.shape or Kp.shape[0] != self.H_kv or Kp.shape[2] != self.d:
+            raise ValueError(f"the prefix must be [{self.H_kv}, rows, {self.d}]")
+        if K.dim() != 3 or K.shape != V.shape or K.shape[0] != heads or K.shape[2] != self.d:
+            raise ValueError(f"the sequences' rows must be [{heads}, rows, {self.d}]")
+        if any(t.shape[1] and t.stride(2) != 1 for t in (Kp, Vp, K, V)):
+            raise ValueError("the caches must have a unit last stride")
 
     def __call__(self, q: torch.Tensor, Kp: torch.Tensor, Vp: torch.Tensor, K: torch.Tensor, V: torch.Tensor,
                  n_dev: torch.Tensor) -> torch.Tensor:
         """``q [B*H, d]``; ``Kp, Vp [H_kv, P, d]`` the shared rows; ``K, V [B*H_kv, L, d]`` the sequences' own rows;
         ``n_dev`` int32 on the device, own lengths: one, or one per ``n_group`` KV heads.  A row without keys gets zeros."""
-        heads = self.B * self.H_kv
-        if q.shape != self.out.shape or q.dtype != self.dtype:
-            raise ValueError(f"queries must be {tuple(self.out.shape)} {self.dtype}")
-        if Kp.dim() != 3 or Kp.shape != Vp.shape or Kp.shape[0] != self.H_kv or Kp.shape[2] != self.d:
-            raise ValueError(f"the prefix must be [{self.H_kv}, rows, {self.d}]")
-        if K.dim() != 3 or K.shape != V.shape or K.shape[0] != heads or K.shape[2] != self.d:
-            raise ValueError(f"the sequences' rows must be [{heads}, rows, {self.d}]")
-        dev = self.out.device
-        for t in (Kp, Vp, K, V):
-            if t.dtype != self.dtype or t.device != dev or (t.shape[1] and t.stride(2) != 1):
-                raise ValueError("the caches must have the queries' type and device and a unit last stride")
-        if n_dev.dtype != torch.int32 or n_dev.device != dev or q.device != dev \
-                or n_dev.numel() < (-(-heads // self.n_group) if self.n_group else 1):
+        layout = (Kp.shape, Kp.stride(), Vp.shape, Vp.stride(), K.shape, K.stride(), V.shape, V.stride())
+        if layout != self._checked:                        # (a decode step has the same layout again and again)
+            self._check_layout(Kp, Vp, K, V)
+            self._checked = layout
+        dev, dtype = self.device, self.dtype
+        if q.shape != self._shape or q.dtype is not dtype:
+            raise ValueError(f"queries must be {tuple(self._shape)} {dtype}")
+        if not (Kp.dtype is Vp.dtype is K.dtype is V.dtype is dtype and
+                Kp.device == Vp.device == K.device == V.device == q.device == dev):
+            raise ValueError("the caches must have the queries' type and device")
+        if n_dev.dtype is not torch.int32 or n_dev.device != dev or not n_dev.is_contiguous() \
+                or n_dev.numel() < (-(-self.B * self.H_kv // self.n_group) if self.n_group else 1):
             raise ValueError("lengths must be int32 on the queries' device: one, or one per n_group KV heads")
         if not q.is_contiguous() or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
+        ks, vs, pks, pvs = layout[5], layout[7], layout[1], layout[3]
         with on_device(dev):
-            check(lib().skv_attend_prefix(q.data_ptr(), Kp.data_ptr(), Vp.data_ptr(), Kp.shape[1], K.data_ptr(),
+            check(lib().skv_attend_prefix(q.data_ptr(), Kp.data_ptr(), Vp.data_ptr(), layout[0][1], K.data_ptr(),
                                           V.data_ptr(), n_dev.data_ptr(), self.n_group, self.out.data_ptr(),
                                           self.ws.data_ptr(), self.status.data_ptr(), self.B, self.H_kv, self.G, self.d,
-                                          self._code, Kp.stride(0), Kp.stride(1), Vp.stride(0), Vp.stride(1), K.stride(0),
-                                          K.stride(1), V.stride(0), V.stride(1), K.shape[1], self.num_splits, self._scale,
-                                          stream_ptr(dev)), "skv_attend_prefix")
+                                          self._code, pks[0], pks[1], pvs[0], pvs[1], ks[0], ks[1], vs[0], vs[1],
+                                          layout[4][1], self.num_splits, self._scale, stream_ptr(dev)),
+                  "skv_attend_prefix")
         return self.out

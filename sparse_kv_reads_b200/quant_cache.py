@@ -60,6 +60,7 @@ class QuantKVCache:
         self.batch, self.h_kv, self.max_seq_len, _ = k[0].shape
         self.d, self.device = 128, k[0].device
         self.cur_len = 0
+        self._plans = {}
         self.status = torch.zeros(self.batch * self.h_kv, dtype=torch.int32, device=self.device) if status is None else status
         self._st = [SkvQCache(a.data_ptr(), b.data_ptr(), s.data_ptr(), self.status.data_ptr(), self.batch, self.h_kv,
                               self.max_seq_len, self.d, bits, 0) for a, b, s in zip(k, v, scale)]
@@ -77,46 +78,59 @@ class QuantKVCache:
             bits |= s
         return bits
 
-    def _where(self, pos, b: int):
-        """``pos`` as (device address or None, one per sequence, host value)."""
-        if not torch.is_tensor(pos):
-            return None, 0, int(pos)
-        if pos.dtype != torch.long or pos.device != self.device or pos.dim() != 1 or not pos.is_contiguous() \
-                or pos.shape[0] not in (1, b):
-            raise ValueError("positions are an int, or int64 [1] or [sequences] on the cache's device")
-        return pos.data_ptr(), int(pos.shape[0] != 1), 0
+    def _where(self, pos, b: int, count: int):
+        """``pos`` as (device address or None, one per sequence, host value), the host value checked."""
+        if torch.is_tensor(pos):
+            if pos.dtype is not torch.long or pos.device != self.device or pos.dim() != 1 or not pos.is_contiguous() \
+                    or pos.shape[0] not in (1, b):
+                raise ValueError("positions are an int, or int64 [1] or [sequences] on the cache's device")
+            return pos.data_ptr(), int(pos.shape[0] != 1), 0
+        at = int(pos)
+        if not 0 <= at <= self.max_seq_len - count:
+            raise ValueError(f"rows [{at}, {at + count}) lie outside the cache's {self.max_seq_len} positions")
+        return None, 0, at
 
-    @staticmethod
-    def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
-        per16 = 16 // t.element_size()
-        s0, s1, s2, s3 = t.stride()
-        if s3 != 1 or s0 % per16 or s1 % per16 or s2 % per16 or t.data_ptr() % 16:
-            return t.contiguous()
-        return t
+    def _plan(self, k: torch.Tensor, v: torch.Tensor):
+        """What a write of tensors of these shapes, strides and types passes on: the type's code, sizes and strides; no
+        strides where the rows have to be copied first (a last stride other than 1, rows off the 16-byte boundaries)."""
+        if k.dim() != 4 or k.shape != v.shape or k.shape[1] != self.h_kv or k.shape[3] != self.d or k.shape[0] > self.batch:
+            raise ValueError(f"keys and values must be [sequences <= {self.batch}, {self.h_kv}, tokens, {self.d}]")
+        if k.dtype != v.dtype:
+            raise ValueError("keys and values must be of one type, on the cache's device")
+        if k.shape[2] > self.max_seq_len:
+            raise ValueError(f"{k.shape[2]} rows do not fit the cache's {self.max_seq_len} positions")
+        head = (dtype_code(k.dtype), k.shape[0], k.shape[2])
+        per16 = 16 // k.element_size()
+        strides = k.stride()[:3] + v.stride()[:3]
+        straight = k.stride(3) == v.stride(3) == 1 and not any(s % per16 for s in strides)
+        return head, strides if straight else None
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, pos) -> None:
         """Quantise ``k, v [b, H_kv, T, 128]`` (bf16 or float32, any strides) into the rows ``[pos, pos + T)`` of the
         first ``b`` sequences.  ``pos``: an int, or int64 in device memory, one for all or one per sequence; rows of a
         device position that fall outside the cache are left out and recorded in ``status``."""
-        if k.dim() != 4 or k.shape != v.shape or k.shape[1] != self.h_kv or k.shape[3] != self.d or k.shape[0] > self.batch:
-            raise ValueError(f"keys and values must be [sequences <= {self.batch}, {self.h_kv}, tokens, {self.d}]")
-        if k.dtype != v.dtype or k.device != self.device or v.device != self.device:
+        key = (k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype)
+        plan = self._plans.get(key)                        # (a decode step writes the same shape again and again)
+        if plan is None:
+            plan = self._plan(k, v)
+            if len(self._plans) >= 256:
+                self._plans.clear()
+            self._plans[key] = plan
+        if k.device != self.device or v.device != self.device:
             raise ValueError("keys and values must be of one type, on the cache's device")
-        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
             raise ValueError("a quantised cache has no gradient: write under torch.no_grad()")
-        code = dtype_code(k.dtype)
-        b, T = k.shape[0], k.shape[2]
-        at, per_seq, host = self._where(pos, b)
-        if at is None and not 0 <= host <= self.max_seq_len - T:
-            raise ValueError(f"rows [{host}, {host + T}) lie outside the cache's {self.max_seq_len} positions")
-        if T > self.max_seq_len:
-            raise ValueError(f"{T} rows do not fit the cache's {self.max_seq_len} positions")
+        (code, b, T), strides = plan
+        at, per_seq, host = self._where(pos, b, T)
         if b == 0 or T == 0:
             return
-        k, v = self._rows("k", k), self._rows("v", v)
+        kp, vp = k.data_ptr(), v.data_ptr()
+        if strides is None or (kp | vp) % 16:
+            k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+            kp, vp, strides = k.data_ptr(), v.data_ptr(), k.stride()[:3] + v.stride()[:3]
         with on_device(self.device):
-            check(lib().skv_quant_write(self._st[layer], k.data_ptr(), v.data_ptr(), code, b, T, *k.stride()[:3],
-                                        *v.stride()[:3], at, per_seq, host, stream_ptr(self.device)), "skv_quant_write")
+            check(lib().skv_quant_write(self._st[layer], kp, vp, code, b, T, *strides, at, per_seq, host,
+                                        stream_ptr(self.device)), "skv_quant_write")
 
     def read(self, layer: int, pos, count: int, *, dtype: torch.dtype = torch.bfloat16,
              batch: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -125,12 +139,11 @@ class QuantKVCache:
         b = self.batch if batch is None else batch
         if not 0 <= b <= self.batch:
             raise ValueError(f"the cache holds {self.batch} sequences")
-        at, per_seq, host = self._where(pos, b)
-        if not 0 <= count <= self.max_seq_len or (at is None and not 0 <= host <= self.max_seq_len - count):
-            raise ValueError(f"rows [{host}, {host + count}) lie outside the cache's {self.max_seq_len} positions")
+        if not 0 <= count <= self.max_seq_len:
+            raise ValueError(f"{count} rows lie outside the cache's {self.max_seq_len} positions")
+        at, per_seq, host = self._where(pos, b, count)
         code = dtype_code(dtype)
-        out = torch.empty(2, b, self.h_kv, count, self.d, dtype=dtype, device=self.device)
-        k, v = out[0], out[1]
+        k, v = torch.empty(2, b, self.h_kv, count, self.d, dtype=dtype, device=self.device).unbind(0)
         if b and count:
             hs = count * self.d
             bs = self.h_kv * hs
@@ -155,31 +168,33 @@ class QuantAttentionGraph:
         L = lib()
         self.H, self.H_kv, self.d, self.G = H, H_kv, d, H // H_kv
         self.n_group = 0                                   # heads per entry of the device-side lengths (0: one length)
-        self.dtype, self.device = dtype, torch.device(device)
+        self.dtype = dtype
         self._code = dtype_code(dtype)
-        with on_device(self.device):
+        with on_device(torch.device(device)):
             self.ctas = L.skv_quant_ctas()
             size = L.skv_quant_workspace_bytes(H_kv, self.G, d, self.ctas)
             if size < 0:
                 raise SkvError(L.skv_error_string(int(size)).decode())
             self.ws = torch.zeros(size, dtype=torch.uint8, device=device)
             self.out = torch.empty(H, d, dtype=dtype, device=device)
-        self._scale = 1.0 / math.sqrt(d)
+        self.device = self.out.device                      # (with its index)
+        self._shape, self._scale = self.out.shape, 1.0 / math.sqrt(d)
 
     def __call__(self, q: torch.Tensor, cache: QuantKVCache, layer: int, n_dev: torch.Tensor) -> torch.Tensor:
         """``q [H, d]`` (all sequences' query heads), ``n_dev`` int32 on the device: one length, or one per ``n_group``
         heads.  A head without rows gets zeros."""
-        if q.shape != self.out.shape or q.dtype != self.dtype:
-            raise ValueError(f"queries must be {tuple(self.out.shape)} {self.dtype}")
-        if cache.batch * cache.h_kv != self.H_kv or cache.device != q.device or q.device != self.out.device:
+        if q.shape != self._shape or q.dtype is not self.dtype:
+            raise ValueError(f"queries must be {tuple(self._shape)} {self.dtype}")
+        dev = self.device
+        if cache.batch * cache.h_kv != self.H_kv or cache.device != dev or q.device != dev:
             raise ValueError(f"the cache must hold {self.H_kv} KV heads, on the queries' device")
-        if n_dev.dtype != torch.int32 or n_dev.device != q.device \
+        if n_dev.dtype is not torch.int32 or n_dev.device != dev or not n_dev.is_contiguous() \
                 or n_dev.numel() < (-(-self.H_kv // self.n_group) if self.n_group else 1):
             raise ValueError("lengths must be int32 on the queries' device: one, or one per n_group heads")
         if not q.is_contiguous() or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
-        with on_device(q.device):
+        with on_device(dev):
             check(lib().skv_attend_quant(cache._st[layer], q.data_ptr(), self._code, self.G, n_dev.data_ptr(),
-                                         self.n_group, self.out.data_ptr(), self.ws.data_ptr(), self.ctas,
-                                         self._scale, stream_ptr(q.device)), "skv_attend_quant")
+                                         self.n_group, self.out.data_ptr(), self.ws.data_ptr(), self.ctas, self._scale,
+                                         stream_ptr(dev)), "skv_attend_quant")
         return self.out

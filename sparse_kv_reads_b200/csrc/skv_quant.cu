@@ -18,6 +18,7 @@ struct RowsParams {
     int64_t pos0;
     int pos_per_seq, batch, h_kv, capacity, tokens;
     uint32_t items;              // positions x heads x sequences
+    int flat;                    // the grid is flat over them, else (positions, KV heads, sequences)
 };
 
 constexpr int AT_ONCE = 2;       // positions of a half warp
@@ -34,26 +35,49 @@ __device__ __forceinline__ int64_t row_position(const RowsParams &p, int b, int 
     return at;
 }
 
-// A lane's eight values and the magnitude bits of the largest.  bf16: compared two at a time as they lie in memory.
-__device__ __forceinline__ uint32_t largest_of(const uint4 &raw, float (&x)[8]) {
-    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&raw);
-    __nv_bfloat162 top = __habs2(h[0]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __bfloat1622float2(h[i]);
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-        if (i) top = __hmax2_nan(top, __habs2(h[i]));
+// Where the work of a half warp lies: 3-d grid (positions, KV heads, sequences), or, for few tokens per sequence, a flat one.
+struct Place {
+    int b, h, t, head;
+    bool any;
+};
+__device__ __forceinline__ Place place_of(const RowsParams &p, int r) {
+    Place w;
+    const uint32_t item = blockIdx.x * PER_CTA + r * 16 + (threadIdx.x >> 4);
+    if (p.flat) {
+        const uint32_t head = item / (uint32_t)p.tokens;
+        w.any = item < p.items;
+        w.t = (int)(item - head * p.tokens);
+        w.head = (int)head;
+        w.b = (int)(head / (uint32_t)p.h_kv);
+        w.h = w.head - w.b * p.h_kv;
+    } else {
+        w.any = item < (uint32_t)p.tokens;
+        w.t = (int)item;
+        w.h = blockIdx.y;
+        w.b = blockIdx.z;
+        w.head = w.b * p.h_kv + w.h;
     }
-    const uint32_t t = *reinterpret_cast<const uint32_t *>(&top);
-    return max(t << 16, t & 0xffff0000u);
+    return w;
 }
 
+// A lane's eight values of a key or value row.
 template <typename T> struct Eight;
 template <> struct Eight<__nv_bfloat16> {
     uint4 v;
     __device__ __forceinline__ void load(const __nv_bfloat16 *p) { v = __ldcs(reinterpret_cast<const uint4 *>(p)); }
-    __device__ __forceinline__ uint32_t values(float (&x)[8]) const { return largest_of(v, x); }
+    __device__ __forceinline__ void values(float (&x)[8]) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    // the largest magnitude in both halves' order of the packed numbers (NaN above all)
+    __device__ __forceinline__ __nv_bfloat162 largest() const {
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+        return __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    }
 };
 template <> struct Eight<float> {
     float4 a, b;
@@ -61,14 +85,42 @@ template <> struct Eight<float> {
         a = __ldcs(reinterpret_cast<const float4 *>(p));
         b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
     }
-    __device__ __forceinline__ uint32_t values(float (&x)[8]) const {
+    __device__ __forceinline__ void values(float (&x)[8]) const {
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(x[i]));
-        return top;
     }
 };
+
+// The scales of the lane's groups of key and value: over 16 lanes (8 bits) or 4 (4 bits).
+template <int BITS>
+__device__ __forceinline__ void scales_of(const Eight<__nv_bfloat16> &k, const Eight<__nv_bfloat16> &v, unsigned hmask, float &ks,
+                                          float &vs) {
+    const __nv_bfloat162 tk = k.largest(), tv = v.largest();
+    __nv_bfloat162 top = __hmax2_nan(__lows2bfloat162(tk, tv), __highs2bfloat162(tk, tv));      // (key, value)
+#pragma unroll
+    for (int o = 1; o < (BITS == 8 ? 16 : 4); o <<= 1) {
+        const uint32_t u = __shfl_xor_sync(hmask, *reinterpret_cast<const uint32_t *>(&top), o, 16);
+        top = __hmax2_nan(top, *reinterpret_cast<const __nv_bfloat162 *>(&u));
+    }
+    const uint32_t u = *reinterpret_cast<const uint32_t *>(&top);
+    ks = group_scale_bf16<BITS>(u << 16 & 0x7fffffffu);
+    vs = group_scale_bf16<BITS>(u & 0x7fff0000u);
+}
+template <int BITS>
+__device__ __forceinline__ void scales_of(const Eight<float> &k, const Eight<float> &v, unsigned hmask, float &ks, float &vs) {
+    float x[8], y[8];
+    k.values(x);
+    v.values(y);
+    uint32_t a = 0, b = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { a = max(a, magnitude_bits(x[i])); b = max(b, magnitude_bits(y[i])); }
+#pragma unroll
+    for (int o = 1; o < (BITS == 8 ? 16 : 4); o <<= 1) {
+        a = max(a, __shfl_xor_sync(hmask, a, o, 16));
+        b = max(b, __shfl_xor_sync(hmask, b, o, 16));
+    }
+    ks = group_scale<BITS>(a);
+    vs = group_scale<BITS>(b);
+}
 
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256) quant_write_kernel(const RowsParams p) {
@@ -80,25 +132,28 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const RowsParams p) {
     int64_t row[AT_ONCE];
 #pragma unroll
     for (int r = 0; r < AT_ONCE; ++r) {                    // (everything about a position is uniform within its half warp)
-        const uint32_t item = blockIdx.x * PER_CTA + r * 16 + (threadIdx.x >> 4);
+        const Place w = place_of(p, r);
         row[r] = -1;
-        if (item >= p.items) continue;
-        const uint32_t head = item / (uint32_t)p.tokens;
-        const int t = (int)(item - head * p.tokens), b = (int)(head / (uint32_t)p.h_kv), h = (int)head - b * p.h_kv;
-        const int64_t at = row_position(p, b, (int)head, t);
+        if (!w.any) continue;
+        const int64_t at = row_position(p, w.b, w.head, w.t);
         if (at < 0) continue;
-        row[r] = (int64_t)head * p.capacity + at;
-        k[r].load(static_cast<const T *>(p.k) + b * p.kb + h * p.kh + t * p.kr + sub * 8);
-        v[r].load(static_cast<const T *>(p.v) + b * p.vb + h * p.vh + t * p.vr + sub * 8);
+        row[r] = (int64_t)w.head * p.capacity + at;
+        k[r].load(static_cast<const T *>(p.k) + w.b * p.kb + w.h * p.kh + w.t * p.kr + sub * 8);
+        v[r].load(static_cast<const T *>(p.v) + w.b * p.vb + w.h * p.vh + w.t * p.vr + sub * 8);
     }
 #pragma unroll
     for (int r = 0; r < AT_ONCE; ++r) {
         if (row[r] < 0) continue;
-        float x[8];
-        uint32_t top = k[r].values(x);
-        const float ks = quantise_row8<BITS, EXACT>(x, top, sub, hmask, p.kc + row[r] * Q::ROW_BYTES);
-        top = v[r].values(x);
-        const float vs = quantise_row8<BITS, EXACT>(x, top, sub, hmask, p.vc + row[r] * Q::ROW_BYTES);
+        float ks, vs, x[8];
+        uint32_t c[8];
+        scales_of<BITS>(k[r], v[r], hmask, ks, vs);
+        k[r].values(x);
+        stored_codes<BITS, EXACT>(x, ks, c);
+        const uint2 kc = packed_codes<BITS>(c);
+        v[r].values(x);
+        stored_codes<BITS, EXACT>(x, vs, c);
+        const uint2 vc = packed_codes<BITS>(c);
+        store_rows<BITS>(kc, vc, sub, hmask, p.kc + row[r] * Q::ROW_BYTES, p.vc + row[r] * Q::ROW_BYTES);
         if (sub % (16 / Q::GROUPS) == 0) {
             __nv_bfloat16 *s = p.scale + row[r] * Q::SCALES + group_of<BITS>(sub);
             s[0] = __float2bfloat16(ks);
@@ -166,14 +221,12 @@ __global__ void __launch_bounds__(256) quant_read_kernel(const RowsParams p) {
     T *ko[AT_ONCE], *vo[AT_ONCE];
 #pragma unroll
     for (int r = 0; r < AT_ONCE; ++r) {
-        const uint32_t item = blockIdx.x * PER_CTA + r * 16 + (threadIdx.x >> 4);
+        const Place w = place_of(p, r);
         ko[r] = nullptr;
-        if (item >= p.items) continue;
-        const uint32_t head = item / (uint32_t)p.tokens;
-        const int t = (int)(item - head * p.tokens), b = (int)(head / (uint32_t)p.h_kv), h = (int)head - b * p.h_kv;
-        ko[r] = static_cast<T *>(p.k) + b * p.kb + h * p.kh + t * p.kr + sub * 8;
-        vo[r] = static_cast<T *>(p.v) + b * p.vb + h * p.vh + t * p.vr + sub * 8;
-        const int64_t at = row_position(p, b, (int)head, t);
+        if (!w.any) continue;
+        ko[r] = static_cast<T *>(p.k) + w.b * p.kb + w.h * p.kh + w.t * p.kr + sub * 8;
+        vo[r] = static_cast<T *>(p.v) + w.b * p.vb + w.h * p.vh + w.t * p.vr + sub * 8;
+        const int64_t at = row_position(p, w.b, w.head, w.t);
         if (at < 0) {
             float4 *o[2] = {reinterpret_cast<float4 *>(ko[r]), reinterpret_cast<float4 *>(vo[r])};
 #pragma unroll
@@ -181,7 +234,7 @@ __global__ void __launch_bounds__(256) quant_read_kernel(const RowsParams p) {
             ko[r] = nullptr;
             continue;
         }
-        const int64_t row = (int64_t)head * p.capacity + at;
+        const int64_t row = (int64_t)w.head * p.capacity + at;
         k[r].load(p.kc + row * Q::ROW_BYTES, sub);
         v[r].load(p.vc + row * Q::ROW_BYTES, sub);
         const __nv_bfloat16 *s = p.scale + row * Q::SCALES + group_of<BITS>(sub);
@@ -227,7 +280,7 @@ __global__ void __launch_bounds__(128) qk_rope_quant_kernel(const __nv_bfloat16 
     uint32_t top = max(max(magnitude_bits(r.x), magnitude_bits(r.y)), max(magnitude_bits(r.z), magnitude_bits(r.w)));
 #pragma unroll
     for (int o = 1; o < (BITS == 8 ? 32 : 8); o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float s = group_scale<BITS>(top);
+    const float s = group_scale_bf16<BITS>(top);
     const float x[8] = {r.x, r.y, r.z, r.w, 0.f, 0.f, 0.f, 0.f};
     uint32_t c[8];
     stored_codes<BITS, false>(x, s, c);
@@ -238,6 +291,13 @@ __global__ void __launch_bounds__(128) qk_rope_quant_kernel(const __nv_bfloat16 
     else *reinterpret_cast<uint16_t *>(dst + ((lane & 7) * 4 + (lane >> 3)) * 2) = (uint16_t)(c0 | c1 << 4 | c2 << 8 | c3 << 12);
     if (lane % (32 / Q::GROUPS) == 0)
         p.scale[row * Q::SCALES + (is_v ? Q::GROUPS : 0) + lane / (32 / Q::GROUPS)] = __float2bfloat16(s);
+}
+
+// A flat grid where a CTA would otherwise be mostly idle (a decode step writes one position per sequence).
+static dim3 rows_grid(RowsParams &p) {
+    p.flat = p.tokens < PER_CTA;
+    if (p.flat) return dim3((p.items + PER_CTA - 1) / PER_CTA);
+    return dim3((unsigned)(p.tokens + PER_CTA - 1) / PER_CTA, (unsigned)p.h_kv, (unsigned)p.batch);
 }
 
 static int rows_check(const skv_qcache *c, const void *k, const void *v, int dtype, int batch, int tokens, int64_t kb,
@@ -278,7 +338,7 @@ extern "C" int skv_quant_write(const skv_qcache *c, const void *k, const void *v
     if (rc) return rc;
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
-    const dim3 grid((p.items + PER_CTA - 1) / PER_CTA);
+    const dim3 grid = rows_grid(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_BF16 && c->bits == 8) quant_write_kernel<__nv_bfloat16, 8><<<grid, 256, 0, st>>>(p);
     else if (dtype == SKV_BF16) quant_write_kernel<__nv_bfloat16, 4><<<grid, 256, 0, st>>>(p);
@@ -298,7 +358,7 @@ extern "C" int skv_quant_read(const skv_qcache *c, void *k, void *v, int dtype, 
     if (rc) return rc;
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
-    const dim3 grid((p.items + PER_CTA - 1) / PER_CTA);
+    const dim3 grid = rows_grid(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_BF16 && c->bits == 8) quant_read_kernel<__nv_bfloat16, 8><<<grid, 256, 0, st>>>(p);
     else if (dtype == SKV_BF16) quant_read_kernel<__nv_bfloat16, 4><<<grid, 256, 0, st>>>(p);

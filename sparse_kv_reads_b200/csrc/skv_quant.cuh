@@ -11,6 +11,7 @@
 #pragma once
 
 #include "skv_common.cuh"
+#include "skv_pairs.cuh"
 
 namespace skv {
 
@@ -34,61 +35,74 @@ __device__ __forceinline__ float group_scale(uint32_t largest) {
     return s < 1.17549435e-38f ? 0.f : s;
 }
 
+// The same for values that are bf16 themselves (`largest`: the float32 bits of one).  The quotient by 127 or 7 of an 8-bit
+// significand stays 2^-16 of itself away from the middle between two bf16 numbers, so a product with the rounded 1 / 127 or
+// 1 / 7 rounds to the same scale.
+template <int BITS>
+__device__ __forceinline__ float group_scale_bf16(uint32_t largest) {
+    const float s = __bfloat162float(__float2bfloat16(__uint_as_float(largest) * (1.f / (float)Quant<BITS>::MOST)));
+    return largest >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : s < 1.17549435e-38f ? 0.f : s;
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // The stored codes of eight values, as the low bits of the results.  Adding 1.5 * 2^23 rounds a quotient to an integer, ties
 // to even, and leaves it, biased, in the low bits; no clamp is needed, since the scale is at most 2^-9 of itself too small.
-// EXACT: an IEEE quotient.  Else the values are bf16, like the scale: a quotient from the rounded reciprocal y with one
-// correction by its exact remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).
-// Where the true quotient lies half-way between two codes it is a float32 number t, the first quotient is t + d, its
-// remainder -s d, and the corrected one t - d (1 - s y) rounds to t; everywhere else two 8-bit significands keep the
-// quotient 2^-16 of itself away from there.  So the code is the nearest one (ties to even) of the true quotient.
+// EXACT: an IEEE quotient.  Else the values are bf16, like the scale: a quotient from a reciprocal y with one correction by
+// its exact remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).  Where the true
+// quotient lies half-way between two codes it is a float32 number t, the first quotient is t + d, its remainder -s d, and the
+// corrected one t + d (1 - s y) rounds to t; everywhere else two 8-bit significands keep the quotient 2^-16 of itself away
+// from there.  So the code is the nearest one (ties to even) of the true quotient, with a reciprocal good to 2^-22.
 // (Remainders of scales below 2^-90 could leave the numbers: those take the IEEE quotient as well.)
 template <int BITS, bool EXACT>
 __device__ __forceinline__ void stored_codes(const float (&x)[8], float scale, uint32_t (&c)[8]) {
     constexpr float ROUND = 12582912.f + (float)Quant<BITS>::BIAS;
-    if (!(scale > 0.f)) {                                  // zeros, or a group that has no scale
+    if (!EXACT && scale >= 8.077936e-28f) {
+        const float y = rcp_approx(scale);
+        const float2 y2 = make_float2(y, y), s2 = make_float2(-scale, -scale), round = make_float2(ROUND, ROUND);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = Quant<BITS>::BIAS;
-    } else if (EXACT || scale < 8.077936e-28f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(__fdiv_rn(x[i], scale) + ROUND);
-    } else {
-        const float y = __frcp_rn(scale);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float q = x[i] * y;
-            c[i] = __float_as_uint(fmaf(fmaf(-q, scale, x[i]), y, q) + ROUND);
+        for (int i = 0; i < 8; i += 2) {
+            const float2 v = make_float2(x[i], x[i + 1]), q = mul2(v, y2);
+            const float2 t = add2(fma2(fma2(q, s2, v), y2, q), round);
+            c[i] = __float_as_uint(t.x);
+            c[i + 1] = __float_as_uint(t.y);
         }
+    } else {
+        const bool some = scale > 0.f;                     // else zeros, or a group that has no scale
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = __float_as_uint((some ? __fdiv_rn(x[i], scale) : 0.f) + ROUND);
     }
 }
 
-// Eight consecutive values (lane `sub` of 16 owns components 8 sub .. 8 sub + 7), whose largest magnitude has the bits
-// `top`, -> their place in the stored row.  The lanes of a half warp call this together.  Returns the lane's group's scale.
-template <int BITS, bool EXACT>
-__device__ __forceinline__ float quantise_row8(const float (&x)[8], uint32_t top, int sub, unsigned hmask,
-                                               unsigned char *row) {
-#pragma unroll
-    for (int o = 1; o < (BITS == 8 ? 16 : 4); o <<= 1) top = max(top, __shfl_xor_sync(hmask, top, o, 16));
-    const float s = group_scale<BITS>(top);
-    uint32_t c[8];
-    stored_codes<BITS, EXACT>(x, s, c);
+// Eight codes -> the lane's bytes of the stored row: 8 bits: eight bytes in order; 4 bits: the two runs (lower 16 bits of each).
+template <int BITS>
+__device__ __forceinline__ uint2 packed_codes(const uint32_t (&c)[8]) {
+    if (BITS == 8)
+        return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                          __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+    // (above a code lies 0x4b4000, whose low bits are zero: sums of shifted codes carry nothing into the lower 16)
+    return make_uint2(((c[3] << 4) + c[2] << 8) + ((c[1] << 4) + c[0]), ((c[7] << 4) + c[6] << 8) + ((c[5] << 4) + c[4]));
+}
+
+// Key and value of a position, lane `sub` of 16 with its eight codes of each (packed_codes), into their stored rows.  4 bits:
+// the lane's runs 2 sub and 2 sub + 1 belong to group sub / 4, places j = 2 (sub % 4) and j + 1; the neighbouring group's
+// lane (sub ^ 4) has the run that lies beside either of them: one exchange for key and value.
+template <int BITS>
+__device__ __forceinline__ void store_rows(uint2 k, uint2 v, int sub, unsigned hmask, unsigned char *krow, unsigned char *vrow) {
     if (BITS == 8) {
-        uint2 w;
-        w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-        w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-        *reinterpret_cast<uint2 *>(row + sub * 8) = w;
+        *reinterpret_cast<uint2 *>(krow + sub * 8) = k;
+        *reinterpret_cast<uint2 *>(vrow + sub * 8) = v;
     } else {
-        // runs 2 sub and 2 sub + 1: group sub / 4, places j = 2 (sub % 4) and j + 1; the neighbouring group's lane
-        // (sub ^ 4) has the run that lies beside either of them
-        const uint32_t r0 = (c[0] & 15u) | (c[1] & 15u) << 4 | (c[2] & 15u) << 8 | (c[3] & 15u) << 12;
-        const uint32_t r1 = (c[4] & 15u) | (c[5] & 15u) << 4 | (c[6] & 15u) << 8 | (c[7] & 15u) << 12;
-        const int grp = sub >> 2, j = 2 * (sub & 3);
-        const bool odd = grp & 1;
-        const uint32_t other = __shfl_xor_sync(hmask, odd ? r0 : r1, 4, 16);
-        const uint32_t w = odd ? (other | r1 << 16) : (r0 | other << 16);
-        const int unit = odd ? (j + 1) * 4 + grp - 1 : j * 4 + grp;
-        *reinterpret_cast<uint32_t *>(row + unit * 2) = w;
+        const bool odd = (sub >> 2) & 1;
+        const uint32_t other = __shfl_xor_sync(hmask, odd ? __byte_perm(k.x, v.x, 0x5410) : __byte_perm(k.y, v.y, 0x5410), 4, 16);
+        const int unit = odd ? 8 * (sub & 3) + 4 + (sub >> 2) - 1 : 8 * (sub & 3) + (sub >> 2);
+        *reinterpret_cast<uint32_t *>(krow + unit * 2) = odd ? __byte_perm(other, k.y, 0x5410) : __byte_perm(k.x, other, 0x5410);
+        *reinterpret_cast<uint32_t *>(vrow + unit * 2) = odd ? __byte_perm(other, v.y, 0x5432) : __byte_perm(v.x, other, 0x7610);
     }
-    return s;
 }
 
 // The inverse: the lane's eight values of a stored row, given the scale of the lane's group.

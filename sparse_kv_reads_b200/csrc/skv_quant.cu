@@ -18,11 +18,9 @@ struct RowsParams {
     int64_t pos0;
     int pos_per_seq, batch, h_kv, capacity, tokens;
     uint32_t items;              // positions x heads x sequences
-    int flat;                    // the grid is flat over them, else (positions, KV heads, sequences)
 };
 
-constexpr int AT_ONCE = 2;       // positions of a half warp
-constexpr int PER_CTA = 16 * AT_ONCE;
+constexpr int AT_ONCE = 2;       // positions of a half warp in a chunk
 
 // Position of token `t` of sequence `b`; -1 (recorded in the head's status) when it lies outside the cache.
 __device__ __forceinline__ int64_t row_position(const RowsParams &p, int b, int head, int t) {
@@ -35,30 +33,41 @@ __device__ __forceinline__ int64_t row_position(const RowsParams &p, int b, int 
     return at;
 }
 
-// Where the work of a half warp lies: 3-d grid (positions, KV heads, sequences), or, for few tokens per sequence, a flat one.
-struct Place {
-    int b, h, t, head;
-    bool any;
-};
-__device__ __forceinline__ Place place_of(const RowsParams &p, int r) {
-    Place w;
-    const uint32_t item = blockIdx.x * PER_CTA + r * 16 + (threadIdx.x >> 4);
-    if (p.flat) {
-        const uint32_t head = item / (uint32_t)p.tokens;
-        w.any = item < p.items;
-        w.t = (int)(item - head * p.tokens);
-        w.head = (int)head;
-        w.b = (int)(head / (uint32_t)p.h_kv);
-        w.h = w.head - w.b * p.h_kv;
-    } else {
-        w.any = item < (uint32_t)p.tokens;
-        w.t = (int)item;
-        w.h = blockIdx.y;
-        w.b = blockIdx.z;
-        w.head = w.b * p.h_kv + w.h;
+// The positions of a half warp.  A chunk: 3-d grid (positions, KV heads, sequences), N positions 16 apart, so that only the
+// first one's addresses are computed.  FLAT, for few tokens per sequence: one position of a flat grid over all.
+template <bool FLAT>
+struct Places {
+    static constexpr int N = FLAT ? 1 : AT_ONCE;
+    int b, h, t, head, count;    // first token; positions there are
+    int64_t first;               // cache row of token 0 (-1 - capacity: none of them lies in the cache)
+    __device__ __forceinline__ explicit Places(const RowsParams &p) {
+        const int half = threadIdx.x >> 4;
+        if (FLAT) {
+            const uint32_t item = blockIdx.x * 16 + half;
+            head = (int)(item / (uint32_t)p.tokens);
+            t = (int)(item - (uint32_t)head * p.tokens);
+            b = head / p.h_kv;
+            h = head - b * p.h_kv;
+            count = item < p.items;
+        } else {
+            t = (int)blockIdx.x * (16 * N) + half;
+            h = blockIdx.y;
+            b = blockIdx.z;
+            head = b * p.h_kv + h;
+            count = t < p.tokens ? min(N, (p.tokens - t + 15) >> 4) : 0;
+        }
+        if (!count) b = h = head = t = 0;
+        first = p.pos ? p.pos[p.pos_per_seq ? b : 0] : p.pos0;
+        if (first < 0 || first > p.capacity) first = -1 - (int64_t)p.capacity;
     }
-    return w;
-}
+    // cache row of the r-th position; -1 (recorded in the head's status) where it lies outside
+    __device__ __forceinline__ int row(const RowsParams &p, int r) const {
+        const int64_t at = first + t + 16 * r;
+        if (at >= 0 && at < p.capacity) return (int)at;
+        if (p.status) atomicOr(p.status + head, SKV_ST_BAD_INDEX);
+        return -1;
+    }
+};
 
 // A lane's eight values of a key or value row.
 template <typename T> struct Eight;
@@ -122,40 +131,43 @@ __device__ __forceinline__ void scales_of(const Eight<float> &k, const Eight<flo
     vs = group_scale<BITS>(b);
 }
 
-template <typename T, int BITS>
+template <typename T, int BITS, bool FLAT>
 __global__ void __launch_bounds__(256) quant_write_kernel(const RowsParams p) {
     using Q = Quant<BITS>;
     constexpr bool EXACT = sizeof(T) == 4;
     const int sub = threadIdx.x & 15;
     const unsigned hmask = (threadIdx.x & 16) ? 0xffff0000u : 0x0000ffffu;
-    Eight<T> k[AT_ONCE], v[AT_ONCE];
-    int64_t row[AT_ONCE];
+    const Places<FLAT> w(p);                               // (everything about a position is uniform within its half warp)
+    constexpr int N = Places<FLAT>::N;
+    const T *kg = static_cast<const T *>(p.k) + (w.b * p.kb + w.h * p.kh + w.t * p.kr + sub * 8);
+    const T *vg = static_cast<const T *>(p.v) + (w.b * p.vb + w.h * p.vh + w.t * p.vr + sub * 8);
+    Eight<T> k[N], v[N];
+    int row[N];
 #pragma unroll
-    for (int r = 0; r < AT_ONCE; ++r) {                    // (everything about a position is uniform within its half warp)
-        const Place w = place_of(p, r);
-        row[r] = -1;
-        if (!w.any) continue;
-        const int64_t at = row_position(p, w.b, w.head, w.t);
-        if (at < 0) continue;
-        row[r] = (int64_t)w.head * p.capacity + at;
-        k[r].load(static_cast<const T *>(p.k) + w.b * p.kb + w.h * p.kh + w.t * p.kr + sub * 8);
-        v[r].load(static_cast<const T *>(p.v) + w.b * p.vb + w.h * p.vh + w.t * p.vr + sub * 8);
+    for (int r = 0; r < N; ++r, kg += 16 * p.kr, vg += 16 * p.vr) {
+        row[r] = r < w.count ? w.row(p, r) : -1;
+        if (row[r] < 0) continue;
+        k[r].load(kg);
+        v[r].load(vg);
     }
+    const int64_t base = (int64_t)w.head * p.capacity;
+    unsigned char *const kc = p.kc + base * Q::ROW_BYTES, *const vc = p.vc + base * Q::ROW_BYTES;
+    __nv_bfloat16 *const scale = p.scale + base * Q::SCALES + group_of<BITS>(sub);
 #pragma unroll
-    for (int r = 0; r < AT_ONCE; ++r) {
+    for (int r = 0; r < N; ++r) {
         if (row[r] < 0) continue;
         float ks, vs, x[8];
         uint32_t c[8];
         scales_of<BITS>(k[r], v[r], hmask, ks, vs);
         k[r].values(x);
         stored_codes<BITS, EXACT>(x, ks, c);
-        const uint2 kc = packed_codes<BITS>(c);
+        const uint2 kp = packed_codes<BITS>(c);
         v[r].values(x);
         stored_codes<BITS, EXACT>(x, vs, c);
-        const uint2 vc = packed_codes<BITS>(c);
-        store_rows<BITS>(kc, vc, sub, hmask, p.kc + row[r] * Q::ROW_BYTES, p.vc + row[r] * Q::ROW_BYTES);
+        const uint2 vp = packed_codes<BITS>(c);
+        store_rows<BITS>(kp, vp, sub, hmask, kc + (int64_t)row[r] * Q::ROW_BYTES, vc + (int64_t)row[r] * Q::ROW_BYTES);
         if (sub % (16 / Q::GROUPS) == 0) {
-            __nv_bfloat16 *s = p.scale + row[r] * Q::SCALES + group_of<BITS>(sub);
+            __nv_bfloat16 *s = scale + (int64_t)row[r] * Q::SCALES;
             s[0] = __float2bfloat16(ks);
             s[Q::GROUPS] = __float2bfloat16(vs);
         }
@@ -212,41 +224,42 @@ __device__ __forceinline__ void store_values(float *out, const Stored<BITS> &c, 
 template <int BITS>
 __device__ __forceinline__ void store_values(__nv_bfloat16 *out, const Stored<BITS> &c, __nv_bfloat16 scale) { c.store(out, scale); }
 
-template <typename T, int BITS>
+template <typename T, int BITS, bool FLAT>
 __global__ void __launch_bounds__(256) quant_read_kernel(const RowsParams p) {
     using Q = Quant<BITS>;
     const int sub = threadIdx.x & 15;
-    Stored<BITS> k[AT_ONCE], v[AT_ONCE];
-    __nv_bfloat16 ks[AT_ONCE], vs[AT_ONCE];
-    T *ko[AT_ONCE], *vo[AT_ONCE];
+    const Places<FLAT> w(p);
+    constexpr int N = Places<FLAT>::N;
+    const int64_t base = (int64_t)w.head * p.capacity;
+    const unsigned char *const kc = p.kc + base * Q::ROW_BYTES, *const vc = p.vc + base * Q::ROW_BYTES;
+    const __nv_bfloat16 *const scale = p.scale + base * Q::SCALES + group_of<BITS>(sub);
+    Stored<BITS> k[N], v[N];
+    __nv_bfloat16 ks[N], vs[N];
+    int row[N];
 #pragma unroll
-    for (int r = 0; r < AT_ONCE; ++r) {
-        const Place w = place_of(p, r);
-        ko[r] = nullptr;
-        if (!w.any) continue;
-        ko[r] = static_cast<T *>(p.k) + w.b * p.kb + w.h * p.kh + w.t * p.kr + sub * 8;
-        vo[r] = static_cast<T *>(p.v) + w.b * p.vb + w.h * p.vh + w.t * p.vr + sub * 8;
-        const int64_t at = row_position(p, w.b, w.head, w.t);
-        if (at < 0) {
-            float4 *o[2] = {reinterpret_cast<float4 *>(ko[r]), reinterpret_cast<float4 *>(vo[r])};
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) o[0][i] = o[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            ko[r] = nullptr;
-            continue;
-        }
-        const int64_t row = (int64_t)w.head * p.capacity + at;
-        k[r].load(p.kc + row * Q::ROW_BYTES, sub);
-        v[r].load(p.vc + row * Q::ROW_BYTES, sub);
-        const __nv_bfloat16 *s = p.scale + row * Q::SCALES + group_of<BITS>(sub);
+    for (int r = 0; r < N; ++r) {
+        row[r] = r < w.count ? w.row(p, r) : -1;
+        if (row[r] < 0) continue;
+        k[r].load(kc + (int64_t)row[r] * Q::ROW_BYTES, sub);
+        v[r].load(vc + (int64_t)row[r] * Q::ROW_BYTES, sub);
+        const __nv_bfloat16 *s = scale + (int64_t)row[r] * Q::SCALES;
         ks[r] = s[0];
         vs[r] = s[Q::GROUPS];
     }
+    T *kg = static_cast<T *>(p.k) + (w.b * p.kb + w.h * p.kh + w.t * p.kr + sub * 8);
+    T *vg = static_cast<T *>(p.v) + (w.b * p.vb + w.h * p.vh + w.t * p.vr + sub * 8);
 #pragma unroll
-    for (int r = 0; r < AT_ONCE; ++r)
-        if (ko[r]) {
-            store_values<BITS>(ko[r], k[r], ks[r]);
-            store_values<BITS>(vo[r], v[r], vs[r]);
+    for (int r = 0; r < N; ++r, kg += 16 * p.kr, vg += 16 * p.vr) {
+        if (r >= w.count) continue;
+        if (row[r] >= 0) {
+            store_values<BITS>(kg, k[r], ks[r]);
+            store_values<BITS>(vg, v[r], vs[r]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                reinterpret_cast<float4 *>(kg)[i] = reinterpret_cast<float4 *>(vg)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
+    }
 }
 
 // The decode step's QK-norm + rotary (qk_rope_cache_kernel's arithmetic and roundings) with the new key and value rows
@@ -293,11 +306,21 @@ __global__ void __launch_bounds__(128) qk_rope_quant_kernel(const __nv_bfloat16 
         p.scale[row * Q::SCALES + (is_v ? Q::GROUPS : 0) + lane / (32 / Q::GROUPS)] = __float2bfloat16(s);
 }
 
-// A flat grid where a CTA would otherwise be mostly idle (a decode step writes one position per sequence).
-static dim3 rows_grid(RowsParams &p) {
-    p.flat = p.tokens < PER_CTA;
-    if (p.flat) return dim3((p.items + PER_CTA - 1) / PER_CTA);
-    return dim3((unsigned)(p.tokens + PER_CTA - 1) / PER_CTA, (unsigned)p.h_kv, (unsigned)p.batch);
+// A flat grid where a chunk's CTA would be mostly idle (a decode step writes one position per sequence).
+static bool rows_flat(const RowsParams &p) { return p.tokens < 16 * AT_ONCE || p.batch > 65535 || p.h_kv > 65535; }
+static dim3 rows_grid(const RowsParams &p) {
+    if (rows_flat(p)) return dim3((p.items + 15) / 16);
+    return dim3((unsigned)(p.tokens + 16 * AT_ONCE - 1) / (16 * AT_ONCE), (unsigned)p.h_kv, (unsigned)p.batch);
+}
+template <typename T, int BITS>
+static void launch_write(const RowsParams &p, cudaStream_t st) {
+    if (rows_flat(p)) quant_write_kernel<T, BITS, true><<<rows_grid(p), 256, 0, st>>>(p);
+    else quant_write_kernel<T, BITS, false><<<rows_grid(p), 256, 0, st>>>(p);
+}
+template <typename T, int BITS>
+static void launch_read(const RowsParams &p, cudaStream_t st) {
+    if (rows_flat(p)) quant_read_kernel<T, BITS, true><<<rows_grid(p), 256, 0, st>>>(p);
+    else quant_read_kernel<T, BITS, false><<<rows_grid(p), 256, 0, st>>>(p);
 }
 
 static int rows_check(const skv_qcache *c, const void *k, const void *v, int dtype, int batch, int tokens, int64_t kb,
@@ -338,12 +361,11 @@ extern "C" int skv_quant_write(const skv_qcache *c, const void *k, const void *v
     if (rc) return rc;
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
-    const dim3 grid = rows_grid(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == SKV_BF16 && c->bits == 8) quant_write_kernel<__nv_bfloat16, 8><<<grid, 256, 0, st>>>(p);
-    else if (dtype == SKV_BF16) quant_write_kernel<__nv_bfloat16, 4><<<grid, 256, 0, st>>>(p);
-    else if (c->bits == 8) quant_write_kernel<float, 8><<<grid, 256, 0, st>>>(p);
-    else quant_write_kernel<float, 4><<<grid, 256, 0, st>>>(p);
+    if (dtype == SKV_BF16 && c->bits == 8) launch_write<__nv_bfloat16, 8>(p, st);
+    else if (dtype == SKV_BF16) launch_write<__nv_bfloat16, 4>(p, st);
+    else if (c->bits == 8) launch_write<float, 8>(p, st);
+    else launch_write<float, 4>(p, st);
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -358,12 +380,11 @@ extern "C" int skv_quant_read(const skv_qcache *c, void *k, void *v, int dtype, 
     if (rc) return rc;
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
-    const dim3 grid = rows_grid(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == SKV_BF16 && c->bits == 8) quant_read_kernel<__nv_bfloat16, 8><<<grid, 256, 0, st>>>(p);
-    else if (dtype == SKV_BF16) quant_read_kernel<__nv_bfloat16, 4><<<grid, 256, 0, st>>>(p);
-    else if (c->bits == 8) quant_read_kernel<float, 8><<<grid, 256, 0, st>>>(p);
-    else quant_read_kernel<float, 4><<<grid, 256, 0, st>>>(p);
+    if (dtype == SKV_BF16 && c->bits == 8) launch_read<__nv_bfloat16, 8>(p, st);
+    else if (dtype == SKV_BF16) launch_read<__nv_bfloat16, 4>(p, st);
+    else if (c->bits == 8) launch_read<float, 8>(p, st);
+    else launch_read<float, 4>(p, st);
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }

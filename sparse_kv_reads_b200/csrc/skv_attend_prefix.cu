@@ -22,6 +22,7 @@ struct PrefixParams {
     int32_t *status;
     int batch, h_kv, G, n_group, prefix, rows_limit, splits;
     int prefix_splits, own_splits;      // bf16: prefix_splits + own_splits <= splits
+    int own_ctas;                       // bf16: CTAs of the second launch per sequence and KV head
     int listed;                         // bf16: rows of the prefix that the second launch reads itself
     int64_t kph, kpr, vph, vpr, ksh, ksr, vsh, vsr;
     float scale_log2;
@@ -165,31 +166,45 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
         s_fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_proxy();
-        // the first tiles are on their way before anything else: no earlier kernel of the same step writes the prefix
-        for (int i = 0; i < min(n, PSTAGES); ++i) {
-            load(kmap, kbase + i * 2 * P_TILE, b_kfull + 8 * i, t0 + i);
-            load(vmap, kbase + i * 2 * P_TILE + P_TILE, b_vfull + 8 * i, t0 + i);
-        }
+        // the first keys are on their way before anything else: no earlier kernel of the same step writes the prefix
+        if (n > 0) load(kmap, kbase, b_kfull, t0);
     }
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
     pdl_wait();
     pdl_trigger();
     // Queries into the 128-byte swizzle, 16 bytes at a time; rows beyond the last are zero.  A negative softmax scale goes
-    // into their sign: the running maximum is one of scaled scores.
-    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-    const int qrows = both ? PT : 2 * PT;
-    #pragma unroll 4
-    for (int i = tid; i < qrows * 16; i += P_THREADS) {
-        const int r = i >> 4, c = i & 15, row = row0 + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) {
-            const int b = row / p.G, g = row - b * p.G;
-            v = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.q) +
-                                                 (((int64_t)b * p.h_kv + h) * p.G + g) * HEAD_DIM + c * 8);
-            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+    // into their sign: the running maximum is one of scaled scores.  All of a thread's loads are requested at once, and ahead
+    // of the other tiles: behind them they took up to 14,000 cycles.
+    {
+        constexpr int CHUNKS = (2 * PT * 16 + P_THREADS - 1) / P_THREADS;
+        const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+        const int qrows = both ? PT : 2 * PT;
+        uint4 v[CHUNKS];
+#pragma unroll
+        for (int e = 0; e < CHUNKS; ++e) {
+            const int i = tid + e * P_THREADS, row = row0 + (i >> 4);
+            v[e] = make_uint4(0u, 0u, 0u, 0u);
+            if ((i >> 4) < qrows && row < rows) {
+                const int b = (int)((unsigned)row / (unsigned)p.G), g = row - b * p.G;
+                v[e] = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.q) +
+                                                        (((int64_t)b * p.h_kv + h) * p.G + g) * HEAD_DIM + (i & 15) * 8);
+            }
         }
-        const int rr = r & (PT - 1);
-        *reinterpret_cast<uint4 *>(smem + (r >> 7) * P_TILE + (c >> 3) * (P_TILE / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+        if (tid == 256) {
+            if (n > 0) load(vmap, kbase + P_TILE, b_vfull, t0);
+            for (int i = 1; i < min(n, PSTAGES); ++i) {
+                load(kmap, kbase + i * 2 * P_TILE, b_kfull + 8 * i, t0 + i);
+                load(vmap, kbase + i * 2 * P_TILE + P_TILE, b_vfull + 8 * i, t0 + i);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < CHUNKS; ++e) {
+            const int i = tid + e * P_THREADS, r = i >> 4, c = i & 15, rr = r & (PT - 1);
+            if (r >= qrows) continue;
+            v[e].x ^= flip; v[e].y ^= flip; v[e].z ^= flip; v[e].w ^= flip;
+            *reinterpret_cast<uint4 *>(smem + (r >> 7) * P_TILE + (c >> 3) * (P_TILE / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
+                v[e];
+        }
     }
     fence_async_proxy();
     tcgen05_before_sync();
@@ -351,9 +366,37 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
         if (!ok) s_fail = 1;
         tcgen05_after_sync();
         asm volatile("bar.sync 1, 256;" ::: "memory");    // both slots' products have ended: the tiles' memory is free
-        float *out = reinterpret_cast<float *>(smem + w * P_OUT) + r * PART_LD;
-        const bool fold = both && n > 1;                  // slot 1's rows are folded into slot 0's
-        if (turns > 0 && !(fold && w == 0)) {
+        const bool fold = both && n > 1;                  // the two slots have the same rows: a half of the columns each
+        float *out = reinterpret_cast<float *>(smem + (fold ? 0 : w) * P_OUT) + r * PART_LD;
+        const int row = row0 + (both ? 0 : w * PT) + r, b = (int)((unsigned)row / (unsigned)p.G), g = row - b * p.G;
+        float *dst = p.part + ((((int64_t)b * p.h_kv + h) * p.splits + split) * p.G + g) * PART_LD;
+        if (fold) {
+            float2 *ml = reinterpret_cast<float2 *>(smem + P_OUT);
+            ml[w * PT + r] = make_float2(m, l);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float2 a = ml[r], o = ml[PT + r];
+            const float M = fmaxf(a.x, o.x), f0 = fast_exp2(a.x - M), f1 = fast_exp2(o.x - M);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t x[32], y[32];
+                tmem_ld32(mine + 256 + w * 64 + c * 32, x);
+                tmem_ld32(mine + 256 + PT + w * 64 + c * 32, y);
+                tmem_ld_done(x);
+                tmem_ld_done(y);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<float4 *>(out + w * 64 + c * 32 + e) =
+                        make_float4(fmaf(f1, __uint_as_float(y[e]), f0 * __uint_as_float(x[e])),
+                                    fmaf(f1, __uint_as_float(y[e + 1]), f0 * __uint_as_float(x[e + 1])),
+                                    fmaf(f1, __uint_as_float(y[e + 2]), f0 * __uint_as_float(x[e + 2])),
+                                    fmaf(f1, __uint_as_float(y[e + 3]), f0 * __uint_as_float(x[e + 3])));
+            }
+            if (w == 1) *reinterpret_cast<float4 *>(out + HEAD_DIM) = make_float4(M, fmaf(f1, o.y, f0 * a.y), 0.f, 0.f);
+            if (row < rows) {
+                fence_async_proxy();
+                bulk_store(dst + w * 64, smem_u32(out + w * 64), w ? (PART_LD - 64) * 4 : 64 * 4);
+            }
+        } else if (turns > 0) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
@@ -364,36 +407,12 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
                     *reinterpret_cast<uint4 *>(out + c * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
             *reinterpret_cast<float4 *>(out + HEAD_DIM) = make_float4(m, l, 0.f, 0.f);
-        }
-        if (fold) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (w == 0) {
-                const float *other = reinterpret_cast<const float *>(smem + P_OUT) + r * PART_LD;
-                const float4 ml = *reinterpret_cast<const float4 *>(other + HEAD_DIM);
-                const float M = fmaxf(m, ml.x), f0 = fast_exp2(m - M), f1 = fast_exp2(ml.x - M);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(oc + c * 32, o);
-                    tmem_ld_done(o);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 a = *reinterpret_cast<const float4 *>(other + c * 32 + e);
-                        *reinterpret_cast<float4 *>(out + c * 32 + e) =
-                            make_float4(fmaf(f1, a.x, f0 * __uint_as_float(o[e])), fmaf(f1, a.y, f0 * __uint_as_float(o[e + 1])),
-                                        fmaf(f1, a.z, f0 * __uint_as_float(o[e + 2])), fmaf(f1, a.w, f0 * __uint_as_float(o[e + 3])));
-                    }
-                }
-                *reinterpret_cast<float4 *>(out + HEAD_DIM) = make_float4(M, fmaf(f1, ml.y, f0 * l), 0.f, 0.f);
+            if (row < rows) {
+                fence_async_proxy();
+                bulk_store(dst, smem_u32(out), PART_LD * 4);
             }
         }
-        const int row = row0 + (both ? 0 : w * PT) + r;
-        if (row < rows && turns > 0 && !(both && w == 1)) {
-            const int b = row / p.G, g = row - b * p.G;
-            fence_async_proxy();
-            bulk_store(p.part + ((((int64_t)b * p.h_kv + h) * p.splits + split) * p.G + g) * PART_LD, smem_u32(out), PART_LD * 4);
-            bulk_store_wait();
-        }
+        bulk_store_wait_read();
         tcgen05_before_sync();
     }
     __syncwarp();
@@ -405,7 +424,9 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
     }
 }
 
-// The sequences' own rows, and everything merged: grid (own splits, sequence x KV head).  With `listed`, the prefix's rows
+// The sequences' own rows, and everything merged: grid (CTAs, sequence x KV head).  Own rows that one CTA serves alone may be
+// served by several all the same, each for some of the query heads: the partials of a long prefix take longer to join than
+// a few own rows to read (8 sequences of one KV head with 8 query heads, 30,000 + 100 rows: 32 us with one).  With `listed`, the prefix's rows
 // too, as one list ahead of the own ones (short prefixes and small batches, which the second-level cache serves).
 // STAGES tiles of 16 rows per warp: as many as the shared memory allows at the CTAs per SM that the grid makes.
 template <int STAGES>
@@ -417,13 +438,16 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
     const int tid = threadIdx.x, warp = tid >> 5, head = blockIdx.y, split = blockIdx.x, h = head % p.h_kv, G = p.G;
     const int n = own_rows(p, head);
     const int shared_tiles = (p.listed + TILE_ROWS - 1) / TILE_ROWS, tiles = shared_tiles + (n + TILE_ROWS - 1) / TILE_ROWS;
-    const int s_eff = min(p.own_splits, max(1, (tiles + WARPS - 1) / WARPS));
-    if (split >= s_eff) {
+    // tiles of a warp at least before another CTA takes part: four where the prefix's partials have to be joined as well
+    const int least = WARPS * (p.prefix_splits > 0 ? 4 : 1);
+    const int s_eff = min(p.own_splits, max(1, (tiles + least - 1) / least));
+    const int joint = s_eff == 1 ? min((int)gridDim.x, G) : 1;         // CTAs that share the query heads
+    if (split >= max(s_eff, joint)) {
         pdl_wait();
         return;
     }
     const int slots = s_eff * WARPS, per = (tiles + slots - 1) / slots;
-    const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
+    const int t0 = min((s_eff == 1 ? warp : split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
     const char *ko = static_cast<const char *>(p.k) + (int64_t)head * p.ksh * 2, *vo = static_cast<const char *>(p.v) + (int64_t)head * p.vsh * 2;
     WarpAttendT<STAGES> wa;
     wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * G * HEAD_DIM, G, smem + warp * (STAGES * 8192),
@@ -440,17 +464,19 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
     const int parts = p.prefix_splits + s_eff;
     const int64_t slot0 = (int64_t)head * p.splits;
     pdl_wait();                            // the prefix's partials, and whoever read the output before
+    pdl_trigger();
     if (s_eff == 1) {
         // Alone: the prefix's partials straight from where they lie.  Every warp folds a quarter of each row's into its own
         // partial (a lane has four columns; the loads of two query heads are in flight together), then the four are joined.
         constexpr int AT_ONCE = 5;
         const int lane = tid & 31;
-        for (int g0 = 0; g0 < G; g0 += 2) {
+        const int ga = G * split / joint, gb = G * (split + 1) / joint;      // this CTA's query heads
+        for (int g0 = ga; g0 < gb; g0 += 2) {
             float M[2], dn[2];
             float4 nm[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float *r = red + (warp * G + min(g0 + e, G - 1)) * PART_LD;
+                const float *r = red + (warp * G + min(g0 + e, gb - 1)) * PART_LD;
                 M[e] = r[128]; dn[e] = r[129];
                 nm[e] = *reinterpret_cast<const float4 *>(r + lane * 4);
             }
@@ -464,7 +490,7 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
                         ml[e][i] = make_float2(NEG_BIG, 0.f);
                         a[e][i] = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (i0 + i * WARPS < p.prefix_splits) {
-                            const float *r = p.part + ((slot0 + i0 + i * WARPS) * G + min(g0 + e, G - 1)) * PART_LD;
+                            const float *r = p.part + ((slot0 + i0 + i * WARPS) * G + min(g0 + e, gb - 1)) * PART_LD;
                             ml[e][i] = __ldcg(reinterpret_cast<const float2 *>(r + 128));
                             a[e][i] = __ldcg(reinterpret_cast<const float4 *>(r + lane * 4));
                         }
@@ -489,7 +515,7 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                if (g0 + e >= G) continue;
+                if (g0 + e >= gb) continue;
                 float *r = red + (warp * G + g0 + e) * PART_LD;
                 __syncwarp();
                 *reinterpret_cast<float4 *>(r + lane * 4) = nm[e];
@@ -497,7 +523,19 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
             }
         }
         __syncthreads();
-        publish_head<__nv_bfloat16>(p, red, WARPS, head, 0, 1, 0);
+        for (int g = ga; g < gb; ++g) {
+            float M = NEG_BIG, dn = 0.f, nm = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) M = fmaxf(M, red[(w * G + g) * PART_LD + 128]);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float *r = red + (w * G + g) * PART_LD;
+                const float f = fast_exp2(r[128] - M);
+                dn += f * r[129];
+                nm += f * r[tid];
+            }
+            store_out(static_cast<__nv_bfloat16 *>(p.out) + ((int64_t)head * G + g) * HEAD_DIM + tid, dn > 0.f ? nm / dn : 0.f);
+        }
         return;
     }
     publish_head<__nv_bfloat16>(p, red, WARPS, head, p.prefix_splits + split, parts, slot0);
@@ -535,7 +573,7 @@ static int launch_own(const PrefixParams &p, cudaStream_t st) {
     // Behind the prefix's launch, which waits for everything before it, this one may always start early: its own rows are
     // read while the last tiles of the prefix are multiplied.
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.own_splits, p.batch * p.h_kv); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = SMEM; cfg.stream = st;
+    cfg.gridDim = dim3(p.own_ctas, p.batch * p.h_kv); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = SMEM; cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -598,6 +636,9 @@ static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
     p.prefix_splits = ps;
     p.own_splits = own;
     p.listed = ps > 0 ? 0 : p.prefix;
+    int joint = 2 * device_sm_count() / heads;             // two CTAs per SM at most share a head's partials out
+    joint = joint > p.G ? p.G : joint;
+    p.own_ctas = ps > 0 && joint > own ? joint : own;
     if (ps > 0) {
         static bool configured[64] = {};   // the attribute is kept per device
         int dev = 0;
@@ -610,7 +651,7 @@ static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
         const int groups = (p.batch * p.G + 2 * PT - 1) / (2 * PT);
         SKV_CUDA_OK(launch_pdl(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(P_THREADS), P_SMEM, st, p, kmap, vmap));
     }
-    const int ctas = heads * own, sms = device_sm_count();
+    const int ctas = heads * p.own_ctas, sms = device_sm_count();
     return ctas <= sms ? launch_own<6>(p, st) : ctas <= 2 * sms ? launch_own<3>(p, st) : launch_own<2>(p, st);
 }
 

@@ -55,8 +55,9 @@ __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.
 __device__ __forceinline__ void bulk_store(void *dst, uint32_t src, int bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void bulk_store_wait() {
-    asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group 0;" ::: "memory");
+// Until the stores issued by this thread have read their shared memory (the grid's end waits for the rest).
+__device__ __forceinline__ void bulk_store_wait_read() {
+    asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 // ---- tensor memory and matrix products --------------------------------------------------------------------------

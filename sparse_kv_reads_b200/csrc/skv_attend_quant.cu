@@ -3,12 +3,14 @@
 // bf16 queries: tensor-core kernel.  Both products take half-float operands, because a code turns into a half float with
 // one byte permutation or one logic operation: 0x6400 | c is 1024 + c, 0x6400 | c << 4 is 1024 + 16 c.
 //   S^T = K Q^T (16 keys on M, up to 8 query heads on N).  The order of the 128 components is free as long as both sides
-//     agree on it, so a lane takes the bytes it needs straight from global memory, 16 at a time, and the queries are
-//     fetched in the matching order; nothing goes through shared memory.  The offsets (1152 = 1024 + 128 in 8 bits) stay
+//     agree on it, so a lane takes a row's bytes 16 at a time and the queries are fetched in the matching order.  The offsets (1152 = 1024 + 128 in 8 bits) stay
 //     in the codes: the accumulators start at minus the offset times the sum of the query.  Queries are scaled by a power
 //     of two to a largest component in [1, 2), which half floats hold to 2^-25 of that.
 //   O^T = V^T (P vs): component d of the values on M, keys on K.  A lane reads the same bytes of the value rows of its
-//     four keys and pairs them up by permutation.  The value's scale goes into the weights (per scale group in 4 bits).
+//     four keys and pairs them up by permutation.
+// A warp has a ring of tiles of its own in shared memory, filled by 16-byte asynchronous copies and laid out so that neither
+// the rows' nor the columns' reads meet in a bank (loads straight into registers kept one tile in flight per warp: 46 us
+// against XX us for the ragged 8-bit batch, 86 against XX for 64 heads of 32,768 4-bit rows).  The value's scale goes into the weights (per scale group in 4 bits).
 // Two running references per head, in base 2: m for the sum of weights (largest score) and r for the accumulators (largest
 // score + log2 of the value's scale), so that the half floats 2^(z - r) vs keep their precision whatever the scales.  A
 // reference is only raised when something passes it by 8: products up to 256 cost a half float nothing, and most tiles
@@ -32,7 +34,7 @@ struct AttendQuantParams {
     int heads, G, n_group, capacity;
     int ctas;          // CTAs that share the rows
     int splits;        // CTAs per head of the float32 kernel
-    int stage_rows;    // rows of 132 floats of shared memory
+    int rows;          // rows of 132 floats of shared memory
     float scale_log2;
 };
 
@@ -139,7 +141,7 @@ template <int BITS>
 struct RawTile;
 template <>
 struct RawTile<8> {
-    uint4 k[2][2];                                        // [row g, g + 8][16-byte chunk t, t + 4]
+    uint4 k[2][2];                                        // [row g, g + 8][16-byte chunk 2t, 2t + 1]
     uint4 v[4];                                           // chunk g of the four rows
     uint32_t s[2];                                        // (key scale, value scale) of rows g, g + 8
 };
@@ -170,7 +172,7 @@ struct WarpAttendQuant {
         float top = 0.f;
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-            const int d = BITS == 8 ? (s < 4 ? t * 16 + 4 * s : 64 + t * 16 + 4 * (s - 4)) : 32 * (s >> 1) + 8 * t + 4 * (s & 1);
+            const int d = BITS == 8 ? 32 * t + 4 * s : 32 * (s >> 1) + 8 * t + 4 * (s & 1);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (g < G) v = load4(q + g * HEAD_DIM + d);
             x[s][0] = v.x; x[s][1] = v.y; x[s][2] = v.z; x[s][3] = v.w;
@@ -380,49 +382,76 @@ struct WarpAttendQuant {
     }
 };
 
-template <int BITS>
-__device__ __forceinline__ void load_keys(RawTile<BITS> &r, const unsigned char *k, int left, int g) {
+// One warp's ring in shared memory: STAGES tiles of 16 U positions.  8 bits: the 16-byte chunk c of row r lies at place
+// c ^ (r % 8) of the row's 128 bytes.  4 bits: two rows share 128 bytes, chunk c of row r lies at place
+// (4 (r % 2) + c) ^ (2 (r / 2) % 8) of them.  Either way the eight lanes that read together meet no bank twice.
+template <int BITS, int U, int STAGES>
+struct Ring {
+    using Q = Quant<BITS>;
+    static constexpr int ROWS = 16 * U, CODES = ROWS * Q::ROW_BYTES, SCALES = ROWS * Q::SCALES * 2, BYTES = 2 * CODES + SCALES;
+    unsigned char *base;
+    int lane, copy;                                       // this lane's place in a tile as it is copied
+
+    __device__ __forceinline__ explicit Ring(unsigned char *smem) : base(smem), lane(threadIdx.x & 31) {
+        const int eight = lane >> 3;
+        copy = eight * 128 + (((lane & 7) ^ (BITS == 8 ? eight : 2 * eight)) << 4);
+    }
+    // start the copies of a tile, `left` of its positions cached; k, v, s: where the tile begins in memory
+    __device__ __forceinline__ void issue(int stage, const unsigned char *k, const unsigned char *v, const unsigned char *s, int left) {
+        unsigned char *to = base + stage * BYTES;
+        constexpr int PER = 512 / Q::ROW_BYTES;           // rows that the warp copies at once
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const bool ok = g + 8 * h < left;
-        if constexpr (BITS == 8) {
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-            r.k[h][0] = ok ? __ldcs(reinterpret_cast<const uint4 *>(k + h * 1024)) : zero;
-            r.k[h][1] = ok ? __ldcs(reinterpret_cast<const uint4 *>(k + h * 1024 + 64)) : zero;
-        } else {
-            r.k[h] = ok ? __ldcs(reinterpret_cast<const uint4 *>(k + h * 512)) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < ROWS / PER; ++i) {
+            const bool ok = i * PER + lane / (32 / PER) < left;
+            const int at = i * 512 + (BITS == 8 ? copy ^ ((i & 1) << 6) : copy);
+            cp_async16(to + at, ok ? k + i * 512 + lane * 16 : k, ok ? 16 : 0);
+            cp_async16(to + CODES + at, ok ? v + i * 512 + lane * 16 : v, ok ? 16 : 0);
+        }
+        if (lane < ROWS) {
+            const bool ok = lane < left;
+            if (BITS == 4) cp_async16(to + 2 * CODES + lane * 16, ok ? s + lane * 16 : s, ok ? 16 : 0);
+            else {
+                const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(to + 2 * CODES + lane * 4));
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(ok ? s + lane * 4 : s), "r"(ok ? 4 : 0));
+            }
         }
     }
-}
-template <int BITS>
-__device__ __forceinline__ void load_scales(RawTile<BITS> &r, const unsigned char *s, int left, int g) {
+    __device__ __forceinline__ void keys(int stage, int u, RawTile<BITS> &r) const {
+        const int g = lane >> 2, t = lane & 3;
+        const unsigned char *k = base + stage * BYTES + u * 16 * Q::ROW_BYTES, *s = base + stage * BYTES + 2 * CODES;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const bool ok = g + 8 * h < left;
-        if constexpr (BITS == 8) r.s[h] = ok ? __ldcs(reinterpret_cast<const uint32_t *>(s + h * 32)) : 0u;
-        else r.s[h] = ok ? __ldcs(reinterpret_cast<const uint4 *>(s + h * 128)) : make_uint4(0u, 0u, 0u, 0u);
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (BITS == 8) {
+                const unsigned char *row = k + (g + 8 * h) * 128;
+                r.k[h][0] = *reinterpret_cast<const uint4 *>(row + ((2 * t ^ g) << 4));
+                r.k[h][1] = *reinterpret_cast<const uint4 *>(row + (((2 * t + 1) ^ g) << 4));
+                r.s[h] = *reinterpret_cast<const uint32_t *>(s + (16 * u + g + 8 * h) * 4);
+            } else {
+                r.k[h] = *reinterpret_cast<const uint4 *>(k + ((g >> 1) + 4 * h) * 128 + (((((g & 1) << 2) + t) ^ (g & 6)) << 4));
+                r.s[h] = *reinterpret_cast<const uint4 *>(s + (16 * u + g + 8 * h) * 16);
+            }
+        }
     }
-}
-template <int BITS>
-__device__ __forceinline__ void load_values(RawTile<BITS> &r, const unsigned char *v, int left, int t) {
+    __device__ __forceinline__ void values(int stage, int u, RawTile<BITS> &r) const {
+        const int g = lane >> 2, t = lane & 3;
+        const unsigned char *v = base + stage * BYTES + CODES + u * 16 * Q::ROW_BYTES;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = (i & 1) + (i >> 1) * 8;           // beside row 2t
-        const bool ok = 2 * t + row < left;
-        if constexpr (BITS == 8) r.v[i] = ok ? __ldcs(reinterpret_cast<const uint4 *>(v + row * 128)) : make_uint4(0u, 0u, 0u, 0u);
-        else r.v[i] = ok ? __ldcs(reinterpret_cast<const uint2 *>(v + row * 64)) : make_uint2(0u, 0u);
+        for (int i = 0; i < 4; ++i) {                     // rows 2t, 2t + 1, 2t + 8, 2t + 9
+            if constexpr (BITS == 8)
+                r.v[i] = *reinterpret_cast<const uint4 *>(v + (2 * t + (i & 1) + 8 * (i >> 1)) * 128 + ((g ^ (2 * t + (i & 1))) << 4));
+            else
+                r.v[i] = *reinterpret_cast<const uint2 *>(v + (t + 4 * (i >> 1)) * 128 +
+                                                          (((((i & 1) << 2) + (g >> 1)) ^ (2 * t)) << 4) + (g & 1) * 8);
+        }
     }
-}
+};
 
 constexpr int QUANT_CTAS_PER_SM = 3;   // 168 registers a thread
-// Rows of 132 floats of shared memory: the warps' partials of two heads at least, and what the merging CTA stages of a head
-// in one trip.  No more than that: the first-level cache, which the loads in flight pass through, gets the rest (128 heads
-// of 8,191 rows and fewer, four query heads: 46 us with 32 rows per CTA, 53 us with 128).
-constexpr int QUANT_MAX_ROWS = 128;
-static int quant_stage_rows(int heads, int G, int ctas) {
-    const int merge = (ctas / heads + 1) * G;
-    return merge < 8 * G ? 8 * G : merge > QUANT_MAX_ROWS ? QUANT_MAX_ROWS : merge;
-}
+constexpr int QUANT_MAX_SEG = 32;       // heads of a CTA whose partials wait in shared memory
+// Rows of 132 floats of shared memory behind the rings: the warps' partials of one head of eight query heads, of two and
+// more heads of fewer.  (The CTA that merges a head stages its partials over rings and rows alike.)
+constexpr int QUANT_MOST_ROWS = 32;
+static int quant_rows(int G) { return 8 * G < 16 ? 16 : 8 * G > QUANT_MOST_ROWS ? QUANT_MOST_ROWS : 8 * G; }
 
 // The ways of sharing the work out, below, in blocks of 16 rows.  Measured on B200 (8-bit rows, two query heads, us):
 // ALONE: a head up to this long is left to one CTA, without a merge (32 blocks: 8.2, in two parts 9.7; 63 blocks: 10.2 and
@@ -452,11 +481,13 @@ struct QuantSegment {
     int64_t slot0;
 };
 
-template <int BITS, int U>
+template <int BITS, int U, int STAGES>
 __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kernel(const AttendQuantParams p) {
     using Q = Quant<BITS>;
-    constexpr int WARPS = 4, ROWS = 16 * U, MAX_SEG = QUANT_MAX_ROWS / WARPS;
-    extern __shared__ __align__(16) float red[];          // stage_rows x 132
+    using Tiles = Ring<BITS, U, STAGES>;
+    constexpr int WARPS = 4, ROWS = 16 * U, MAX_SEG = QUANT_MAX_SEG;
+    extern __shared__ __align__(128) unsigned char smem[];    // the warps' rings, then rows x 132 floats
+    float *const red = reinterpret_cast<float *>(smem + WARPS * STAGES * Tiles::BYTES);
     __shared__ int s_scan[40];
     __shared__ float s_max[32];
     // (kept here, the tile loop needs the registers)
@@ -464,7 +495,7 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
     __shared__ int s_ctas, s_even, s_head[WARPS], s_b0[WARPS];
     __shared__ QuantSegment s_seg[MAX_SEG];
     __shared__ int s_last[MAX_SEG];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     pdl_trigger();
     const int group = p.n_group > 0 ? min(p.n_group, p.heads) : p.heads;
@@ -530,7 +561,8 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
     }
     if (tid == 0) s_even = even;
     __syncthreads();
-    const int seg_cap = p.stage_rows / (WARPS * p.G), seg_floats = WARPS * p.G * PART_LD;
+    const int seg_cap = min(MAX_SEG, p.rows / (WARPS * p.G)), seg_floats = WARPS * p.G * PART_LD;
+    Tiles ring(smem + warp * STAGES * Tiles::BYTES);
     for (bool more = true; more;) {
         int segs = 0;
         while (segs < seg_cap) {
@@ -553,35 +585,38 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
             const int per = (b1 - b0 + WARPS - 1) / WARPS;
             const int r0 = min((b0 + warp * per) * 16, n), r1 = min((b0 + min((warp + 1) * per, b1 - b0)) * 16, n);
             const int64_t row0 = (int64_t)head * p.capacity + r0;
-            const unsigned char *k = p.kc + (row0 + g) * Q::ROW_BYTES + t * 16;
-            const unsigned char *v = p.vc + (row0 + 2 * t) * Q::ROW_BYTES + g * (Q::ROW_BYTES / 8);
-            const unsigned char *s = reinterpret_cast<const unsigned char *>(p.scale) + (row0 + g) * Q::SCALES * 2;
-            RawTile<BITS> r[U];
+            const unsigned char *k = p.kc + row0 * Q::ROW_BYTES, *v = p.vc + row0 * Q::ROW_BYTES;
+            const unsigned char *s = reinterpret_cast<const unsigned char *>(p.scale) + row0 * Q::SCALES * 2;
+            int ahead = r1 - r0, put = 0, get = 0;        // positions not asked for yet; stages
+            auto more_rows = [&]() {
+                if (ahead > 0) ring.issue(put, k, v, s, ahead);
+                cp_async_commit();
+                ahead -= ROWS;
+                k += ROWS * Q::ROW_BYTES; v += ROWS * Q::ROW_BYTES; s += ROWS * Q::SCALES * 2;
+                put = put + 1 == STAGES ? 0 : put + 1;
+            };
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, r1 - r0 - 16 * u, g);
-                load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, r1 - r0 - 16 * u, g);
-                load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, r1 - r0 - 16 * u, t);
-            }
+            for (int i = 0; i < STAGES - 1; ++i) more_rows();
             WarpAttendQuant<BITS> wa;
             wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * p.G * HEAD_DIM, p.G, p.scale_log2);
             for (int left = r1 - r0; left > 0; left -= ROWS) {
-                // a part's registers take the next tile's as soon as they are used up: a whole tile is always in flight
-                const int next = left - ROWS;
-                k += ROWS * Q::ROW_BYTES; v += ROWS * Q::ROW_BYTES; s += ROWS * Q::SCALES * 2;
+                more_rows();
+                cp_async_wait<STAGES - 1>();
+                __syncwarp();
+                RawTile<BITS> r[U];
                 float z[U][4];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
+                    ring.keys(get, u, r[u]);
                     wa.scores(r[u], z[u]);
-                    load_keys<BITS>(r[u], k + u * 16 * Q::ROW_BYTES, next - 16 * u, g);
                 }
-                wa.consume(r, z, left);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    load_scales<BITS>(r[u], s + u * 32 * Q::SCALES, next - 16 * u, g);
-                    load_values<BITS>(r[u], v + u * 16 * Q::ROW_BYTES, next - 16 * u, t);
-                }
+                for (int u = 0; u < U; ++u) ring.values(get, u, r[u]);
+                wa.consume(r, z, left);
+                __syncwarp();                             // the stage may be filled again
+                get = get + 1 == STAGES ? 0 : get + 1;
             }
+            cp_async_wait<0>();
             wa.store_partial(red + segs * seg_floats, warp, p.G);
             ++segs;
         }
@@ -602,25 +637,28 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
             __syncthreads();
             __threadfence();
             for (int i = 0; i < segs; ++i)
-                if (s_last[i]) merge_head<__nv_bfloat16>(p, s_seg[i].head, s_seg[i].parts, s_seg[i].slot0, red, p.stage_rows);
+                if (s_last[i]) merge_head<__nv_bfloat16>(p, s_seg[i].head, s_seg[i].parts, s_seg[i].slot0,
+                                                         reinterpret_cast<float *>(smem),
+                                                         p.rows + WARPS * STAGES * Tiles::BYTES / (PART_LD * 4));
         }
         __syncthreads();                                  // the next heads' partials go where these were
     }
 }
 
-template <int BITS, int U>
+template <int BITS, int U, int STAGES>
 static int launch_quant_mma(const AttendQuantParams &p, cudaStream_t st) {
-    auto kern = attend_quant_mma_kernel<BITS, U>;
-    constexpr int SMEM = QUANT_MAX_ROWS * PART_LD * 4;
+    auto kern = attend_quant_mma_kernel<BITS, U, STAGES>;
+    constexpr int RINGS = 4 * STAGES * Ring<BITS, U, STAGES>::BYTES;
+    static_assert(QUANT_CTAS_PER_SM * (RINGS + QUANT_MOST_ROWS * PART_LD * 4 + 4096) <= 227 * 1024, "the CTAs of an SM fit at eight query heads");
     static bool configured[64] = {};       // the attribute is kept per device
     int dev = 0;
     SKV_CUDA_OK(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return SKV_E_RANGE;
     if (!configured[dev]) {
-        SKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        SKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RINGS + QUANT_MOST_ROWS * PART_LD * 4));
         configured[dev] = true;
     }
-    SKV_CUDA_OK(launch_pdl(kern, dim3(p.ctas), dim3(128), (size_t)p.stage_rows * PART_LD * 4, st, p));
+    SKV_CUDA_OK(launch_pdl(kern, dim3(p.ctas), dim3(128), (size_t)RINGS + (size_t)p.rows * PART_LD * 4, st, p));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -660,7 +698,7 @@ extern "C" int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, i
     AttendQuantParams p;
     p.heads = c->batch * c->h_kv; p.G = G; p.n_group = n_group; p.capacity = c->capacity;
     p.ctas = ctas; p.splits = (ctas + p.heads) / p.heads;
-    p.stage_rows = quant_stage_rows(p.heads, G, ctas);
+    p.rows = quant_rows(G);
     p.q = q; p.out = out; p.n_dev = n_dev;
     p.kc = static_cast<const unsigned char *>(c->k); p.vc = static_cast<const unsigned char *>(c->v);
     p.scale = static_cast<const __nv_bfloat16 *>(c->scale);
@@ -669,5 +707,5 @@ extern "C" int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, i
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_F32) return c->bits == 8 ? launch_quant_simple<float, 8>(p, st) : launch_quant_simple<float, 4>(p, st);
-    return c->bits == 8 ? launch_quant_mma<8, 2>(p, st) : launch_quant_mma<4, 2>(p, st);
+    return c->bits == 8 ? launch_quant_mma<8, 1, 3>(p, st) : launch_quant_mma<4, 2, 3>(p, st);
 }

@@ -32,10 +32,11 @@ static const DevProps &props() {
 
 int device_sm_count() { return props().sms; }
 static bool g_pdl = false;
-bool pdl_enabled() {
+bool pdl_allowed() {
     static const bool allowed = [] { const char *e = getenv("SKV_PDL"); return !(e && e[0] == '0'); }();
-    return allowed && g_pdl;
+    return allowed;
 }
+bool pdl_enabled() { return pdl_allowed() && g_pdl; }
 int device_max_smem_optin() { return props().smem_optin; }
 
 }  // namespace skv

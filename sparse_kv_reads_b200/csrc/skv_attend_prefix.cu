@@ -166,8 +166,6 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
         s_fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_proxy();
-        // the first keys are on their way before anything else: no earlier kernel of the same step writes the prefix
-        if (n > 0) load(kmap, kbase, b_kfull, t0);
     }
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
     pdl_wait();
@@ -191,8 +189,7 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
             }
         }
         if (tid == 256) {
-            if (n > 0) load(vmap, kbase + P_TILE, b_vfull, t0);
-            for (int i = 1; i < min(n, PSTAGES); ++i) {
+            for (int i = 0; i < min(n, PSTAGES); ++i) {
                 load(kmap, kbase + i * 2 * P_TILE, b_kfull + 8 * i, t0 + i);
                 load(vmap, kbase + i * 2 * P_TILE + P_TILE, b_vfull + 8 * i, t0 + i);
             }
@@ -572,14 +569,8 @@ static int launch_own(const PrefixParams &p, cudaStream_t st) {
     }
     // Behind the prefix's launch, which waits for everything before it, this one may always start early: its own rows are
     // read while the last tiles of the prefix are multiplied.
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.own_ctas, p.batch * p.h_kv); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = SMEM; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.prefix_splits > 0 ? 1 : 0;
-    SKV_CUDA_OK(cudaLaunchKernelEx(&cfg, prefix_own_kernel<STAGES>, p));
+    SKV_CUDA_OK(launch_as(pdl_allowed() && p.prefix_splits > 0, prefix_own_kernel<STAGES>, dim3(p.own_ctas, p.batch * p.h_kv), dim3(128),
+                          SMEM, st, p));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -649,7 +640,7 @@ static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
             configured[dev] = true;
         }
         const int groups = (p.batch * p.G + 2 * PT - 1) / (2 * PT);
-        SKV_CUDA_OK(launch_pdl(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(P_THREADS), P_SMEM, st, p, kmap, vmap));
+        SKV_CUDA_OK(launch_early(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(P_THREADS), P_SMEM, st, p, kmap, vmap));
     }
     const int ctas = heads * p.own_ctas, sms = device_sm_count();
     return ctas <= sms ? launch_own<6>(p, st) : ctas <= 2 * sms ? launch_own<3>(p, st) : launch_own<2>(p, st);

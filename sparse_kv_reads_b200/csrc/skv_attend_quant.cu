@@ -446,7 +446,7 @@ struct Ring {
     }
 };
 
-constexpr int QUANT_CTAS_PER_SM = 3;   // 168 registers a thread
+constexpr int QUANT_CTAS_PER_SM = 2;
 constexpr int QUANT_MAX_SEG = 32;       // heads of a CTA whose partials wait in shared memory
 // Rows of 132 floats of shared memory behind the rings: the warps' partials of one head of eight query heads, of two and
 // more heads of fewer.  (The CTA that merges a head stages its partials over rings and rows alike.)
@@ -658,7 +658,7 @@ static int launch_quant_mma(const AttendQuantParams &p, cudaStream_t st) {
         SKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RINGS + QUANT_MOST_ROWS * PART_LD * 4));
         configured[dev] = true;
     }
-    SKV_CUDA_OK(launch_pdl(kern, dim3(p.ctas), dim3(128), (size_t)RINGS + (size_t)p.rows * PART_LD * 4, st, p));
+    SKV_CUDA_OK(launch_early(kern, dim3(p.ctas), dim3(128), (size_t)RINGS + (size_t)p.rows * PART_LD * 4, st, p));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -707,5 +707,5 @@ extern "C" int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, i
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == SKV_F32) return c->bits == 8 ? launch_quant_simple<float, 8>(p, st) : launch_quant_simple<float, 4>(p, st);
-    return c->bits == 8 ? launch_quant_mma<8, 1, 3>(p, st) : launch_quant_mma<4, 2, 3>(p, st);
+    return c->bits == 8 ? launch_quant_mma<8, 2, 2>(p, st) : launch_quant_mma<4, 2, 3>(p, st);
 }

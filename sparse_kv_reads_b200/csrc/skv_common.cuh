@@ -30,6 +30,7 @@ static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t
 int device_sm_count();
 int device_max_smem_optin();
 bool pdl_enabled();
+bool pdl_allowed();
 
 // Programmatic dependent launch.  A kernel launched through launch_pdl may start while the kernel before it
 // on the stream is still running; everything it reads from that kernel (and every write it makes) must come
@@ -42,16 +43,28 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... KArgs, typename... Args>
-static inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                                     Args... args) {
+static inline cudaError_t launch_as(bool early, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                    cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    cfg.numAttrs = early ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+static inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                     Args... args) {
+    return launch_as(pdl_enabled(), kern, grid, block, smem, stream, args...);
+}
+// The same for kernels that touch no memory another kernel writes before their pdl_wait(): they may start early behind any
+// kernel, whoever launches it, so the switch of skv_set_overlap is not asked (SKV_PDL=0 still keeps it off).
+template <typename... KArgs, typename... Args>
+static inline cudaError_t launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                       Args... args) {
+    return launch_as(pdl_allowed(), kern, grid, block, smem, stream, args...);
 }
 
 // Cached positions of head `head`: runs of `n_group` consecutive heads share one entry of n_dev (a batch whose

@@ -135,6 +135,8 @@ template <typename T, int BITS, bool FLAT>
 __global__ void __launch_bounds__(256) quant_write_kernel(const RowsParams p) {
     using Q = Quant<BITS>;
     constexpr bool EXACT = sizeof(T) == 4;
+    pdl_wait();
+    pdl_trigger();
     const int sub = threadIdx.x & 15;
     const unsigned hmask = (threadIdx.x & 16) ? 0xffff0000u : 0x0000ffffu;
     const Places<FLAT> w(p);                               // (everything about a position is uniform within its half warp)
@@ -227,6 +229,8 @@ __device__ __forceinline__ void store_values(__nv_bfloat16 *out, const Stored<BI
 template <typename T, int BITS, bool FLAT>
 __global__ void __launch_bounds__(256) quant_read_kernel(const RowsParams p) {
     using Q = Quant<BITS>;
+    pdl_wait();
+    pdl_trigger();
     const int sub = threadIdx.x & 15;
     const Places<FLAT> w(p);
     constexpr int N = Places<FLAT>::N;
@@ -313,14 +317,14 @@ static dim3 rows_grid(const RowsParams &p) {
     return dim3((unsigned)(p.tokens + 16 * AT_ONCE - 1) / (16 * AT_ONCE), (unsigned)p.h_kv, (unsigned)p.batch);
 }
 template <typename T, int BITS>
-static void launch_write(const RowsParams &p, cudaStream_t st) {
-    if (rows_flat(p)) quant_write_kernel<T, BITS, true><<<rows_grid(p), 256, 0, st>>>(p);
-    else quant_write_kernel<T, BITS, false><<<rows_grid(p), 256, 0, st>>>(p);
+static cudaError_t launch_write(const RowsParams &p, cudaStream_t st) {
+    auto kern = rows_flat(p) ? quant_write_kernel<T, BITS, true> : quant_write_kernel<T, BITS, false>;
+    return launch_early(kern, rows_grid(p), dim3(256), 0, st, p);
 }
 template <typename T, int BITS>
-static void launch_read(const RowsParams &p, cudaStream_t st) {
-    if (rows_flat(p)) quant_read_kernel<T, BITS, true><<<rows_grid(p), 256, 0, st>>>(p);
-    else quant_read_kernel<T, BITS, false><<<rows_grid(p), 256, 0, st>>>(p);
+static cudaError_t launch_read(const RowsParams &p, cudaStream_t st) {
+    auto kern = rows_flat(p) ? quant_read_kernel<T, BITS, true> : quant_read_kernel<T, BITS, false>;
+    return launch_early(kern, rows_grid(p), dim3(256), 0, st, p);
 }
 
 static int rows_check(const skv_qcache *c, const void *k, const void *v, int dtype, int batch, int tokens, int64_t kb,
@@ -362,10 +366,8 @@ extern "C" int skv_quant_write(const skv_qcache *c, const void *k, const void *v
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == SKV_BF16 && c->bits == 8) launch_write<__nv_bfloat16, 8>(p, st);
-    else if (dtype == SKV_BF16) launch_write<__nv_bfloat16, 4>(p, st);
-    else if (c->bits == 8) launch_write<float, 8>(p, st);
-    else launch_write<float, 4>(p, st);
+    if (dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_write<__nv_bfloat16, 8>(p, st) : launch_write<__nv_bfloat16, 4>(p, st)));
+    else SKV_CUDA_OK((c->bits == 8 ? launch_write<float, 8>(p, st) : launch_write<float, 4>(p, st)));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -381,10 +383,8 @@ extern "C" int skv_quant_read(const skv_qcache *c, void *k, void *v, int dtype, 
     if (tokens == 0) return SKV_OK;
     p.pos_per_seq = pos_per_seq;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == SKV_BF16 && c->bits == 8) launch_read<__nv_bfloat16, 8>(p, st);
-    else if (dtype == SKV_BF16) launch_read<__nv_bfloat16, 4>(p, st);
-    else if (c->bits == 8) launch_read<float, 8>(p, st);
-    else launch_read<float, 4>(p, st);
+    if (dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_read<__nv_bfloat16, 8>(p, st) : launch_read<__nv_bfloat16, 4>(p, st)));
+    else SKV_CUDA_OK((c->bits == 8 ? launch_read<float, 8>(p, st) : launch_read<float, 4>(p, st)));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }

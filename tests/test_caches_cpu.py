@@ -97,7 +97,7 @@ def test_attention_over_quantised_rows_is_refused_on_the_host(L):
         assert call(**{name: None}) == -1
     assert call(dtype=2) == -3 and call(G=0) == -2 and call(G=9) == -2 and call(ctas=0) == -5 and call(ng=-1) == -5
     assert call(q=0x1008) == -4 and call(out=0x1002) == -4 and call(ws=0x1008) == -4
-    assert L.skv_quant_ctas() == 3 * 148 and L.skv_quant_workspace_bytes(8, 2, 128, 444) == 452 * 2 * 528 + 256
+    assert L.skv_quant_ctas() == 2 * 148 and L.skv_quant_workspace_bytes(8, 2, 128, 444) == 452 * 2 * 528 + 256
     assert L.skv_quant_workspace_bytes(0, 2, 128, 4) == -5 and L.skv_quant_workspace_bytes(8, 9, 128, 4) == -2
 
 

@@ -446,18 +446,25 @@ typedef struct skv_qcache {
     int32_t reserved;
 } skv_qcache;
 
-/* Quantises rows as they are written: k, v [batch, h_kv, tokens, 128] (dtype; element strides, unit last stride, rows
- * 16-byte aligned) into rows [first, first + tokens) of the first `batch` sequences; first = pos[0], or pos[sequence]
- * with pos_per_seq, in device memory, or pos0 where pos is null.  Rows that fall outside the cache by a device position
- * are left out and recorded (SKV_ST_BAD_INDEX); a pos0 outside is SKV_E_RANGE. */
-int skv_quant_write(const skv_qcache *c, const void *k, const void *v, int dtype, int batch, int tokens,
-                    int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride, int64_t v_batch_stride,
-                    int64_t v_head_stride, int64_t v_row_stride, const int64_t *pos, int pos_per_seq, int64_t pos0,
-                    void *stream);
+/* Rows of a call below: k, v [batch, h_kv, tokens, 128] (dtype; element strides, unit last stride, rows 16-byte aligned) and
+ * the cache rows [first, first + tokens) of the first `batch` sequences; first = pos[0], or pos[sequence] with pos_per_seq, in
+ * device memory, or pos0 where pos is null. */
+typedef struct skv_rows {
+    void *k, *v;
+    const int64_t *pos;
+    int64_t pos0;
+    int64_t k_batch_stride, k_head_stride, k_row_stride, v_batch_stride, v_head_stride, v_row_stride;
+    int32_t pos_per_seq;
+    int32_t dtype;
+    int32_t batch;
+    int32_t tokens;
+} skv_rows;
+
+/* Quantises rows as they are written.  Rows that fall outside the cache by a device position are left out and recorded
+ * (SKV_ST_BAD_INDEX); a pos0 outside is SKV_E_RANGE. */
+int skv_quant_write(const skv_qcache *c, const skv_rows *rows, void *stream);
 /* The way back: value = code * scale, rounded once to dtype.  Rows outside the cache come back as zeros, recorded. */
-int skv_quant_read(const skv_qcache *c, void *k, void *v, int dtype, int batch, int tokens, int64_t k_batch_stride,
-                   int64_t k_head_stride, int64_t k_row_stride, int64_t v_batch_stride, int64_t v_head_stride,
-                   int64_t v_row_stride, const int64_t *pos, int pos_per_seq, int64_t pos0, void *stream);
+int skv_quant_read(const skv_qcache *c, const skv_rows *rows, void *stream);
 /* skv_qk_rope_cache with a quantised cache: the same queries, and the key and value rows that skv_quant_write would store
  * of that call's cache rows.  qkv [batch, (H + 2 h_kv) * 128] bf16; the tables need `capacity` rows.  A position outside
  * the cache is recorded and its sequence left out. */

@@ -52,6 +52,14 @@ class SkvQCache(C.Structure):
                 ("bits", C.c_int32), ("reserved", C.c_int32)]
 
 
+class SkvRows(C.Structure):
+    """``skv_rows`` of include/skv.h: the rows of one write into or read from a quantised cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("pos", C.c_void_p), ("pos0", C.c_int64),
+                ("k_batch_stride", C.c_int64), ("k_head_stride", C.c_int64), ("k_row_stride", C.c_int64),
+                ("v_batch_stride", C.c_int64), ("v_head_stride", C.c_int64), ("v_row_stride", C.c_int64),
+                ("pos_per_seq", C.c_int32), ("dtype", C.c_int32), ("batch", C.c_int32), ("tokens", C.c_int32)]
+
+
 class SkvState(C.Structure):
     """Mirror of ``struct skv_state``."""
     _fields_ = [("heads", C.c_int32), ("C", C.c_int32), ("d", C.c_int32), ("capacity", C.c_int32),
@@ -159,7 +167,7 @@ def _declare(lib) -> None:
     lib.skv_gemv.argtypes = [vp, i32, i32, vp, i32, i32, vp, vp, vp, vp, vp, f32, vp]
     qc = C.POINTER(SkvQCache)
     lib.skv_quant_write.restype = i32
-    lib.skv_quant_write.argtypes = [qc, vp, vp, i32, i32, i32, i64, i64, i64, i64, i64, i64, vp, i32, i64, vp]
+    lib.skv_quant_write.argtypes = [qc, C.POINTER(SkvRows), vp]
     lib.skv_quant_read.restype = i32
     lib.skv_quant_read.argtypes = lib.skv_quant_write.argtypes
     lib.skv_qk_rope_quant.restype = i32
@@ -226,23 +234,10 @@ def dtype_code(dt: torch.dtype) -> int:
     raise ValueError(f"unsupported cache dtype {dt}; the kernels take bfloat16 or float32")
 
 
-class _Nothing:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NOTHING = _Nothing()
-
-
-def on_device(device):
-    """Context in which ``device`` is the current CUDA device: a launch goes to the current device, a caller's tensors
-    may live on another."""
-    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
-        return _NOTHING
-    return torch.cuda.device(device)
+def elsewhere(device) -> bool:
+    """Whether another CUDA device than ``device`` (given with its index) is the current one: a launch goes to the current
+    device, a caller's tensors may live on another."""
+    return device.type == "cuda" and device.index != torch._C._cuda_getDevice()
 
 
 def stream_ptr(device=None) -> int:

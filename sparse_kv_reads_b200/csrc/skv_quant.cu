@@ -355,35 +355,31 @@ static int rows_check(const skv_qcache *c, const void *k, const void *v, int dty
 
 using namespace skv;
 
-extern "C" int skv_quant_write(const skv_qcache *c, const void *k, const void *v, int dtype, int batch, int tokens,
-                               int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
-                               int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride, const int64_t *pos,
-                               int pos_per_seq, int64_t pos0, void *stream) {
+extern "C" int skv_quant_write(const skv_qcache *c, const skv_rows *r, void *stream) {
+    if (!r) return SKV_E_NULL;
     RowsParams p;
-    const int rc = rows_check(c, k, v, dtype, batch, tokens, k_batch_stride, k_head_stride, k_row_stride, v_batch_stride,
-                              v_head_stride, v_row_stride, pos, pos0, p);
+    const int rc = rows_check(c, r->k, r->v, r->dtype, r->batch, r->tokens, r->k_batch_stride, r->k_head_stride, r->k_row_stride,
+                              r->v_batch_stride, r->v_head_stride, r->v_row_stride, r->pos, r->pos0, p);
     if (rc) return rc;
-    if (tokens == 0) return SKV_OK;
-    p.pos_per_seq = pos_per_seq;
+    if (r->tokens == 0) return SKV_OK;
+    p.pos_per_seq = r->pos_per_seq;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_write<__nv_bfloat16, 8>(p, st) : launch_write<__nv_bfloat16, 4>(p, st)));
+    if (r->dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_write<__nv_bfloat16, 8>(p, st) : launch_write<__nv_bfloat16, 4>(p, st)));
     else SKV_CUDA_OK((c->bits == 8 ? launch_write<float, 8>(p, st) : launch_write<float, 4>(p, st)));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
 
-extern "C" int skv_quant_read(const skv_qcache *c, void *k, void *v, int dtype, int batch, int tokens,
-                              int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
-                              int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride, const int64_t *pos,
-                              int pos_per_seq, int64_t pos0, void *stream) {
+extern "C" int skv_quant_read(const skv_qcache *c, const skv_rows *r, void *stream) {
+    if (!r) return SKV_E_NULL;
     RowsParams p;
-    const int rc = rows_check(c, k, v, dtype, batch, tokens, k_batch_stride, k_head_stride, k_row_stride, v_batch_stride,
-                              v_head_stride, v_row_stride, pos, pos0, p);
+    const int rc = rows_check(c, r->k, r->v, r->dtype, r->batch, r->tokens, r->k_batch_stride, r->k_head_stride, r->k_row_stride,
+                              r->v_batch_stride, r->v_head_stride, r->v_row_stride, r->pos, r->pos0, p);
     if (rc) return rc;
-    if (tokens == 0) return SKV_OK;
-    p.pos_per_seq = pos_per_seq;
+    if (r->tokens == 0) return SKV_OK;
+    p.pos_per_seq = r->pos_per_seq;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_read<__nv_bfloat16, 8>(p, st) : launch_read<__nv_bfloat16, 4>(p, st)));
+    if (r->dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_read<__nv_bfloat16, 8>(p, st) : launch_read<__nv_bfloat16, 4>(p, st)));
     else SKV_CUDA_OK((c->bits == 8 ? launch_read<float, 8>(p, st) : launch_read<float, 4>(p, st)));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;

@@ -4,10 +4,11 @@ rows exist once, each sequence keeps only the rows behind it, and a decode step 
 from __future__ import annotations
 
 import math
+from contextlib import nullcontext
 
 import torch
 
-from ._lib import SkvError, check, dtype_code, lib, on_device, stream_ptr
+from ._lib import SkvError, check, dtype_code, elsewhere, lib, stream_ptr
 from .qwen3 import KVCache
 
 __all__ = ["PrefixKVCache", "PrefixAttentionGraph"]
@@ -81,7 +82,7 @@ class PrefixAttentionGraph:
         self.n_group = 0                                   # KV heads per entry of the device-side lengths (0: one length)
         self.dtype = dtype
         self._code = dtype_code(dtype)
-        with on_device(torch.device(device)):
+        with torch.cuda.device(device) if torch.device(device).type == "cuda" else nullcontext():
             self.num_splits = L.skv_prefix_splits(B, H_kv, self.G, self._code)
             size = L.skv_prefix_workspace_bytes(B, H_kv, self.G, d, self.num_splits) if self.num_splits > 0 \
                 else self.num_splits
@@ -123,11 +124,12 @@ class PrefixAttentionGraph:
         if not q.is_contiguous() or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
         ks, vs, pks, pvs = layout[5], layout[7], layout[1], layout[3]
-        with on_device(dev):
-            check(lib().skv_attend_prefix(q.data_ptr(), Kp.data_ptr(), Vp.data_ptr(), layout[0][1], K.data_ptr(),
-                                          V.data_ptr(), n_dev.data_ptr(), self.n_group, self.out.data_ptr(),
-                                          self.ws.data_ptr(), self.status.data_ptr(), self.B, self.H_kv, self.G, self.d,
-                                          self._code, pks[0], pks[1], pvs[0], pvs[1], ks[0], ks[1], vs[0], vs[1],
-                                          layout[4][1], self.num_splits, self._scale, stream_ptr(dev)),
-                  "skv_attend_prefix")
+        if elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self(q, Kp, Vp, K, V, n_dev)
+        check(lib().skv_attend_prefix(q.data_ptr(), Kp.data_ptr(), Vp.data_ptr(), layout[0][1], K.data_ptr(), V.data_ptr(),
+                                      n_dev.data_ptr(), self.n_group, self.out.data_ptr(), self.ws.data_ptr(),
+                                      self.status.data_ptr(), self.B, self.H_kv, self.G, self.d, self._code, pks[0], pks[1],
+                                      pvs[0], pvs[1], ks[0], ks[1], vs[0], vs[1], layout[4][1], self.num_splits, self._scale,
+                                      stream_ptr(dev)), "skv_attend_prefix")
         return self.out

@@ -10,10 +10,12 @@ the order ``(run % 8, run // 8)``, the lower nibble of a byte first.  Values hav
 from __future__ import annotations
 
 import math
+import threading
+from contextlib import nullcontext
 
 import torch
 
-from ._lib import SkvQCache, SkvError, check, dtype_code, lib, on_device, stream_ptr
+from ._lib import SkvError, SkvQCache, SkvRows, check, dtype_code, elsewhere, lib, stream_ptr
 
 __all__ = ["QuantKVCache", "QuantAttentionGraph"]
 
@@ -60,7 +62,7 @@ class QuantKVCache:
         self.batch, self.h_kv, self.max_seq_len, _ = k[0].shape
         self.d, self.device = 128, k[0].device
         self.cur_len = 0
-        self._plans = {}
+        self._kept = threading.local()                     # plans of writes and reads (below), one set per thread
         self.status = torch.zeros(self.batch * self.h_kv, dtype=torch.int32, device=self.device) if status is None else status
         self._st = [SkvQCache(a.data_ptr(), b.data_ptr(), s.data_ptr(), self.status.data_ptr(), self.batch, self.h_kv,
                               self.max_seq_len, self.d, bits, 0) for a, b, s in zip(k, v, scale)]
@@ -78,78 +80,90 @@ class QuantKVCache:
             bits |= s
         return bits
 
-    def _where(self, pos, b: int, count: int):
-        """``pos`` as (device address or None, one per sequence, host value), the host value checked."""
+    def _where(self, rows: SkvRows, pos, b: int, count: int) -> None:
+        """Set the call's position, checked where the host knows it."""
         if torch.is_tensor(pos):
             if pos.dtype is not torch.long or pos.device != self.device or pos.dim() != 1 or not pos.is_contiguous() \
                     or pos.shape[0] not in (1, b):
                 raise ValueError("positions are an int, or int64 [1] or [sequences] on the cache's device")
-            return pos.data_ptr(), int(pos.shape[0] != 1), 0
+            rows.pos, rows.pos_per_seq = pos.data_ptr(), int(pos.shape[0] != 1)
+            return
         at = int(pos)
         if not 0 <= at <= self.max_seq_len - count:
             raise ValueError(f"rows [{at}, {at + count}) lie outside the cache's {self.max_seq_len} positions")
-        return None, 0, at
+        rows.pos, rows.pos_per_seq, rows.pos0 = None, 0, at
 
-    def _plan(self, k: torch.Tensor, v: torch.Tensor):
-        """What a write of tensors of these shapes, strides and types passes on: the type's code, sizes and strides; no
-        strides where the rows have to be copied first (a last stride other than 1, rows off the 16-byte boundaries)."""
+    def _plan(self, key, make):
+        """What calls of one shape and type have in common, checked once (a decode step makes the same call again and
+        again).  Per thread: the struct is filled in and read by the call."""
+        kept = self._kept.__dict__
+        plan = kept.get(key)
+        if plan is None:
+            if len(kept) >= 256:
+                kept.clear()
+            plan = kept[key] = make()
+        return plan
+
+    def _plan_write(self, k: torch.Tensor, v: torch.Tensor):
+        """``(rows, straight)``; not straight: the rows have to be copied first (a last stride other than 1, rows off the
+        16-byte boundaries)."""
         if k.dim() != 4 or k.shape != v.shape or k.shape[1] != self.h_kv or k.shape[3] != self.d or k.shape[0] > self.batch:
             raise ValueError(f"keys and values must be [sequences <= {self.batch}, {self.h_kv}, tokens, {self.d}]")
         if k.dtype != v.dtype:
             raise ValueError("keys and values must be of one type, on the cache's device")
         if k.shape[2] > self.max_seq_len:
             raise ValueError(f"{k.shape[2]} rows do not fit the cache's {self.max_seq_len} positions")
-        head = (dtype_code(k.dtype), k.shape[0], k.shape[2])
-        per16 = 16 // k.element_size()
         strides = k.stride()[:3] + v.stride()[:3]
-        straight = k.stride(3) == v.stride(3) == 1 and not any(s % per16 for s in strides)
-        return head, strides if straight else None
+        straight = k.stride(3) == v.stride(3) == 1 and not any(s % (16 // k.element_size()) for s in strides)
+        return SkvRows(0, 0, None, 0, *strides, 0, dtype_code(k.dtype), k.shape[0], k.shape[2]), straight
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, pos) -> None:
         """Quantise ``k, v [b, H_kv, T, 128]`` (bf16 or float32, any strides) into the rows ``[pos, pos + T)`` of the
         first ``b`` sequences.  ``pos``: an int, or int64 in device memory, one for all or one per sequence; rows of a
         device position that fall outside the cache are left out and recorded in ``status``."""
-        key = (k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype)
-        plan = self._plans.get(key)                        # (a decode step writes the same shape again and again)
-        if plan is None:
-            plan = self._plan(k, v)
-            if len(self._plans) >= 256:
-                self._plans.clear()
-            self._plans[key] = plan
-        if k.device != self.device or v.device != self.device:
+        rows, straight = self._plan((k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype), lambda: self._plan_write(k, v))
+        dev = self.device
+        if k.device != dev or v.device != dev:
             raise ValueError("keys and values must be of one type, on the cache's device")
         if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
             raise ValueError("a quantised cache has no gradient: write under torch.no_grad()")
-        (code, b, T), strides = plan
-        at, per_seq, host = self._where(pos, b, T)
-        if b == 0 or T == 0:
-            return
         kp, vp = k.data_ptr(), v.data_ptr()
-        if strides is None or (kp | vp) % 16:
-            k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
-            kp, vp, strides = k.data_ptr(), v.data_ptr(), k.stride()[:3] + v.stride()[:3]
-        with on_device(self.device):
-            check(lib().skv_quant_write(self._st[layer], kp, vp, code, b, T, *strides, at, per_seq, host,
-                                        stream_ptr(self.device)), "skv_quant_write")
+        if not straight or (kp | vp) % 16:
+            return self.write(layer, k.clone(memory_format=torch.contiguous_format),
+                              v.clone(memory_format=torch.contiguous_format), pos)
+        self._where(rows, pos, rows.batch, rows.tokens)
+        if rows.batch == 0 or rows.tokens == 0:
+            return
+        if elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self.write(layer, k, v, pos)
+        rows.k, rows.v = kp, vp
+        check(lib().skv_quant_write(self._st[layer], rows, stream_ptr(dev)), "skv_quant_write")
+
+    def _plan_read(self, b: int, count: int, dtype: torch.dtype):
+        if not 0 <= b <= self.batch:
+            raise ValueError(f"the cache holds {self.batch} sequences")
+        if not 0 <= count <= self.max_seq_len:
+            raise ValueError(f"{count} rows lie outside the cache's {self.max_seq_len} positions")
+        hs = count * self.d
+        return (2, b, self.h_kv, count, self.d), SkvRows(0, 0, None, 0, self.h_kv * hs, hs, self.d, self.h_kv * hs, hs, self.d,
+                                                         0, dtype_code(dtype), b, count)
 
     def read(self, layer: int, pos, count: int, *, dtype: torch.dtype = torch.bfloat16,
              batch: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The rows ``[pos, pos + count)`` of the first ``batch`` (all) sequences as ``k, v [b, H_kv, count, 128]`` of
         ``dtype``; ``pos`` as in ``write`` (rows outside the cache come back as zeros and are recorded)."""
-        b = self.batch if batch is None else batch
-        if not 0 <= b <= self.batch:
-            raise ValueError(f"the cache holds {self.batch} sequences")
-        if not 0 <= count <= self.max_seq_len:
-            raise ValueError(f"{count} rows lie outside the cache's {self.max_seq_len} positions")
-        at, per_seq, host = self._where(pos, b, count)
-        code = dtype_code(dtype)
-        k, v = torch.empty(2, b, self.h_kv, count, self.d, dtype=dtype, device=self.device).unbind(0)
-        if b and count:
-            hs = count * self.d
-            bs = self.h_kv * hs
-            with on_device(self.device):
-                check(lib().skv_quant_read(self._st[layer], k.data_ptr(), v.data_ptr(), code, b, count, bs, hs, self.d, bs,
-                                           hs, self.d, at, per_seq, host, stream_ptr(self.device)), "skv_quant_read")
+        b, dev = self.batch if batch is None else batch, self.device
+        shape, rows = self._plan((b, count, dtype), lambda: self._plan_read(b, count, dtype))
+        self._where(rows, pos, b, count)
+        k, v = torch.empty(shape, dtype=dtype, device=dev).unbind(0)
+        if b == 0 or count == 0:
+            return k, v
+        if elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self.read(layer, pos, count, dtype=dtype, batch=batch)
+        rows.k, rows.v = k.data_ptr(), v.data_ptr()
+        check(lib().skv_quant_read(self._st[layer], rows, stream_ptr(dev)), "skv_quant_read")
         return k, v
 
     def rows(self, layer: int, b: int, n: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
@@ -170,7 +184,7 @@ class QuantAttentionGraph:
         self.n_group = 0                                   # heads per entry of the device-side lengths (0: one length)
         self.dtype = dtype
         self._code = dtype_code(dtype)
-        with on_device(torch.device(device)):
+        with torch.cuda.device(device) if torch.device(device).type == "cuda" else nullcontext():
             self.ctas = L.skv_quant_ctas()
             size = L.skv_quant_workspace_bytes(H_kv, self.G, d, self.ctas)
             if size < 0:
@@ -193,8 +207,10 @@ class QuantAttentionGraph:
             raise ValueError("lengths must be int32 on the queries' device: one, or one per n_group heads")
         if not q.is_contiguous() or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
-        with on_device(dev):
-            check(lib().skv_attend_quant(cache._st[layer], q.data_ptr(), self._code, self.G, n_dev.data_ptr(),
-                                         self.n_group, self.out.data_ptr(), self.ws.data_ptr(), self.ctas, self._scale,
-                                         stream_ptr(dev)), "skv_attend_quant")
+        if elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self(q, cache, layer, n_dev)
+        check(lib().skv_attend_quant(cache._st[layer], q.data_ptr(), self._code, self.G, n_dev.data_ptr(), self.n_group,
+                                     self.out.data_ptr(), self.ws.data_ptr(), self.ctas, self._scale, stream_ptr(dev)),
+              "skv_attend_quant")
         return self.out

@@ -34,13 +34,14 @@ def qcache(**o):
     return ctypes.byref(c)
 
 
-def test_the_struct_matches_the_header():
+@pytest.mark.parametrize("name,mirror,size", [("skv_qcache", _lib.SkvQCache, 4 * 8 + 6 * 4), ("skv_rows", _lib.SkvRows, 10 * 8 + 4 * 4)])
+def test_the_structs_match_the_header(name, mirror, size):
     text = open(os.path.join(ROOT, "include", "skv.h")).read()
-    body = text[text.index("typedef struct skv_qcache {"):text.index("} skv_qcache;")]
+    body = text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")]
     body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
     names = re.findall(r"[\s*]([a-z_0-9]+)(?=[,;])", body)
-    assert names == [f[0] for f in _lib.SkvQCache._fields_]
-    assert ctypes.sizeof(_lib.SkvQCache) == 4 * 8 + 6 * 4
+    assert names == [f[0] for f in mirror._fields_]
+    assert ctypes.sizeof(mirror) == size
 
 
 BAD_CACHES = [(dict(k=None), -1), (dict(v=None), -1), (dict(scale=None), -1), (dict(d=64), -2), (dict(bits=6), -5),
@@ -55,12 +56,14 @@ def test_rows_are_refused_on_the_host(L, name):
 
     def call(c=None, **o):
         a = {**base, **o}
-        return getattr(L, name)(qcache() if c is None else c, a["k"], a["v"], a["dtype"], a["batch"], a["tokens"], a["kb"],
-                                a["kh"], a["kr"], a["vb"], a["vh"], a["vr"], a["pos"], a["per"], a["pos0"], None)
+        rows = _lib.SkvRows(a["k"], a["v"], a["pos"], a["pos0"], a["kb"], a["kh"], a["kr"], a["vb"], a["vh"], a["vr"], a["per"],
+                            a["dtype"], a["batch"], a["tokens"])
+        return getattr(L, name)(qcache() if c is None else c, ctypes.byref(rows), None)
 
     for over, code in BAD_CACHES:
         assert call(qcache(**over)) == code, over
-    assert getattr(L, name)(None, OK, OK, 0, 1, 1, 0, 0, 0, 0, 0, 0, None, 0, 0, None) == -1
+    assert getattr(L, name)(None, ctypes.byref(_lib.SkvRows()), None) == -1
+    assert getattr(L, name)(qcache(), None, None) == -1
     assert call(k=None) == -1 and call(v=None) == -1 and call(dtype=3) == -3
     assert call(batch=3) == -5 and call(batch=0) == -5 and call(tokens=-1) == -5 and call(tokens=65) == -5
     assert call(pos0=62) == -5 and call(pos0=-1) == -5

@@ -481,24 +481,32 @@ int64_t skv_quant_workspace_bytes(int heads, int G, int d, int ctas);
 int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, int G, const int32_t *n_dev, int n_group, void *out,
                      void *workspace, int ctas, float scale, void *stream);
 
-/* Attention of a batch whose sequences share a prefix: query row of (sequence b, KV head h) attends over the prefix's
- * rows [0, prefix) of head h, which exist once, and over its own rows [0, n) of cache head b * h_kv + h.  The reference
- * keeps and reads the prompt's rows once per sequence (ssa/models/graph_decode.py:29-157).
- *   q, out             [batch * h_kv * G, 128] dtype, G <= 8
- *   k_prefix, v_prefix [h_kv, prefix, 128]; may be null when prefix == 0
- *   k, v               [batch * h_kv, rows_limit, 128]; element strides, unit last stride, rows 16-byte aligned
- *   n_dev, n_group     own lengths as everywhere; one beyond rows_limit counts as rows_limit and is recorded in `status`
- *                      ([batch * h_kv], may be null)
- *   splits             skv_prefix_splits(batch, h_kv, G, dtype); workspace of skv_prefix_workspace_bytes bytes,
- *                      zero-initialised once
+/* The caches of a batch whose sequences share a prefix: its rows [0, prefix) of every KV head exist once, sequence b's own
+ * rows are those of the heads b * h_kv + h. */
+typedef struct skv_prefix {
+    const void *k_prefix, *v_prefix;  /* [h_kv, prefix, 128]; may be null when prefix == 0 */
+    const void *k, *v;                /* [batch * h_kv, rows_limit, 128] */
+    int64_t kp_head_stride, kp_row_stride, vp_head_stride, vp_row_stride;   /* elements; unit last stride, rows 16-byte aligned */
+    int64_t k_head_stride, k_row_stride, v_head_stride, v_row_stride;
+    int32_t prefix, rows_limit;
+    int32_t batch, h_kv;
+    int32_t G;                        /* query heads per KV head, <= 8 */
+    int32_t d;                        /* 128 */
+    int32_t dtype;                    /* of the caches, the queries and the output */
+    int32_t n_group;                  /* as everywhere, over the batch * h_kv heads */
+} skv_prefix;
+
+/* Softmax attention of one query per query head over the shared prefix and over its sequence's own rows [0, n).  The
+ * reference keeps and reads the prompt's rows once per sequence (ssa/models/graph_decode.py:29-157); here the batch's query
+ * rows read them together.
+ *   q, out     [batch * h_kv * G, 128]
+ *   n_dev      own lengths; one beyond rows_limit counts as rows_limit and is recorded in `status` ([batch * h_kv], may be null)
+ *   splits     skv_prefix_splits(batch, h_kv, G, dtype); workspace of skv_prefix_workspace_bytes bytes, zero-initialised once
  * A row without any key gets zeros. */
 int skv_prefix_splits(int batch, int h_kv, int G, int dtype);
 int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d, int splits);
-int skv_attend_prefix(const void *q, const void *k_prefix, const void *v_prefix, int prefix, const void *k, const void *v,
-                      const int32_t *n_dev, int n_group, void *out, void *workspace, int32_t *status, int batch, int h_kv,
-                      int G, int d, int dtype, int64_t kp_head_stride, int64_t kp_row_stride, int64_t vp_head_stride,
-                      int64_t vp_row_stride, int64_t k_head_stride, int64_t k_row_stride, int64_t v_head_stride,
-                      int64_t v_row_stride, int rows_limit, int splits, float scale, void *stream);
+int skv_attend_prefix(const skv_prefix *c, const void *q, const int32_t *n_dev, void *out, void *workspace, int splits,
+                      int32_t *status, float scale, void *stream);
 
 #ifdef __cplusplus
 }

@@ -60,6 +60,16 @@ class SkvRows(C.Structure):
                 ("pos_per_seq", C.c_int32), ("dtype", C.c_int32), ("batch", C.c_int32), ("tokens", C.c_int32)]
 
 
+class SkvPrefix(C.Structure):
+    """``skv_prefix`` of include/skv.h: the caches of a batch whose sequences share a prefix."""
+    _fields_ = [("k_prefix", C.c_void_p), ("v_prefix", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("kp_head_stride", C.c_int64), ("kp_row_stride", C.c_int64), ("vp_head_stride", C.c_int64),
+                ("vp_row_stride", C.c_int64), ("k_head_stride", C.c_int64), ("k_row_stride", C.c_int64),
+                ("v_head_stride", C.c_int64), ("v_row_stride", C.c_int64), ("prefix", C.c_int32), ("rows_limit", C.c_int32),
+                ("batch", C.c_int32), ("h_kv", C.c_int32), ("G", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32),
+                ("n_group", C.c_int32)]
+
+
 class SkvState(C.Structure):
     """Mirror of ``struct skv_state``."""
     _fields_ = [("heads", C.c_int32), ("C", C.c_int32), ("d", C.c_int32), ("capacity", C.c_int32),
@@ -183,8 +193,7 @@ def _declare(lib) -> None:
     lib.skv_prefix_workspace_bytes.restype = i64
     lib.skv_prefix_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
     lib.skv_attend_prefix.restype = i32
-    lib.skv_attend_prefix.argtypes = [vp, vp, vp, i32, vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64,
-                                      i64, i64, i64, i64, i64, i32, i32, f32, vp]
+    lib.skv_attend_prefix.argtypes = [C.POINTER(SkvPrefix), vp, vp, vp, vp, i32, vp, f32, vp]
     lib.skv_rebin.restype = i32
     lib.skv_rebin.argtypes = [C.POINTER(SkvState), vp, i32, i32, vp, i32, i64, i64, f32, i32, f32, vp, i64, vp]
 

@@ -663,40 +663,36 @@ extern "C" int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d,
     return skv_attend_workspace_bytes(batch * h_kv, G, d, splits);
 }
 
-extern "C" int skv_attend_prefix(const void *q, const void *k_prefix, const void *v_prefix, int prefix, const void *k,
-                                 const void *v, const int32_t *n_dev, int n_group, void *out, void *workspace,
-                                 int32_t *status, int batch, int h_kv, int G, int d, int dtype,
-                                 int64_t kp_head_stride, int64_t kp_row_stride, int64_t vp_head_stride,
-                                 int64_t vp_row_stride, int64_t k_head_stride, int64_t k_row_stride,
-                                 int64_t v_head_stride, int64_t v_row_stride, int rows_limit, int splits, float scale,
-                                 void *stream) {
-    if (!q || !k || !v || !n_dev || !out || !workspace) return SKV_E_NULL;
-    if (prefix > 0 && (!k_prefix || !v_prefix)) return SKV_E_NULL;
-    if (d != HEAD_DIM) return SKV_E_DIM;
-    if (dtype != SKV_BF16 && dtype != SKV_F32) return SKV_E_DTYPE;
-    if (G < 1 || G > 8) return SKV_E_DIM;
-    if (batch <= 0 || h_kv <= 0 || (int64_t)batch * h_kv > 65535 || prefix < 0 || rows_limit < 0 ||
-        (int64_t)prefix + rows_limit > 0x7fffffff - 64 || splits <= 0 || splits > 65535 || n_group < 0)
+extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32_t *n_dev, void *out, void *workspace, int splits,
+                                 int32_t *status, float scale, void *stream) {
+    if (!c || !q || !c->k || !c->v || !n_dev || !out || !workspace) return SKV_E_NULL;
+    if (c->prefix > 0 && (!c->k_prefix || !c->v_prefix)) return SKV_E_NULL;
+    if (c->d != HEAD_DIM) return SKV_E_DIM;
+    if (c->dtype != SKV_BF16 && c->dtype != SKV_F32) return SKV_E_DTYPE;
+    if (c->G < 1 || c->G > 8) return SKV_E_DIM;
+    if (c->batch <= 0 || c->h_kv <= 0 || (int64_t)c->batch * c->h_kv > 65535 || c->prefix < 0 || c->rows_limit < 0 ||
+        (int64_t)c->prefix + c->rows_limit > 0x7fffffff - 64 || splits <= 0 || splits > 65535 || c->n_group < 0)
         return SKV_E_RANGE;
-    const int per16 = dtype == SKV_BF16 ? 8 : 4;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace) ||
-        !aligned16(k_prefix) || !aligned16(v_prefix))
+    if (!aligned16(q) || !aligned16(c->k) || !aligned16(c->v) || !aligned16(out) || !aligned16(workspace) ||
+        !aligned16(c->k_prefix) || !aligned16(c->v_prefix))
         return SKV_E_ALIGN;
-    if (kp_head_stride % per16 || kp_row_stride % per16 || vp_head_stride % per16 || vp_row_stride % per16 ||
-        k_head_stride % per16 || k_row_stride % per16 || v_head_stride % per16 || v_row_stride % per16 ||
-        (prefix > 1 && (kp_row_stride < d || vp_row_stride < d)) || (rows_limit > 1 && (k_row_stride < d || v_row_stride < d)))
-        return SKV_E_ALIGN;
-    PrefixParams p;
-    p.q = q; p.kp = k_prefix; p.vp = v_prefix; p.k = k; p.v = v; p.n_dev = n_dev; p.out = out; p.status = status;
-    p.batch = batch; p.h_kv = h_kv; p.G = G; p.n_group = n_group; p.prefix = prefix; p.rows_limit = rows_limit;
+    const int per16 = c->dtype == SKV_BF16 ? 8 : 4;
+    const int64_t strides[8] = {c->kp_head_stride, c->kp_row_stride, c->vp_head_stride, c->vp_row_stride,
+                                c->k_head_stride, c->k_row_stride, c->v_head_stride, c->v_row_stride};
+    for (int i = 0; i < 8; ++i) {
+        const int rows = i < 4 ? c->prefix : c->rows_limit;
+        if (strides[i] % per16 || ((i & 1) && rows > 1 && strides[i] < HEAD_DIM)) return SKV_E_ALIGN;
+    }
+    PrefixParams p = {};
+    p.q = q; p.kp = c->k_prefix; p.vp = c->v_prefix; p.k = c->k; p.v = c->v; p.n_dev = n_dev; p.out = out; p.status = status;
+    p.batch = c->batch; p.h_kv = c->h_kv; p.G = c->G; p.n_group = c->n_group; p.prefix = c->prefix; p.rows_limit = c->rows_limit;
     p.splits = splits;
     p.part = static_cast<float *>(workspace);
-    p.ticket = reinterpret_cast<int32_t *>(p.part + (int64_t)batch * h_kv * splits * G * PART_LD);
-    p.kph = kp_head_stride; p.kpr = kp_row_stride; p.vph = vp_head_stride; p.vpr = vp_row_stride;
-    p.ksh = k_head_stride; p.ksr = k_row_stride; p.vsh = v_head_stride; p.vsr = v_row_stride;
+    p.ticket = reinterpret_cast<int32_t *>(p.part + (int64_t)c->batch * c->h_kv * splits * c->G * PART_LD);
+    p.kph = c->kp_head_stride; p.kpr = c->kp_row_stride; p.vph = c->vp_head_stride; p.vpr = c->vp_row_stride;
+    p.ksh = c->k_head_stride; p.ksr = c->k_row_stride; p.vsh = c->v_head_stride; p.vsr = c->v_row_stride;
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    p.prefix_splits = p.own_splits = p.listed = 0;
-    if (dtype == SKV_F32) return launch_prefix_simple<float>(p, st);
+    if (c->dtype == SKV_F32) return launch_prefix_simple<float>(p, st);
     return splits > 1 ? launch_prefix_mma(p, st) : launch_prefix_simple<__nv_bfloat16>(p, st);
 }

@@ -8,7 +8,7 @@ from contextlib import nullcontext
 
 import torch
 
-from ._lib import SkvError, check, dtype_code, elsewhere, lib, stream_ptr
+from ._lib import SkvError, SkvPrefix, check, dtype_code, elsewhere, lib, stream_ptr
 from .qwen3 import KVCache
 
 __all__ = ["PrefixKVCache", "PrefixAttentionGraph"]
@@ -93,9 +93,10 @@ class PrefixAttentionGraph:
             self.status = torch.zeros(B * H_kv, dtype=torch.int32, device=device)
         self.device = self.out.device                      # (with its index)
         self._shape, self._scale = self.out.shape, 1.0 / math.sqrt(d)
-        self._checked = None
+        self._layout = self._call = None                   # of the last call, and what it passed on
 
-    def _check_layout(self, Kp, Vp, K, V) -> None:
+    def _plan(self, Kp, Vp, K, V) -> SkvPrefix:
+        """What calls with caches of this layout pass on, checked once."""
         heads = self.B * self.H_kv
         if Kp.dim() != 3 or Kp.shape != Vp.shape or Kp.shape[0] != self.H_kv or Kp.shape[2] != self.d:
             raise ValueError(f"the prefix must be [{self.H_kv}, rows, {self.d}]")
@@ -103,15 +104,16 @@ class PrefixAttentionGraph:
             raise ValueError(f"the sequences' rows must be [{heads}, rows, {self.d}]")
         if any(t.shape[1] and t.stride(2) != 1 for t in (Kp, Vp, K, V)):
             raise ValueError("the caches must have a unit last stride")
+        strides = [s for t in (Kp, Vp, K, V) for s in t.stride()[:2]]
+        return SkvPrefix(0, 0, 0, 0, *strides, Kp.shape[1], K.shape[1], self.B, self.H_kv, self.G, self.d, self._code, 0)
 
     def __call__(self, q: torch.Tensor, Kp: torch.Tensor, Vp: torch.Tensor, K: torch.Tensor, V: torch.Tensor,
                  n_dev: torch.Tensor) -> torch.Tensor:
         """``q [B*H, d]``; ``Kp, Vp [H_kv, P, d]`` the shared rows; ``K, V [B*H_kv, L, d]`` the sequences' own rows;
         ``n_dev`` int32 on the device, own lengths: one, or one per ``n_group`` KV heads.  A row without keys gets zeros."""
         layout = (Kp.shape, Kp.stride(), Vp.shape, Vp.stride(), K.shape, K.stride(), V.shape, V.stride())
-        if layout != self._checked:                        # (a decode step has the same layout again and again)
-            self._check_layout(Kp, Vp, K, V)
-            self._checked = layout
+        if layout != self._layout:                         # (a decode step has the same layout again and again)
+            self._call, self._layout = self._plan(Kp, Vp, K, V), layout
         dev, dtype = self.device, self.dtype
         if q.shape != self._shape or q.dtype is not dtype:
             raise ValueError(f"queries must be {tuple(self._shape)} {dtype}")
@@ -123,13 +125,13 @@ class PrefixAttentionGraph:
             raise ValueError("lengths must be int32 on the queries' device: one, or one per n_group KV heads")
         if not q.is_contiguous() or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
-        ks, vs, pks, pvs = layout[5], layout[7], layout[1], layout[3]
         if elsewhere(dev):
             with torch.cuda.device(dev):
                 return self(q, Kp, Vp, K, V, n_dev)
-        check(lib().skv_attend_prefix(q.data_ptr(), Kp.data_ptr(), Vp.data_ptr(), layout[0][1], K.data_ptr(), V.data_ptr(),
-                                      n_dev.data_ptr(), self.n_group, self.out.data_ptr(), self.ws.data_ptr(),
-                                      self.status.data_ptr(), self.B, self.H_kv, self.G, self.d, self._code, pks[0], pks[1],
-                                      pvs[0], pvs[1], ks[0], ks[1], vs[0], vs[1], layout[4][1], self.num_splits, self._scale,
-                                      stream_ptr(dev)), "skv_attend_prefix")
+        c = self._call
+        c.k_prefix, c.v_prefix, c.k, c.v = Kp.data_ptr(), Vp.data_ptr(), K.data_ptr(), V.data_ptr()
+        c.n_group = self.n_group
+        check(lib().skv_attend_prefix(c, q.data_ptr(), n_dev.data_ptr(), self.out.data_ptr(), self.ws.data_ptr(),
+                                      self.num_splits, self.status.data_ptr(), self._scale, stream_ptr(dev)),
+              "skv_attend_prefix")
         return self.out

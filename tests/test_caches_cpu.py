@@ -34,12 +34,13 @@ def qcache(**o):
     return ctypes.byref(c)
 
 
-@pytest.mark.parametrize("name,mirror,size", [("skv_qcache", _lib.SkvQCache, 4 * 8 + 6 * 4), ("skv_rows", _lib.SkvRows, 10 * 8 + 4 * 4)])
+@pytest.mark.parametrize("name,mirror,size", [("skv_qcache", _lib.SkvQCache, 4 * 8 + 6 * 4), ("skv_rows", _lib.SkvRows, 10 * 8 + 4 * 4),
+                                              ("skv_prefix", _lib.SkvPrefix, 12 * 8 + 8 * 4)])
 def test_the_structs_match_the_header(name, mirror, size):
     text = open(os.path.join(ROOT, "include", "skv.h")).read()
     body = text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")]
     body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
-    names = re.findall(r"[\s*]([a-z_0-9]+)(?=[,;])", body)
+    names = re.findall(r"[\s*]([A-Za-z_0-9]+)(?=[,;])", body)
     assert names == [f[0] for f in mirror._fields_]
     assert ctypes.sizeof(mirror) == size
 
@@ -110,10 +111,11 @@ def test_attention_over_a_shared_prefix_is_refused_on_the_host(L):
 
     def call(**o):
         a = {**args, **o}
-        return L.skv_attend_prefix(a["q"], a["kp"], a["vp"], a["P"], a["k"], a["v"], a["n"], a["ng"], a["out"], a["ws"], None,
-                                   a["batch"], a["h"], a["G"], a["d"], a["dtype"], a["kph"], a["kpr"], a["vph"], a["vpr"],
-                                   a["kh"], a["kr"], a["vh"], a["vr"], a["lim"], a["splits"], 0.1, None)
+        c = _lib.SkvPrefix(a["kp"], a["vp"], a["k"], a["v"], a["kph"], a["kpr"], a["vph"], a["vpr"], a["kh"], a["kr"], a["vh"],
+                           a["vr"], a["P"], a["lim"], a["batch"], a["h"], a["G"], a["d"], a["dtype"], a["ng"])
+        return L.skv_attend_prefix(ctypes.byref(c), a["q"], a["n"], a["out"], a["ws"], a["splits"], None, 0.1, None)
 
+    assert L.skv_attend_prefix(None, OK, OK, OK, OK, 4, None, 0.1, None) == -1
     for name in ("q", "kp", "vp", "k", "v", "n", "out", "ws"):
         assert call(**{name: None}) == -1, name
     assert call(d=64) == -2 and call(G=0) == -2 and call(G=9) == -2 and call(dtype=5) == -3

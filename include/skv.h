@@ -485,7 +485,7 @@ int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, int G, const
  * rows are those of the heads b * h_kv + h. */
 typedef struct skv_prefix {
     const void *k_prefix, *v_prefix;  /* [h_kv, prefix, 128]; may be null when prefix == 0 */
-    const void *k, *v;                /* [batch * h_kv, rows_limit, 128] */
+    const void *k, *v;                /* [batch * h_kv, rows_limit, 128]; may be null when rows_limit == 0 */
     int64_t kp_head_stride, kp_row_stride, vp_head_stride, vp_row_stride;   /* elements; unit last stride, rows 16-byte aligned */
     int64_t k_head_stride, k_row_stride, v_head_stride, v_row_stride;
     int32_t prefix, rows_limit;

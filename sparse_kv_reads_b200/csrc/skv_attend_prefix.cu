@@ -414,7 +414,8 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
     }
     __syncwarp();
     __syncthreads();
-    if (s_fail && p.status && tid < p.batch) atomicOr(p.status + tid * p.h_kv + h, SKV_ST_WAIT_TIMEOUT);
+    if (s_fail && p.status)
+        for (int b = tid; b < p.batch; b += P_THREADS) atomicOr(p.status + b * p.h_kv + h, SKV_ST_WAIT_TIMEOUT);
     if (warp == 9) {
         tcgen05_after_sync();
         tmem_free(tmem, 512);
@@ -665,8 +666,8 @@ extern "C" int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d,
 
 extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32_t *n_dev, void *out, void *workspace, int splits,
                                  int32_t *status, float scale, void *stream) {
-    if (!c || !q || !c->k || !c->v || !n_dev || !out || !workspace) return SKV_E_NULL;
-    if (c->prefix > 0 && (!c->k_prefix || !c->v_prefix)) return SKV_E_NULL;
+    if (!c || !q || !n_dev || !out || !workspace) return SKV_E_NULL;
+    if ((c->prefix > 0 && (!c->k_prefix || !c->v_prefix)) || (c->rows_limit > 0 && (!c->k || !c->v))) return SKV_E_NULL;
     if (c->d != HEAD_DIM) return SKV_E_DIM;
     if (c->dtype != SKV_BF16 && c->dtype != SKV_F32) return SKV_E_DTYPE;
     if (c->G < 1 || c->G > 8) return SKV_E_DIM;

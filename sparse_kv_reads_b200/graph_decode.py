@@ -566,16 +566,19 @@ class GraphDecoder:
         return self._peer
 
     def _check_place(self, pos) -> None:
-        """A quantised or shared-prefix cache: the new tokens' positions, where the host knows them, lie behind the
-        prefix that ``prepare`` saw and within the cache."""
-        if not isinstance(self.cache, (QuantKVCache, PrefixKVCache)) or (torch.is_tensor(pos) and pos.is_cuda):
+        """A quantised or shared-prefix cache: the new tokens' positions lie behind the prefix that ``prepare`` saw, within
+        the cache and within the rotary tables."""
+        if not isinstance(self.cache, (QuantKVCache, PrefixKVCache)):
             return
+        if torch.is_tensor(pos) and pos.is_cuda:
+            raise ValueError("positions in a quantised or shared-prefix cache are given on the host, where they are checked")
         if self.first != self.cache.first:
             raise ValueError("the shared prefix has changed since prepare()")
         at = [int(pos)] if isinstance(pos, int) or (torch.is_tensor(pos) and pos.dim() == 0) else [int(x) for x in pos]
-        if min(at) < self.first or max(at) >= self.cache.max_seq_len:
+        end = min(self.cache.max_seq_len, self.model.rope_cos.shape[0])
+        if min(at) < self.first or max(at) >= end:
             raise ValueError(f"position {min(at) if min(at) < self.first else max(at)} lies outside the cache's "
-                             f"[{self.first}, {self.cache.max_seq_len})")
+                             f"[{self.first}, {end})")
 
     def capture(self) -> None:
         """Record one decode step.  Call after ``prepare`` and before the first ``step``; the warm-up

@@ -123,7 +123,9 @@ class PrefixAttentionGraph:
         if n_dev.dtype is not torch.int32 or n_dev.device != dev or not n_dev.is_contiguous() \
                 or n_dev.numel() < (-(-self.B * self.H_kv // self.n_group) if self.n_group else 1):
             raise ValueError("lengths must be int32 on the queries' device: one, or one per n_group KV heads")
-        if not q.is_contiguous() or q.data_ptr() % 16:
+        if dev.type != "cuda":
+            raise ValueError("a shared prefix is attended over on a CUDA device only")
+        if not q.is_contiguous() or q.data_ptr() % 16 or q.data_ptr() == self.out.data_ptr():
             q = q.clone(memory_format=torch.contiguous_format)
         if elsewhere(dev):
             with torch.cuda.device(dev):

@@ -53,6 +53,9 @@ class QuantKVCache:
                 if tuple(t.shape) != want[name][0] or t.dtype != want[name][1] or not t.is_contiguous() \
                         or t.device != k[0].device:
                     raise ValueError(f"{name} must be contiguous {want[name][0]} {want[name][1]} on one device")
+        if status is not None and (status.shape != (B * H,) or status.dtype != torch.int32 or not status.is_contiguous()
+                                   or status.device != k[0].device):
+            raise ValueError(f"status must be contiguous ({B * H},) int32 on the cache's device")
         self = cls.__new__(cls)
         self._set(list(k), list(v), list(scale), bits, status)
         return self
@@ -66,6 +69,10 @@ class QuantKVCache:
         self.status = torch.zeros(self.batch * self.h_kv, dtype=torch.int32, device=self.device) if status is None else status
         self._st = [SkvQCache(a.data_ptr(), b.data_ptr(), s.data_ptr(), self.status.data_ptr(), self.batch, self.h_kv,
                               self.max_seq_len, self.d, bits, 0) for a, b, s in zip(k, v, scale)]
+
+    def _on_gpu(self) -> None:
+        if self.device.type != "cuda":
+            raise ValueError("a quantised cache is written, read and attended over on a CUDA device only")
 
     def sequence(self, b: int) -> "QuantKVCache":
         """Sequence ``b`` alone, on the same memory."""
@@ -134,6 +141,7 @@ class QuantKVCache:
         self._where(rows, pos, rows.batch, rows.tokens)
         if rows.batch == 0 or rows.tokens == 0:
             return
+        self._on_gpu()
         if elsewhere(dev):
             with torch.cuda.device(dev):
                 return self.write(layer, k, v, pos)
@@ -159,6 +167,7 @@ class QuantKVCache:
         k, v = torch.empty(shape, dtype=dtype, device=dev).unbind(0)
         if b == 0 or count == 0:
             return k, v
+        self._on_gpu()
         if elsewhere(dev):
             with torch.cuda.device(dev):
                 return self.read(layer, pos, count, dtype=dtype, batch=batch)
@@ -205,7 +214,8 @@ class QuantAttentionGraph:
         if n_dev.dtype is not torch.int32 or n_dev.device != dev or not n_dev.is_contiguous() \
                 or n_dev.numel() < (-(-self.H_kv // self.n_group) if self.n_group else 1):
             raise ValueError("lengths must be int32 on the queries' device: one, or one per n_group heads")
-        if not q.is_contiguous() or q.data_ptr() % 16:
+        cache._on_gpu()
+        if not q.is_contiguous() or q.data_ptr() % 16 or q.data_ptr() == self.out.data_ptr():
             q = q.clone(memory_format=torch.contiguous_format)
         if elsewhere(dev):
             with torch.cuda.device(dev):

@@ -118,6 +118,7 @@ def test_attention_over_a_shared_prefix_is_refused_on_the_host(L):
     assert L.skv_attend_prefix(None, OK, OK, OK, OK, 4, None, 0.1, None) == -1
     for name in ("q", "kp", "vp", "k", "v", "n", "out", "ws"):
         assert call(**{name: None}) == -1, name
+    assert call(kp=None, vp=None, P=0, d=64) == -2 and call(k=None, v=None, lim=0, d=64) == -2       # no rows: no address
     assert call(d=64) == -2 and call(G=0) == -2 and call(G=9) == -2 and call(dtype=5) == -3
     assert call(batch=0) == -5 and call(h=0) == -5 and call(batch=20000) == -5 and call(P=-1) == -5 and call(lim=-1) == -5
     assert call(P=2 ** 31 - 2) == -5 and call(splits=0) == -5 and call(ng=-1) == -5
@@ -162,6 +163,12 @@ def test_quantised_cache_checks_its_arguments():
         QuantKVCache.from_tensors(c.k, c.v, c.scale, 8)
     with pytest.raises(ValueError, match="scales must be"):
         QuantKVCache.from_tensors(c.k, c.v, [s.float() for s in c.scale], 4)
+    with pytest.raises(ValueError, match="status must be"):
+        QuantKVCache.from_tensors(c.k, c.v, c.scale, 4, c.status[:3])
+    with pytest.raises(ValueError, match="CUDA device only"):
+        c.write(0, x, x, 0)
+    with pytest.raises(ValueError, match="CUDA device only"):
+        c.read(0, 0, 1)
     one = c.sequence(2)
     assert one.batch == 1 and one.k[1].data_ptr() == c.k[1][2].data_ptr() and one.status.data_ptr() == c.status[4:].data_ptr()
 
@@ -188,13 +195,15 @@ def test_attention_objects_check_their_arguments(L):
         a(q, QuantKVCache(1, 1, 4, 16, 128, 8, CPU), 0, n)
     with pytest.raises(ValueError, match="lengths must be"):
         a(q, c, 0, n.long())
+    with pytest.raises(ValueError, match="CUDA device only"):
+        a(q, c, 0, n)
     a.n_group = 1
     with pytest.raises(ValueError, match="lengths must be"):
         a(q, c, 0, n)
     p = PrefixAttentionGraph(B=2, H=4, H_kv=2, d=128, dtype=torch.bfloat16, device=CPU)
     q8, kp, k = torch.zeros(8, 128, dtype=torch.bfloat16), torch.zeros(2, 9, 128, dtype=torch.bfloat16), \
         torch.zeros(4, 5, 128, dtype=torch.bfloat16)
-    for args, word in (((q, kp, kp, k, k, n), "queries must be"), ((q8, kp[:1], kp[:1], k, k, n), "prefix must be"),
+    for args, word in (((q8, kp, kp, k, k, n), "CUDA device only"), ((q, kp, kp, k, k, n), "queries must be"), ((q8, kp[:1], kp[:1], k, k, n), "prefix must be"),
                        ((q8, kp, kp[:, :3], k, k, n), "prefix must be"), ((q8, kp, kp, k[:3], k[:3], n), "rows must be"),
                        ((q8, kp.float(), kp.float(), k, k, n), "type and device"),
                        ((q8, kp, kp, k, k, n.long()), "lengths must be"),
@@ -260,3 +269,6 @@ def test_the_clustered_mode_refuses_the_new_caches_and_steps_are_checked():
     cache.prefix.cur_len = 7
     with pytest.raises(ValueError, match="prefix has changed"):
         dec.step(torch.zeros(2, 1, dtype=torch.long), 8)
+    long = GraphDecoder(m, m.alloc_cache(600, bits=8), mode="dense")             # the rotary tables have 256 rows
+    with pytest.raises(ValueError, match="outside the cache"):
+        long.step(torch.zeros(1, 1, dtype=torch.long), 256)

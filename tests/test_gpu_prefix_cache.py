@@ -120,6 +120,65 @@ def test_scores_far_apart_and_rescaled_sums():
         check_against_definition(out, q, kp2, vp, k2, v, lens, G, torch.bfloat16)
 
 
+@pytest.mark.parametrize("B,Hk,G,P,n", [(2, 2, 2, 300, 9), (40, 2, 4, 2000, 9), (9, 1, 8, 9000, 70)])
+def test_queries_that_alias_the_output_a_negative_scale_and_no_own_rows(B, Hk, G, P, n):
+    """By the list and by the tiles: queries in the output buffer, the softmax scale's sign, a cache without own rows."""
+    lens = [n] * B
+    q, kp, vp, k, v = (t.to(DEV) for t in inputs(B, Hk, G, P, n, lens, B))
+    attn = PrefixAttentionGraph(B=B, H=Hk * G, H_kv=Hk, d=128, dtype=torch.bfloat16, device=DEV)
+    n_dev = torch.tensor([n], dtype=torch.int32, device=DEV)
+    want = attn(q, kp, vp, k, v, n_dev).clone()
+    check_against_definition(want, *(t.cpu() for t in (q, kp, vp, k, v)), lens, G, torch.bfloat16)
+    attn.out.copy_(q)
+    assert torch.equal(attn(attn.out, kp, vp, k, v, n_dev), want)
+    attn._scale = -attn._scale
+    assert torch.equal(attn(-q, kp, vp, k, v, n_dev), want)
+    attn._scale = -attn._scale
+    got = attn(q, kp, vp, k[:, :0], v[:, :0], torch.zeros_like(n_dev))
+    check_against_definition(got, *(t.cpu() for t in (q, kp, vp, k, v)), [0] * B, G, torch.bfloat16)
+
+
+@pytest.mark.parametrize("B,Hk,G", [(1, 1, 1), (30, 2, 4), (100, 1, 3), (70, 4, 8)])
+def test_long_prefixes_through_the_tiles(B, Hk, G):
+    """Enough rows that the prefix goes through the tensor-core tiles: ragged last tiles, one and more groups of 256 rows."""
+    P = 128 * 40 + 77 if B > 1 else 70000
+    lens = [(11 * b) % 40 for b in range(B)]
+    x = inputs(B, Hk, G, P, 40, lens, B)
+    out, attn = run(*x, lens, B, Hk, G)
+    check_against_definition(out, *x, lens, G, torch.bfloat16)
+    assert int(attn.status.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("B,P", [(2100, 64), (2100, 65), (1100, 127), (1100, 128), (1100, 129), (700, 257)])
+def test_short_prefixes_through_the_tiles(B, P):
+    """Batches so large that even a short prefix goes through the tiles: one tile, a tile with one row, masked halves."""
+    G = 2
+    lens = [b % 3 for b in range(B)]
+    q, kp, vp, k, v = inputs(B, 1, G, P, 4, lens, P)
+    out, _ = run(q, kp, vp, k, v, lens, B, 1, G)
+    got = out.cpu().double().view(B, G, 128)
+    for n in (0, 1, 2):                                    # all sequences of a length at once
+        at = torch.tensor([b for b in range(B) if lens[b] == n])
+        kk = torch.cat((kp.expand(len(at), -1, -1), k[at, :n]), 1).double()
+        vv = torch.cat((vp.expand(len(at), -1, -1), v[at, :n]), 1).double()
+        qq = q.view(B, G, 128)[at].double()
+        w = torch.softmax(qq @ kk.transpose(1, 2) * SCALE, -1)
+        ref, mag = w @ vv, w @ vv.abs()
+        e = float((qq.abs() @ kk.abs().transpose(1, 2)).max()) * 2.0 ** -22 * SCALE
+        assert bool(((got[at] - ref).abs() <= output_bound(ref, mag, torch.bfloat16, e)).all())
+
+
+def test_a_prefix_that_no_tensor_map_can_describe():
+    """One KV head's rows for all heads (a stride of zero): served by the list."""
+    B, Hk, G, P = 40, 2, 2, 3000
+    lens = [5] * B
+    q, kp, vp, k, v = inputs(B, Hk, G, P, 8, lens, 2)
+    one_k, one_v = kp[:1].to(DEV).expand(Hk, -1, -1), vp[:1].to(DEV).expand(Hk, -1, -1)
+    attn = PrefixAttentionGraph(B=B, H=Hk * G, H_kv=Hk, d=128, dtype=torch.bfloat16, device=DEV)
+    out = attn(q.to(DEV), one_k, one_v, k.to(DEV), v.to(DEV), torch.tensor([5], dtype=torch.int32, device=DEV))
+    check_against_definition(out, q, kp[:1].expand(Hk, -1, -1), vp[:1].expand(Hk, -1, -1), k, v, lens, G, torch.bfloat16)
+
+
 def test_offsets_beyond_31_bits():
     """A prefix head that begins more than 2^31 bytes into its tensor."""
     Hk, P, L = 3, 40, 16

@@ -178,6 +178,47 @@ def test_a_ragged_batch_with_empty_sequences_and_lengths_beyond_the_cache(bits):
 
 
 @pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("H,G,lens", [(8, 2, [37 * b % 301 for b in range(90)]),           # more heads than CTAs, several a CTA
+                                      (1, 8, [0] * 20 + [1] * 20 + [2000]), (1, 3, [6000, 1, 500]), (5, 1, [3000] * 4)])
+@pytest.mark.parametrize("ctas", [None, 1, 7, 64])
+def test_every_way_of_sharing_rows_out(bits, H, G, lens, ctas):
+    """Many short heads, one long among them, few CTAs: runs that meet several heads and heads that meet several runs."""
+    B = len(lens)
+    cache, k, v = random_cache(B, H, max(lens), bits, B + H, lens)
+    q = (torch.randn(B * H * G, 128, generator=torch.Generator().manual_seed(B)) * 2).to(torch.bfloat16)
+    attn = QuantAttentionGraph(H=B * H * G, H_kv=B * H, d=128, dtype=torch.bfloat16, device=DEV)
+    attn.n_group = H
+    if ctas is not None:
+        attn.ctas = ctas
+        attn.ws = torch.zeros(lib().skv_quant_workspace_bytes(B * H, G, 128, ctas), dtype=torch.uint8, device=DEV)
+    n_dev = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = attn(q.to(DEV), cache, 0, n_dev).clone()
+    assert torch.equal(attn(q.to(DEV), cache, 0, n_dev), out)
+    got = out.cpu().double().view(B, H, G, 128)
+    for b, n in enumerate(lens):
+        for h in range(H):
+            qh = q.view(B, H, G, 128)[b, h]
+            ref, mag = attention(qh, k[b, h, :n], v[b, h, :n], SCALE)
+            e = score_error(qh, k[b, h, :n], bits) if n else 0.0
+            assert bool(((got[b, h] - ref).abs() <= output_bound(ref, mag, torch.bfloat16, e)).all()), (b, h)
+
+
+def test_queries_that_alias_the_output_and_a_negative_softmax_scale():
+    H, G, n = 2, 4, 300
+    cache, k, v = random_cache(1, H, n, 8, 41)
+    attn = QuantAttentionGraph(H=H * G, H_kv=H, d=128, dtype=torch.bfloat16, device=DEV)
+    n_dev = torch.tensor([n], dtype=torch.int32, device=DEV)
+    q = torch.randn(H * G, 128, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).to(DEV)
+    want = attn(q, cache, 0, n_dev).clone()
+    attn.out.copy_(q)
+    assert torch.equal(attn(attn.out, cache, 0, n_dev), want)
+    wide = torch.zeros(H * G, 129, dtype=torch.bfloat16, device=DEV)[:, 1:].copy_(q)         # strided and off the boundary
+    assert torch.equal(attn(wide, cache, 0, n_dev), want)
+    attn._scale = -attn._scale
+    assert torch.equal(attn(-q, cache, 0, n_dev), want)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
 def test_large_and_small_queries_keep_their_scores(bits):
     """Queries and keys far from 1: the queries' own scale must not matter."""
     H, G, n = 2, 2, 200

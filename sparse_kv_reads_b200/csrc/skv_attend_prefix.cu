@@ -2,8 +2,9 @@
 // each sequence's own rows behind it.
 //
 // bf16, two launches.  The first reads the prefix once per KV head for all sequences together: their batch x G query rows
-// are the M side of tcgen05 products over 128-key tiles (prefix_mma_kernel, below).  The second attends over the own rows,
-// one CTA per (split, sequence, KV head), and its last CTA per head merges everything.
+// are the M side of tcgen05 products over 128-key tiles (prefix_mma_kernel).  The second attends over the own rows and merges
+// everything (prefix_own_kernel); where the prefix is short or the batch small it takes the prefix's rows as well and is the
+// only launch.
 // float32: a (sequence, KV head) pair walks the prefix and its own rows as one list, half a warp per row, float32
 // arithmetic on the CUDA cores.
 #include <cuda.h>
@@ -111,8 +112,15 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
 // from tensor memory, so that no maximum needs a shuffle, and writes the weights back over them in bf16 as the A operand of
 // the second product.  One thread feeds the ring of K and V tiles by TMA (rows beyond the prefix read as zeros), one issues
 //   S = Q K^T  (both K-major in shared memory)        O += P V  (P in tensor memory, V MN-major)
-// with S of the next tile issued before O of this one has to wait for its weights: the slots' softmax and products overlap.
-// Accumulators are rescaled only when a row's maximum rises by more than 8 (base 2).
+// with the two slots strictly in turn, so that one's products run beside the other's softmax.  Accumulators are rescaled only
+// when a row's maximum rises by more than 8 (base 2).
+// What bounds it.  Up to 128 rows the memory: a tile of 64 KB takes an SM about 2,700 cycles, which is the copy rate over 144
+// SMs; the rest of 27 us for 8 heads x 32,768 keys (floor 20.5 us) is the start (4,000 cycles to the first scores) and the way
+// out.  With more rows the chain of a slot: about 1,850 cycles of softmax (1,330 of them exponentials, 1,024 at the least),
+// then 1,024 of products and the hand-overs; 3,430 cycles a tile where the tensor cores alone need 2,048.
+// Measured and not kept (128 sequences x 4 query heads x 16,383 keys, 53.5 us with the second launch): scores and weights by
+// halves of a tile (71.6 us: with 64 keys on N the queries are read from shared memory twice as often), an issuing thread per
+// slot (62.4 us: the slots fall into step), weights released by halves (54.9 us).
 constexpr int PT = 128;                                   // keys of a tile, rows of a slot
 constexpr int PSTAGES = 2;
 constexpr uint32_t P_TILE = PT * 256;                     // bytes of a 128 x 128 bf16 tile: two halves of 64 components
@@ -199,8 +207,8 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
             const int i = tid + e * P_THREADS, r = i >> 4, c = i & 15, rr = r & (PT - 1);
             if (r >= qrows) continue;
             v[e].x ^= flip; v[e].y ^= flip; v[e].z ^= flip; v[e].w ^= flip;
-            *reinterpret_cast<uint4 *>(smem + (r >> 7) * P_TILE + (c >> 3) * (P_TILE / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
-                v[e];
+            unsigned char *to = smem + (r >> 7) * P_TILE + (c >> 3) * (P_TILE / 2) + rr * 128;
+            *reinterpret_cast<uint4 *>(to + (((c & 7) ^ (rr & 7)) << 4)) = v[e];
         }
     }
     fence_async_proxy();
@@ -424,8 +432,10 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
 
 // The sequences' own rows, and everything merged: grid (CTAs, sequence x KV head).  Own rows that one CTA serves alone may be
 // served by several all the same, each for some of the query heads: the partials of a long prefix take longer to join than
-// a few own rows to read (8 sequences of one KV head with 8 query heads, 30,000 + 100 rows: 32 us with one).  With `listed`, the prefix's rows
-// too, as one list ahead of the own ones (short prefixes and small batches, which the second-level cache serves).
+// a few own rows to read (8 sequences of one KV head with 8 query heads, 30,000 + 100 rows: 32 us with one CTA per head, 17.6
+// with eight).  With `listed`, the prefix's rows too, as one list ahead of the own ones (short prefixes and small batches,
+// which the second-level cache serves).  Bounded by latencies: 46 MB of own rows and 18 partials each of 512 query rows take
+// 10 us alone, 7 us of which the memory needs.
 // STAGES tiles of 16 rows per warp: as many as the shared memory allows at the CTAs per SM that the grid makes.
 template <int STAGES>
 __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p) {
@@ -446,7 +456,8 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
     }
     const int slots = s_eff * WARPS, per = (tiles + slots - 1) / slots;
     const int t0 = min((s_eff == 1 ? warp : split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
-    const char *ko = static_cast<const char *>(p.k) + (int64_t)head * p.ksh * 2, *vo = static_cast<const char *>(p.v) + (int64_t)head * p.vsh * 2;
+    const char *ko = static_cast<const char *>(p.k) + (int64_t)head * p.ksh * 2;
+    const char *vo = static_cast<const char *>(p.v) + (int64_t)head * p.vsh * 2;
     WarpAttendT<STAGES> wa;
     wa.init(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)head * G * HEAD_DIM, G, smem + warp * (STAGES * 8192),
             s_vmask[warp], static_cast<const char *>(p.kp) + (int64_t)h * p.kph * 2,
@@ -570,13 +581,15 @@ static int launch_own(const PrefixParams &p, cudaStream_t st) {
     }
     // Behind the prefix's launch, which waits for everything before it, this one may always start early: its own rows are
     // read while the last tiles of the prefix are multiplied.
-    SKV_CUDA_OK(launch_as(pdl_allowed() && p.prefix_splits > 0, prefix_own_kernel<STAGES>, dim3(p.own_ctas, p.batch * p.h_kv), dim3(128),
-                          SMEM, st, p));
+    SKV_CUDA_OK(launch_as(pdl_allowed() && p.prefix_splits > 0, prefix_own_kernel<STAGES>, dim3(p.own_ctas, p.batch * p.h_kv),
+                          dim3(128), SMEM, st, p));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
 
-// The prefix's rows go through the list where reading them once per sequence moves at most this much.
+// The prefix's rows go through the list where reading them once per sequence moves at most this much, for the most part
+// through the second-level cache (two sequences of 8,192 rows, 67 MB: 14.3 us by the list, 16.4 by the tiles; four, 134 MB:
+// 21.1 and 15.2; four of 333 rows: 6.7 and 9.5).
 constexpr int64_t LIST_BYTES = 64 << 20;
 
 // Most CTAs the prefix of a KV head is split over: one per SM over all heads and row groups.  (A call uses at most a third
@@ -695,5 +708,5 @@ extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->dtype == SKV_F32) return launch_prefix_simple<float>(p, st);
-    return splits > 1 ? launch_prefix_mma(p, st) : launch_prefix_simple<__nv_bfloat16>(p, st);
+    return launch_prefix_mma(p, st);
 }

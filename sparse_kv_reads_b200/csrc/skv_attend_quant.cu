@@ -3,14 +3,17 @@
 // bf16 queries: tensor-core kernel.  Both products take half-float operands, because a code turns into a half float with
 // one byte permutation or one logic operation: 0x6400 | c is 1024 + c, 0x6400 | c << 4 is 1024 + 16 c.
 //   S^T = K Q^T (16 keys on M, up to 8 query heads on N).  The order of the 128 components is free as long as both sides
-//     agree on it, so a lane takes a row's bytes 16 at a time and the queries are fetched in the matching order.  The offsets (1152 = 1024 + 128 in 8 bits) stay
-//     in the codes: the accumulators start at minus the offset times the sum of the query.  Queries are scaled by a power
-//     of two to a largest component in [1, 2), which half floats hold to 2^-25 of that.
+//     agree on it, so a lane takes a row's bytes 16 at a time and the queries are fetched in the matching order.  The
+//     offsets (1152 = 1024 + 128 in 8 bits) stay in the codes: the accumulators start at minus the offset times the sum of
+//     the query.  Queries are scaled by a power of two to a largest component in [1, 2), which half floats hold to 2^-25 of
+//     that.
 //   O^T = V^T (P vs): component d of the values on M, keys on K.  A lane reads the same bytes of the value rows of its
-//     four keys and pairs them up by permutation.
+//     four keys and pairs them up by permutation.  The value's scale goes into the weights (per scale group in 4 bits).
 // A warp has a ring of tiles of its own in shared memory, filled by 16-byte asynchronous copies and laid out so that neither
-// the rows' nor the columns' reads meet in a bank (loads straight into registers kept one tile in flight per warp: 46 us
-// against XX us for the ragged 8-bit batch, 86 against XX for 64 heads of 32,768 4-bit rows).  The value's scale goes into the weights (per scale group in 4 bits).
+// the rows' nor the columns' reads meet in a bank.  (Loads straight into registers kept one tile in flight per warp: 109 us
+// against 92 us for 64 heads of 32,768 8-bit rows, 85 against 75 us in 4 bits.)
+// What bounds it: 8 bits, the memory (64 heads of 32,768 rows: 83 us at the measured copy rate); 4 bits, the instructions
+// that turn two codes a byte into fragments (338 per 16 rows; the integer pipe is 55 % busy, the memory 60 %).
 // Two running references per head, in base 2: m for the sum of weights (largest score) and r for the accumulators (largest
 // score + log2 of the value's scale), so that the half floats 2^(z - r) vs keep their precision whatever the scales.  A
 // reference is only raised when something passes it by 8: products up to 256 cost a half float nothing, and most tiles
@@ -158,7 +161,8 @@ struct WarpAttendQuant {
     static constexpr int GR = Q::GROUPS;
     uint32_t qb[8][2];                 // Q^T fragments in the order of the codes, column = head g
     float off[GR][2];                  // what the accumulators of heads 2t, 2t + 1 start from, per scale group
-    float acc[8][4];                   // O^T: 8-bit tile j: components 16 g + 2 j, + 1; 4-bit tile (group, i): 32 group + 4 g + 2 i, + 1
+    float acc[8][4];                   // O^T: 8-bit tile j: components 16 g + 2 j and the next; 4-bit tile (group, i): 32 group
+                                       // + 4 g + 2 i and the next
     float mA, mB, lA, lB;              // reference of the weights / partial sum of heads 2t, 2t + 1
     float rA, rB, fA, fB;              // reference of the accumulators, and 2^(m - r)
     float qsA, qsB;                    // score scale of the two heads, with the query's power of two
@@ -397,7 +401,8 @@ struct Ring {
         copy = eight * 128 + (((lane & 7) ^ (BITS == 8 ? eight : 2 * eight)) << 4);
     }
     // start the copies of a tile, `left` of its positions cached; k, v, s: where the tile begins in memory
-    __device__ __forceinline__ void issue(int stage, const unsigned char *k, const unsigned char *v, const unsigned char *s, int left) {
+    __device__ __forceinline__ void issue(int stage, const unsigned char *k, const unsigned char *v, const unsigned char *s,
+                                          int left) {
         unsigned char *to = base + stage * BYTES;
         constexpr int PER = 512 / Q::ROW_BYTES;           // rows that the warp copies at once
 #pragma unroll
@@ -412,7 +417,8 @@ struct Ring {
             if (BITS == 4) cp_async16(to + 2 * CODES + lane * 16, ok ? s + lane * 16 : s, ok ? 16 : 0);
             else {
                 const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(to + 2 * CODES + lane * 4));
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(ok ? s + lane * 4 : s), "r"(ok ? 4 : 0));
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(ok ? s + lane * 4 : s),
+                             "r"(ok ? 4 : 0));
             }
         }
     }
@@ -438,7 +444,8 @@ struct Ring {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                     // rows 2t, 2t + 1, 2t + 8, 2t + 9
             if constexpr (BITS == 8)
-                r.v[i] = *reinterpret_cast<const uint4 *>(v + (2 * t + (i & 1) + 8 * (i >> 1)) * 128 + ((g ^ (2 * t + (i & 1))) << 4));
+                r.v[i] = *reinterpret_cast<const uint4 *>(v + (2 * t + (i & 1) + 8 * (i >> 1)) * 128 +
+                                                          ((g ^ (2 * t + (i & 1))) << 4));
             else
                 r.v[i] = *reinterpret_cast<const uint2 *>(v + (t + 4 * (i >> 1)) * 128 +
                                                           (((((i & 1) << 2) + (g >> 1)) ^ (2 * t)) << 4) + (g & 1) * 8);
@@ -576,7 +583,8 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
             if (lane == 0) {
                 s_head[warp] = head + 1; s_place[warp] = place + blocks; s_b0[warp] = 0;
                 if (warp == 0 && !s_even) {               // CTAs that meet this head: from its first block's to its last's
-                    const int c0 = (int)mul_div(place + 1, s_ctas, s_line, 1), c1 = (int)mul_div(place + blocks, s_ctas, s_line, 1);
+                    const int c0 = (int)mul_div(place + 1, s_ctas, s_line, 1);
+                    const int c1 = (int)mul_div(place + blocks, s_ctas, s_line, 1);
                     s_seg[segs] = {head, (int)blockIdx.x - c0, c1 - c0 + 1, (int64_t)c0 + head};
                 }
             }
@@ -649,13 +657,14 @@ template <int BITS, int U, int STAGES>
 static int launch_quant_mma(const AttendQuantParams &p, cudaStream_t st) {
     auto kern = attend_quant_mma_kernel<BITS, U, STAGES>;
     constexpr int RINGS = 4 * STAGES * Ring<BITS, U, STAGES>::BYTES;
-    static_assert(QUANT_CTAS_PER_SM * (RINGS + QUANT_MOST_ROWS * PART_LD * 4 + 4096) <= 227 * 1024, "the CTAs of an SM fit at eight query heads");
+    constexpr int MOST = RINGS + QUANT_MOST_ROWS * PART_LD * 4;
+    static_assert(QUANT_CTAS_PER_SM * (MOST + 4096) <= 227 * 1024, "the CTAs of an SM fit whatever the query heads");
     static bool configured[64] = {};       // the attribute is kept per device
     int dev = 0;
     SKV_CUDA_OK(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return SKV_E_RANGE;
     if (!configured[dev]) {
-        SKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RINGS + QUANT_MOST_ROWS * PART_LD * 4));
+        SKV_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
         configured[dev] = true;
     }
     SKV_CUDA_OK(launch_early(kern, dim3(p.ctas), dim3(128), (size_t)RINGS + (size_t)p.rows * PART_LD * 4, st, p));

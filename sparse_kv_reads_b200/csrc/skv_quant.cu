@@ -1,6 +1,8 @@
 // Writing rows into a quantised KV cache and reading them back.
 //
-// Both move a few bytes per value and compute little: HBM-bound for a prefill chunk, launch-bound for a decode step.
+// A prefill chunk is bounded by the memory, with the instructions close behind (eight sequences x 8 heads x 2,048 positions in
+// 4 bits, under a profiler: write 23 us for 86 MB, 65 % of the issue slots taken; read 15.4 us); a decode step's few rows by
+// the launch.  An IEEE division per value made the write 35 us.
 // Half a warp serves one cached position of one KV head, key and value together (a lane has 8 values of each), and two
 // positions at once, so that a lane's four loads are requested before any is used.
 #include "skv_quant.cuh"
@@ -185,7 +187,9 @@ __device__ __forceinline__ __nv_bfloat162 bf2(uint32_t x) { return *reinterpret_
 template <int BITS> struct Stored;
 template <> struct Stored<8> {
     uint2 w;
-    __device__ __forceinline__ void load(const unsigned char *row, int sub) { w = __ldcs(reinterpret_cast<const uint2 *>(row + sub * 8)); }
+    __device__ __forceinline__ void load(const unsigned char *row, int sub) {
+        w = __ldcs(reinterpret_cast<const uint2 *>(row + sub * 8));
+    }
     __device__ __forceinline__ void store(__nv_bfloat16 *out, __nv_bfloat16 scale) const {
         const __nv_bfloat162 s = __halves2bfloat162(scale, scale);
         uint32_t o[4];
@@ -196,7 +200,9 @@ template <> struct Stored<8> {
         }
         *reinterpret_cast<uint4 *>(out) = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    __device__ __forceinline__ float code(int i) const { return (float)((int)(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255u) - 128); }
+    __device__ __forceinline__ float code(int i) const {
+        return (float)((int)(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255u) - 128);
+    }
 };
 template <> struct Stored<4> {
     uint32_t r0, r1;
@@ -215,7 +221,9 @@ template <> struct Stored<4> {
         }
         *reinterpret_cast<uint4 *>(out) = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    __device__ __forceinline__ float code(int i) const { return (float)((int)(((i < 4 ? r0 : r1) >> (4 * (i & 3))) & 15u) - 8); }
+    __device__ __forceinline__ float code(int i) const {
+        return (float)((int)(((i < 4 ? r0 : r1) >> (4 * (i & 3))) & 15u) - 8);
+    }
 };
 template <int BITS>
 __device__ __forceinline__ void store_values(float *out, const Stored<BITS> &c, __nv_bfloat16 scale) {
@@ -224,7 +232,9 @@ __device__ __forceinline__ void store_values(float *out, const Stored<BITS> &c, 
     *reinterpret_cast<float4 *>(out + 4) = make_float4(c.code(4) * s, c.code(5) * s, c.code(6) * s, c.code(7) * s);
 }
 template <int BITS>
-__device__ __forceinline__ void store_values(__nv_bfloat16 *out, const Stored<BITS> &c, __nv_bfloat16 scale) { c.store(out, scale); }
+__device__ __forceinline__ void store_values(__nv_bfloat16 *out, const Stored<BITS> &c, __nv_bfloat16 scale) {
+    c.store(out, scale);
+}
 
 template <typename T, int BITS, bool FLAT>
 __global__ void __launch_bounds__(256) quant_read_kernel(const RowsParams p) {
@@ -364,8 +374,9 @@ extern "C" int skv_quant_write(const skv_qcache *c, const skv_rows *r, void *str
     if (r->tokens == 0) return SKV_OK;
     p.pos_per_seq = r->pos_per_seq;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (r->dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_write<__nv_bfloat16, 8>(p, st) : launch_write<__nv_bfloat16, 4>(p, st)));
-    else SKV_CUDA_OK((c->bits == 8 ? launch_write<float, 8>(p, st) : launch_write<float, 4>(p, st)));
+    const bool bf16 = r->dtype == SKV_BF16;
+    if (c->bits == 8) SKV_CUDA_OK((bf16 ? launch_write<__nv_bfloat16, 8>(p, st) : launch_write<float, 8>(p, st)));
+    else SKV_CUDA_OK((bf16 ? launch_write<__nv_bfloat16, 4>(p, st) : launch_write<float, 4>(p, st)));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -379,8 +390,9 @@ extern "C" int skv_quant_read(const skv_qcache *c, const skv_rows *r, void *stre
     if (r->tokens == 0) return SKV_OK;
     p.pos_per_seq = r->pos_per_seq;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (r->dtype == SKV_BF16) SKV_CUDA_OK((c->bits == 8 ? launch_read<__nv_bfloat16, 8>(p, st) : launch_read<__nv_bfloat16, 4>(p, st)));
-    else SKV_CUDA_OK((c->bits == 8 ? launch_read<float, 8>(p, st) : launch_read<float, 4>(p, st)));
+    const bool bf16 = r->dtype == SKV_BF16;
+    if (c->bits == 8) SKV_CUDA_OK((bf16 ? launch_read<__nv_bfloat16, 8>(p, st) : launch_read<float, 8>(p, st)));
+    else SKV_CUDA_OK((bf16 ? launch_read<__nv_bfloat16, 4>(p, st) : launch_read<float, 4>(p, st)));
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }

@@ -436,9 +436,11 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
 // with eight).  With `listed`, the prefix's rows too, as one list ahead of the own ones (short prefixes and small batches,
 // which the second-level cache serves).  Bounded by latencies: 46 MB of own rows and 18 partials each of 512 query rows take
 // 10 us alone, 7 us of which the memory needs.
-// STAGES tiles of 16 rows per warp: as many as the shared memory allows at the CTAs per SM that the grid makes.
+// STAGES tiles of 16 rows per warp: as many as the shared memory allows at the CTAs per SM that the grid makes.  Beyond three
+// per SM one tile and four CTAs: more CTAs at once are worth more than tiles asked for ahead (1,024 heads: 49 us against 55 us
+// for both launches with 40 own rows, 96 against 95 with 1,000).
 template <int STAGES>
-__global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p) {
+__global__ void __launch_bounds__(128, STAGES == 1 ? 4 : 3) prefix_own_kernel(const PrefixParams p) {
     constexpr int WARPS = 4;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t s_vmask[WARPS][STAGES];
@@ -477,7 +479,7 @@ __global__ void __launch_bounds__(128, 3) prefix_own_kernel(const PrefixParams p
     if (s_eff == 1) {
         // Alone: the prefix's partials straight from where they lie.  Every warp folds a quarter of each row's into its own
         // partial (a lane has four columns; the loads of two query heads are in flight together), then the four are joined.
-        constexpr int AT_ONCE = 5;
+        constexpr int AT_ONCE = STAGES == 1 ? 3 : 5;
         const int lane = tid & 31;
         const int ga = G * split / joint, gb = G * (split + 1) / joint;      // this CTA's query heads
         for (int g0 = ga; g0 < gb; g0 += 2) {
@@ -657,7 +659,7 @@ static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
         SKV_CUDA_OK(launch_early(prefix_mma_kernel, dim3(ps, groups, p.h_kv), dim3(P_THREADS), P_SMEM, st, p, kmap, vmap));
     }
     const int ctas = heads * p.own_ctas, sms = device_sm_count();
-    return ctas <= sms ? launch_own<6>(p, st) : ctas <= 2 * sms ? launch_own<3>(p, st) : launch_own<2>(p, st);
+    return ctas <= sms ? launch_own<6>(p, st) : ctas <= 2 * sms ? launch_own<3>(p, st) : ctas <= 3 * sms ? launch_own<2>(p, st) : launch_own<1>(p, st);
 }
 
 }  // namespace skv

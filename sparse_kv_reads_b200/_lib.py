@@ -212,7 +212,7 @@ def lib():
 
 
 # entry points that launch exactly one kernel each: counted, so that a caller can tell how many of the library's
-# kernels a captured decode step holds (GraphDecoder.launches_per_step)
+# kernels a captured decode step holds (GraphDecoder.launches_per_step); skv_attend_prefix launches one or two and counts one
 _ONE_LAUNCH = {"skv_insert", "skv_select", "skv_attend", "skv_attend_weighted", "skv_attend_labels", "skv_step", "skv_gemv", "skv_gemv_tp", "skv_gemv_attended",
                "skv_add_rmsnorm", "skv_qk_rope_cache", "skv_silu_mul", "skv_comm_push", "skv_comm_reduce", "skv_comm_tick",
                "skv_quant_write", "skv_quant_read", "skv_qk_rope_quant", "skv_attend_quant", "skv_attend_prefix"}

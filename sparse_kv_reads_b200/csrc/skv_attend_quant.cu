@@ -13,7 +13,7 @@
 // the rows' nor the columns' reads meet in a bank.  (Loads straight into registers kept one tile in flight per warp: 109 us
 // against 92 us for 64 heads of 32,768 8-bit rows, 85 against 75 us in 4 bits.)
 // What bounds it: 8 bits, the memory (64 heads of 32,768 rows: 83 us at the measured copy rate); 4 bits, the instructions
-// that turn two codes a byte into fragments (338 per 16 rows; the integer pipe is 55 % busy, the memory 60 %).
+// that turn two codes a byte into fragments (322 per 16 rows; the integer pipe is 54 % busy, the memory 61 %).
 // Two running references per head, in base 2: m for the sum of weights (largest score) and r for the accumulators (largest
 // score + log2 of the value's scale), so that the half floats 2^(z - r) vs keep their precision whatever the scales.  A
 // reference is only raised when something passes it by 8: products up to 256 cost a half float nothing, and most tiles
@@ -139,6 +139,21 @@ __device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 constexpr uint32_t F16_1024 = 0x64006400u;                // two half floats of 1024, whose last place counts 1
 
+// d = a b + c: the start of a chain of products (d and c apart, so that c need not be copied first)
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1, const float (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// log2 of a scale: zero or a normal number (-inf for zero)
+__device__ __forceinline__ float log2_scale(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // What one lane holds of 16 cached positions: lane = 4 g + t.  Keys: rows g and g + 8; values: rows 2t, 2t+1, 2t+8, 2t+9.
 template <int BITS>
 struct RawTile;
@@ -245,9 +260,10 @@ struct WarpAttendQuant {
                 const uint32_t sel = gr & 1 ? 0x7632 : 0x5410;
                 uint32_t a = gr < 2 ? __byte_perm(r.k[0].x, r.k[0].z, sel) : __byte_perm(r.k[0].y, r.k[0].w, sel);
                 uint32_t b = gr < 2 ? __byte_perm(r.k[1].x, r.k[1].z, sel) : __byte_perm(r.k[1].y, r.k[1].w, sel);
-                float c[4] = {off[gr][0], off[gr][1], off[gr][0], off[gr][1]};
+                float c[4];
                 mma_f16_16816(c, and_or(a, 0x000f000fu, F16_1024), and_or(b, 0x000f000fu, F16_1024),
-                              and_or(a, 0x00f000f0u, F16_1024), and_or(b, 0x00f000f0u, F16_1024), qb[2 * gr][0], qb[2 * gr][1]);
+                              and_or(a, 0x00f000f0u, F16_1024), and_or(b, 0x00f000f0u, F16_1024), qb[2 * gr][0], qb[2 * gr][1],
+                              {off[gr][0], off[gr][1], off[gr][0], off[gr][1]});
                 a >>= 8; b >>= 8;
                 mma_f16_16816(c, and_or(a, 0x000f000fu, F16_1024), and_or(b, 0x000f000fu, F16_1024),
                               and_or(a, 0x00f000f0u, F16_1024), and_or(b, 0x00f000f0u, F16_1024), qb[2 * gr + 1][0],
@@ -296,7 +312,7 @@ struct WarpAttendQuant {
                 v0 = fmaxf(v0, value_scale(r[u], 0, gr));
                 v1 = fmaxf(v1, value_scale(r[u], 1, gr));
             }
-            v0 = __log2f(v0); v1 = __log2f(v1);            // (-inf for values of zero: they never raise r)
+            v0 = log2_scale(v0); v1 = log2_scale(v1);      // (-inf for values of zero: they never raise r)
             tA = fmaxf(tA, fmaxf(z[u][0], z[u][2])); tB = fmaxf(tB, fmaxf(z[u][1], z[u][3]));
             yA = fmaxf(yA, fmaxf(z[u][0] + v0, z[u][2] + v1)); yB = fmaxf(yB, fmaxf(z[u][1] + v0, z[u][3] + v1));
         }
@@ -386,6 +402,11 @@ struct WarpAttendQuant {
     }
 };
 
+__device__ __forceinline__ void cp_async4(void *smem_dst, const void *gsrc, int src_bytes) {
+    const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(smem_dst));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(gsrc), "r"(src_bytes));
+}
+
 // One warp's ring in shared memory: STAGES tiles of 16 U positions.  8 bits: the 16-byte chunk c of row r lies at place
 // c ^ (r % 8) of the row's 128 bytes.  4 bits: two rows share 128 bytes, chunk c of row r lies at place
 // (4 (r % 2) + c) ^ (2 (r / 2) % 8) of them.  Either way the eight lanes that read together meet no bank twice.
@@ -405,6 +426,19 @@ struct Ring {
                                           int left) {
         unsigned char *to = base + stage * BYTES;
         constexpr int PER = 512 / Q::ROW_BYTES;           // rows that the warp copies at once
+        if (left >= ROWS) {                               // all but the last tile: nothing to ask about
+#pragma unroll
+            for (int i = 0; i < ROWS / PER; ++i) {
+                const int at = i * 512 + (BITS == 8 ? copy ^ ((i & 1) << 6) : copy);
+                cp_async16(to + at, k + i * 512 + lane * 16, 16);
+                cp_async16(to + CODES + at, v + i * 512 + lane * 16, 16);
+            }
+            if (lane < ROWS) {
+                if (BITS == 4) cp_async16(to + 2 * CODES + lane * 16, s + lane * 16, 16);
+                else cp_async4(to + 2 * CODES + lane * 4, s + lane * 4, 4);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < ROWS / PER; ++i) {
             const bool ok = i * PER + lane / (32 / PER) < left;
@@ -415,11 +449,7 @@ struct Ring {
         if (lane < ROWS) {
             const bool ok = lane < left;
             if (BITS == 4) cp_async16(to + 2 * CODES + lane * 16, ok ? s + lane * 16 : s, ok ? 16 : 0);
-            else {
-                const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(to + 2 * CODES + lane * 4));
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(ok ? s + lane * 4 : s),
-                             "r"(ok ? 4 : 0));
-            }
+            else cp_async4(to + 2 * CODES + lane * 4, ok ? s + lane * 4 : s, ok ? 4 : 0);
         }
     }
     __device__ __forceinline__ void keys(int stage, int u, RawTile<BITS> &r) const {

@@ -483,6 +483,38 @@ struct Ring {
     }
 };
 
+// Merge of heads with few partials, by warps: one warp a query head, all its partials asked for at once, a lane owns four
+// columns.  (merge_head goes head by head, staging and synchronising: a CTA that had met two heads and merged both ended 7 us
+// behind the others, 42.8 against 40.5 us for 16 ragged sequences of 8 heads with four query heads.)
+constexpr int QUANT_FEW = 8;
+template <typename Params>
+__device__ __forceinline__ void merge_few(const Params &p, int row, int head, int parts, int64_t slot0) {
+    const int lane = threadIdx.x & 31;
+    const float *src = p.part + (slot0 * p.G + row) * PART_LD;
+    float2 ml = make_float2(NEG_BIG, 0.f);
+    if (lane < parts) ml = __ldcg(reinterpret_cast<const float2 *>(src + (int64_t)lane * p.G * PART_LD + HEAD_DIM));
+    float4 a[QUANT_FEW];
+#pragma unroll
+    for (int i = 0; i < QUANT_FEW; ++i) {
+        a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < parts) a[i] = __ldcg(reinterpret_cast<const float4 *>(src + (int64_t)i * p.G * PART_LD) + lane);
+    }
+    const float f = fast_exp2(ml.x - warp_max(ml.x));
+    const float den = warp_sum(f * ml.y);
+    float4 nm = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < QUANT_FEW; ++i) {
+        if (i >= parts) break;
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        nm.x = fmaf(fi, a[i].x, nm.x); nm.y = fmaf(fi, a[i].y, nm.y);
+        nm.z = fmaf(fi, a[i].z, nm.z); nm.w = fmaf(fi, a[i].w, nm.w);
+    }
+    const bool any = den > 0.f;
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + ((int64_t)head * p.G + row) * HEAD_DIM + lane * 4;
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(any ? nm.x / den : 0.f, any ? nm.y / den : 0.f),
+                                                 pack_bf16(any ? nm.z / den : 0.f, any ? nm.w / den : 0.f));
+}
+
 constexpr int QUANT_CTAS_PER_SM = 2;
 constexpr int QUANT_MAX_SEG = 32;       // heads of a CTA whose partials wait in shared memory
 // Rows of 132 floats of shared memory behind the rings: the warps' partials of one head of eight query heads, of two and
@@ -490,12 +522,15 @@ constexpr int QUANT_MAX_SEG = 32;       // heads of a CTA whose partials wait in
 constexpr int QUANT_MOST_ROWS = 32;
 static int quant_rows(int G) { return 8 * G < 16 ? 16 : 8 * G > QUANT_MOST_ROWS ? QUANT_MOST_ROWS : 8 * G; }
 
-// The ways of sharing the work out, below, in blocks of 16 rows.  Measured on B200 (8-bit rows, two query heads, us):
-// ALONE: a head up to this long is left to one CTA, without a merge (32 blocks: 8.2, in two parts 9.7; 63 blocks: 10.2 and
-//   8.6 in ten parts).  LEAST: blocks of a CTA at least, where a head is split.  HOP: what the longest run of an even
-//   sharing may be beyond the average (64 heads of 512 blocks: even 35.8, line 36.9; of 2,048: 116 and 109; 8 heads of
-//   2,048: 21.8 and 25.6).
-constexpr int QUANT_ALONE = 32, QUANT_LEAST = 8, QUANT_HOP = 24;
+// The ways of sharing the work out, below, in blocks of 16 rows.  Measured on B200 (two query heads, 8-bit rows, us):
+// ALONE: a head up to this long is left to one CTA, without a merge (400 rows: 7.8, in two parts 8.0; 1,000 rows: 10.2 and
+//   8.8 in seven parts).  LEAST: blocks of a CTA at least, where a head is split (4: 9.1 for 1,000 rows).
+// HOP: what the longest run of an even sharing may be beyond the average (64 heads of 256 blocks, 9 beyond it: even 17.7,
+//   line 18.2; of 512 blocks, 17 beyond it: 30.6 and 28.2).
+// START: what a head's start costs the CTA that meets it on the line (filling its rings anew, a second head to publish), as
+//   if the head had so many blocks more (0 / 24 / 48: 40.5 / 39.8 / 39.4 for 16 ragged sequences of 8 heads, 70.8 / 68.7 /
+//   70.0 for 64 heads of 2,048 blocks in 4 bits).
+constexpr int QUANT_ALONE = 32, QUANT_LEAST = 8, QUANT_HOP = 16, QUANT_START = 24;
 
 // (a * b - less) / c where the result fits 31 bits: a 32-bit quotient where the product allows it (all but billions of rows)
 __device__ __forceinline__ int64_t mul_div(int64_t a, int64_t b, int64_t c, int less = 0) {
@@ -507,9 +542,10 @@ __device__ __forceinline__ int64_t mul_div(int64_t a, int64_t b, int64_t c, int 
 // The rows of all heads, cut into blocks of 16, are shared out over the CTAs in one of two ways.
 // Even: every head gets the same number of CTAs, each a run of its blocks.  It costs least where it leaves no CTA much more
 //   than the average: no CTA serves two heads.
-// Line: the blocks of all heads form one line and every CTA takes an equal run of it, whatever the lengths.  A head may be
-//   met by several CTAs and a CTA may meet several heads; the partials of the pair (CTA c, head h) have slot c + h, which
-//   no two pairs share (both only grow along the line), and a head's slots lie side by side.
+// Line: the blocks of all heads, each with QUANT_START empty places ahead of it, form one line and every CTA takes an equal
+//   run of it, whatever the lengths; a run that meets only empty places of a head does not meet the head.  A head may be met
+//   by several CTAs and a CTA may meet several heads; the partials of the pair (CTA c, head h) have slot c + h, which no two
+//   pairs share (both only grow along the line), and a head's slots lie side by side.
 // A CTA's warps take a quarter each of what the CTA has of a head and go on to the next head without waiting for one
 // another; partials are combined, published and merged at the end (or when the shared memory for them is full).
 // A head without rows counts one block, so that it gets its zeros.
@@ -525,8 +561,6 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
     constexpr int WARPS = 4, ROWS = 16 * U, MAX_SEG = QUANT_MAX_SEG;
     extern __shared__ __align__(128) unsigned char smem[];    // the warps' rings, then rows x 132 floats
     float *const red = reinterpret_cast<float *>(smem + WARPS * STAGES * Tiles::BYTES);
-    __shared__ int s_scan[40];
-    __shared__ float s_max[32];
     // (kept here, the tile loop needs the registers)
     __shared__ int64_t s_line, s_end, s_place[WARPS];     // where a warp's next head begins, and its first block there
     __shared__ int s_ctas, s_even, s_head[WARPS], s_b0[WARPS];
@@ -542,59 +576,59 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
         return max(1, (n + 15) >> 4);
     };
     auto heads_of = [&](int i) { return min(group, p.heads - i * group); };
-    // Sums of the groups' blocks ahead of this thread's contiguous share of them (they pass 31 bits beyond 34 billion
-    // rows: the lower 20 bits and the rest are scanned apart), and the longest head.
-    const int share = (groups + 127) / 128;
-    const int i0 = min(tid * share, groups), i1 = min(i0 + share, groups);
-    int64_t before = 0, mine = 0, line;
+    // Every warp for itself: blocks of the groups ahead of this lane's contiguous share of them, and the longest head
+    const int share = (groups + 31) / 32;
+    const int i0 = min(lane * share, groups), i1 = min(i0 + share, groups);
+    int64_t mine = 0;
     int longest = 0;
     for (int i = i0; i < i1; ++i) {
         const int b = blocks_of(i);
         mine += (int64_t)b * heads_of(i);
         longest = max(longest, b);
     }
-    if (groups == 1) {
-        longest = blocks_of(0);
-        line = (int64_t)longest * p.heads;
-    } else {
-        int low, high;
-        const int64_t lo = block_excl_scan((int)(mine & 0xfffff), s_scan, low);
-        const int64_t hi = block_excl_scan((int)(mine >> 20), s_scan, high);
-        before = (hi << 20) + lo;
-        line = ((int64_t)high << 20) + low;
-        longest = (int)block_max((float)longest, s_max);  // (to 24 bits: it only chooses the way of sharing)
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
     }
+    const int64_t real = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
     // CTAs per head, shared out evenly, and CTAs on the line
     const int each = longest <= QUANT_ALONE ? 1 : max(1, min(longest / QUANT_LEAST, (int)gridDim.x / p.heads));
-    const int on_line = (int)max((int64_t)1, min((int64_t)gridDim.x, line / (2 * QUANT_LEAST)));
-    const bool even = (int)gridDim.x >= p.heads && (longest + each - 1) / each <= line / on_line + QUANT_HOP;
+    const int on_line = (int)max((int64_t)1, min((int64_t)gridDim.x, real / (2 * QUANT_LEAST)));
+    const bool even = (int)gridDim.x >= p.heads && (longest + each - 1) / each <= mul_div(real, 1, on_line) + QUANT_HOP;
     const int ctas = even ? each * p.heads : on_line;
     if (blockIdx.x >= ctas) return;
     if (even) {
         const int head = blockIdx.x / each, part = blockIdx.x - head * each, b = blocks_of(head / group);
         const int parts = min(each, b);
         if (part >= parts) return;
-        if (tid < WARPS) {
-            s_head[tid] = head; s_place[tid] = 0;
-            s_b0[tid] = (int)((int64_t)b * part / parts);
-            if (tid == 0) {
-                s_end = (int64_t)b * (part + 1) / parts;
+        if (lane == 0) {
+            s_head[warp] = head; s_place[warp] = 0;
+            s_b0[warp] = (int)mul_div(b, part, parts);
+            if (warp == 0) {
+                s_end = mul_div(b, part + 1, parts);
                 s_seg[0] = {head, part, parts, (int64_t)head * each};
             }
         }
     } else {
-        const int64_t at = mul_div(line, blockIdx.x, ctas);
-        if (groups == 1 ? tid == 0 : (at >= before && at < before + mine)) {            // exactly one thread
-            int i = groups == 1 ? 0 : i0;
-            int64_t one = (int64_t)blocks_of(i) * heads_of(i);
-            while (at >= before + one) { before += one; ++i; one = (int64_t)blocks_of(i) * heads_of(i); }
-            const int h = (int)mul_div(at - before, 1, blocks_of(i));
-            const int64_t place = before + (int64_t)h * blocks_of(i);
-            s_end = mul_div(line, blockIdx.x + 1, ctas);
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) { s_head[w] = i * group + h; s_place[w] = place; s_b0[w] = (int)(at - place); }
+        const int64_t line = real + (int64_t)p.heads * QUANT_START, at = mul_div(line, blockIdx.x, ctas);
+        before += (int64_t)i0 * group * QUANT_START;
+        mine += i1 > i0 ? ((int64_t)(i1 - i0 - 1) * group + heads_of(i1 - 1)) * QUANT_START : 0;
+        if (at >= before && at < before + mine) {         // exactly one lane
+            int i = i0, b = blocks_of(i) + QUANT_START;
+            int64_t one = (int64_t)b * heads_of(i);
+            while (at >= before + one) { before += one; ++i; b = blocks_of(i) + QUANT_START; one = (int64_t)b * heads_of(i); }
+            const int h = (int)mul_div(at - before, 1, b);
+            const int64_t place = before + (int64_t)h * b;
+            s_head[warp] = i * group + h; s_place[warp] = place; s_b0[warp] = (int)(at - place);
         }
-        if (tid == 0) { s_line = line; s_ctas = ctas; }
+        if (tid == 0) {
+            s_line = line; s_ctas = ctas;
+            s_end = mul_div(line, blockIdx.x + 1, ctas);
+        }
     }
     if (tid == 0) s_even = even;
     __syncthreads();
@@ -603,18 +637,21 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
     for (bool more = true; more;) {
         int segs = 0;
         while (segs < seg_cap) {
-            const int head = s_head[warp], b0 = s_b0[warp];
+            const int head = s_head[warp];
             const int64_t place = s_place[warp];
-            more = place + b0 < s_end;
+            more = place < s_end;
             if (!more) break;
             const int n = min(max(positions_of(p.n_dev, p.n_group, head), 0), p.capacity);
-            const int blocks = max(1, (n + 15) >> 4), b1 = (int)min(s_end - place, (int64_t)blocks);
+            const int start = s_even ? 0 : QUANT_START, blocks = max(1, (n + 15) >> 4);
+            const int b0 = max(s_b0[warp] - start, 0), b1 = (int)min(s_end - place, (int64_t)(blocks + start)) - start;
+            more = b1 > b0;
+            if (!more) break;
             __syncwarp();
             if (lane == 0) {
-                s_head[warp] = head + 1; s_place[warp] = place + blocks; s_b0[warp] = 0;
+                s_head[warp] = head + 1; s_place[warp] = place + blocks + start; s_b0[warp] = 0;
                 if (warp == 0 && !s_even) {               // CTAs that meet this head: from its first block's to its last's
-                    const int c0 = (int)mul_div(place + 1, s_ctas, s_line, 1);
-                    const int c1 = (int)mul_div(place + blocks, s_ctas, s_line, 1);
+                    const int c0 = (int)mul_div(place + start + 1, s_ctas, s_line, 1);
+                    const int c1 = (int)mul_div(place + start + blocks, s_ctas, s_line, 1);
                     s_seg[segs] = {head, (int)blockIdx.x - c0, c1 - c0 + 1, (int64_t)c0 + head};
                 }
             }
@@ -666,18 +703,27 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
             shared |= s_seg[i].parts > 1;
         }
         if (shared) {
-            __threadfence();
-            __syncthreads();
+            __syncthreads();                              // the CTA's partials are on their way: one thread per head orders them
             if (tid < segs) {
                 const int parts = s_seg[tid].parts;
-                s_last[tid] = parts > 1 && atomicAdd(p.ticket + s_seg[tid].head, 1) == parts - 1;
+                bool last = false;
+                if (parts > 1) {
+                    __threadfence();
+                    last = atomicAdd(p.ticket + s_seg[tid].head, 1) == parts - 1;
+                    __threadfence();
+                    if (last) p.ticket[s_seg[tid].head] = 0;                   // ready for the next call on this stream
+                }
+                s_last[tid] = last;
             }
             __syncthreads();
-            __threadfence();
             for (int i = 0; i < segs; ++i)
-                if (s_last[i]) merge_head<__nv_bfloat16>(p, s_seg[i].head, s_seg[i].parts, s_seg[i].slot0,
-                                                         reinterpret_cast<float *>(smem),
-                                                         p.rows + WARPS * STAGES * Tiles::BYTES / (PART_LD * 4));
+                if (s_last[i] && s_seg[i].parts > QUANT_FEW)
+                    merge_head<__nv_bfloat16>(p, s_seg[i].head, s_seg[i].parts, s_seg[i].slot0, reinterpret_cast<float *>(smem),
+                                              p.rows + WARPS * STAGES * Tiles::BYTES / (PART_LD * 4));
+            for (int i = warp; i < segs * p.G; i += WARPS) {
+                const QuantSegment &one = s_seg[i / p.G];
+                if (s_last[i / p.G] && one.parts <= QUANT_FEW) merge_few(p, i % p.G, one.head, one.parts, one.slot0);
+            }
         }
         __syncthreads();                                  // the next heads' partials go where these were
     }

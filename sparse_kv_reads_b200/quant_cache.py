@@ -19,6 +19,8 @@ from ._lib import SkvError, SkvQCache, SkvRows, check, dtype_code, elsewhere, li
 
 __all__ = ["QuantKVCache", "QuantAttentionGraph"]
 
+_empty_like, _CONTIGUOUS = torch.empty_like, torch.contiguous_format
+
 
 class QuantKVCache:
     """Quantised cache of all layers, in place of ``KVCache``: ``k[i], v[i] [B, H_kv, L, 128 * bits / 8]`` uint8 and
@@ -154,7 +156,10 @@ class QuantKVCache:
         if not 0 <= count <= self.max_seq_len:
             raise ValueError(f"{count} rows lie outside the cache's {self.max_seq_len} positions")
         hs = count * self.d
-        return (2, b, self.h_kv, count, self.d), SkvRows(0, 0, None, 0, self.h_kv * hs, hs, self.d, self.h_kv * hs, hs, self.d,
+        # (a result made like a tensor at hand costs the host half of one made from a shape: 2.5 against 4.5 us for both; this
+        # one is a single element, expanded)
+        like = torch.empty(1, dtype=dtype, device=self.device).expand(b, self.h_kv, count, self.d)
+        return like, SkvRows(0, 0, None, 0, self.h_kv * hs, hs, self.d, self.h_kv * hs, hs, self.d,
                                                          0, dtype_code(dtype), b, count)
 
     def read(self, layer: int, pos, count: int, *, dtype: torch.dtype = torch.bfloat16,
@@ -162,9 +167,9 @@ class QuantKVCache:
         """The rows ``[pos, pos + count)`` of the first ``batch`` (all) sequences as ``k, v [b, H_kv, count, 128]`` of
         ``dtype``; ``pos`` as in ``write`` (rows outside the cache come back as zeros and are recorded)."""
         b, dev = self.batch if batch is None else batch, self.device
-        shape, rows = self._plan((b, count, dtype), lambda: self._plan_read(b, count, dtype))
+        like, rows = self._plan((b, count, dtype), lambda: self._plan_read(b, count, dtype))
         self._where(rows, pos, b, count)
-        k, v = torch.empty(shape, dtype=dtype, device=dev).unbind(0)
+        k, v = _empty_like(like, memory_format=_CONTIGUOUS), _empty_like(like, memory_format=_CONTIGUOUS)
         if b == 0 or count == 0:
             return k, v
         self._on_gpu()

@@ -116,11 +116,16 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
 // when a row's maximum rises by more than 8 (base 2).
 // What bounds it.  Up to 128 rows the memory: a tile of 64 KB takes an SM about 2,700 cycles, which is the copy rate over 144
 // SMs; the rest of 27 us for 8 heads x 32,768 keys (floor 20.5 us) is the start (4,000 cycles to the first scores) and the way
-// out.  With more rows the chain of a slot: about 1,850 cycles of softmax (1,330 of them exponentials, 1,024 at the least),
-// then 1,024 of products and the hand-overs; 3,430 cycles a tile where the tensor cores alone need 2,048.
+// out.  With more rows the one sequence of products: for each slot of a tile about 560 cycles for the weighted values, 650 for
+// the scores (both operands from shared memory, beside the incoming tiles) and 500 of waits and commits between them, 3,430
+// cycles a tile where the tensor cores alone need 2,048; a slot's weights lie ready 360 cycles before their turn comes (its
+// softmax takes 1,650: loads 115, maximum 280, exponentials 1,230).
 // Measured and not kept (128 sequences x 4 query heads x 16,383 keys, 53.5 us with the second launch): scores and weights by
 // halves of a tile (71.6 us: with 64 keys on N the queries are read from shared memory twice as often), an issuing thread per
-// slot (62.4 us: the slots fall into step), weights released by halves (54.9 us).
+// slot (62.4 us: the slots fall into step), weights released by halves (54.9 us).  Within 1 us of it, either way, since the
+// softmax does not bound it: half the weights against the standing reference while the maximum is found, products issued by
+// a converged warp, barriers looked at ahead of their turn (this one 2.5 us slower for 32 sequences x 32,768 keys); 1 to 5 us
+// slower: an eighth to a half of the exponentials by a polynomial on the multiply-add pipe.
 constexpr int PT = 128;                                   // keys of a tile, rows of a slot
 constexpr int PSTAGES = 2;
 constexpr uint32_t P_TILE = PT * 256;                     // bytes of a 128 x 128 bf16 tile: two halves of 64 components

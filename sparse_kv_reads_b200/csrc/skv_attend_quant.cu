@@ -579,22 +579,28 @@ __global__ void __launch_bounds__(128, QUANT_CTAS_PER_SM) attend_quant_mma_kerne
     // Every warp for itself: blocks of the groups ahead of this lane's contiguous share of them, and the longest head
     const int share = (groups + 31) / 32;
     const int i0 = min(lane * share, groups), i1 = min(i0 + share, groups);
-    int64_t mine = 0;
+    int64_t mine = 0, before = 0, real;
     int longest = 0;
-    for (int i = i0; i < i1; ++i) {
-        const int b = blocks_of(i);
-        mine += (int64_t)b * heads_of(i);
-        longest = max(longest, b);
-    }
-    longest = __reduce_max_sync(0xffffffffu, longest);
-    int64_t before = mine;
+    if (groups == 1) {
+        longest = blocks_of(0);
+        real = (int64_t)longest * p.heads;
+        if (lane == 0) mine = real;
+    } else {
+        for (int i = i0; i < i1; ++i) {
+            const int b = blocks_of(i);
+            mine += (int64_t)b * heads_of(i);
+            longest = max(longest, b);
+        }
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        before = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += x;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
+        }
+        real = __shfl_sync(0xffffffffu, before, 31);
+        before -= mine;
     }
-    const int64_t real = __shfl_sync(0xffffffffu, before, 31);
-    before -= mine;
     // CTAs per head, shared out evenly, and CTAs on the line
     const int each = longest <= QUANT_ALONE ? 1 : max(1, min(longest / QUANT_LEAST, (int)gridDim.x / p.heads));
     const int on_line = (int)max((int64_t)1, min((int64_t)gridDim.x, real / (2 * QUANT_LEAST)));

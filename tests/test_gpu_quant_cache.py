@@ -203,6 +203,34 @@ def test_every_way_of_sharing_rows_out(bits, H, G, lens, ctas):
             assert bool(((got[b, h] - ref).abs() <= output_bound(ref, mag, torch.bfloat16, e)).all()), (b, h)
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("ctas", [None, 5, 33])
+def test_more_lengths_than_a_warp_has_lanes(bits, per_head, ctas):
+    """A length per sequence or per head, more of them than 32, empty ones at both ends and in rows among them."""
+    H, G = 2, 3
+    lens = [0, 0] + [(37 * i) % 211 for i in range(40)] + [900, 0, 0, 0, 1, 640, 0]
+    B = len(lens)
+    cache, k, v = random_cache(B, H, max(lens), bits, 71, lens)
+    q = (torch.randn(B * H * G, 128, generator=torch.Generator().manual_seed(6)) * 2).to(torch.bfloat16)
+    attn = QuantAttentionGraph(H=B * H * G, H_kv=B * H, d=128, dtype=torch.bfloat16, device=DEV)
+    attn.n_group = 1 if per_head else H
+    if ctas is not None:
+        attn.ctas = ctas
+        attn.ws = torch.zeros(lib().skv_quant_workspace_bytes(B * H, G, 128, ctas), dtype=torch.uint8, device=DEV)
+    each = [[max(n - 3 * h, 0) if per_head else n for h in range(H)] for n in lens]
+    n_dev = torch.tensor([n for row in each for n in row] if per_head else lens, dtype=torch.int32, device=DEV)
+    out = attn(q.to(DEV), cache, 0, n_dev).clone()
+    assert torch.equal(attn(q.to(DEV), cache, 0, n_dev), out)
+    got = out.cpu().double().view(B, H, G, 128)
+    for b in range(B):
+        for h in range(H):
+            n, qh = each[b][h], q.view(B, H, G, 128)[b, h]
+            ref, mag = attention(qh, k[b, h, :n], v[b, h, :n], SCALE)
+            e = score_error(qh, k[b, h, :n], bits) if n else 0.0
+            assert bool(((got[b, h] - ref).abs() <= output_bound(ref, mag, torch.bfloat16, e)).all()), (b, h)
+
+
 def test_queries_that_alias_the_output_and_a_negative_softmax_scale():
     H, G, n = 2, 4, 300
     cache, k, v = random_cache(1, H, n, 8, 41)

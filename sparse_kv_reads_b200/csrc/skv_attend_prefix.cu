@@ -180,9 +180,11 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_proxy();
     }
-    if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
     pdl_wait();
     pdl_trigger();
+    // Only behind the wait: an allocation blocks without a limit, so a launch that has started early must not hold the columns
+    // that a launch ahead of it has still to ask for.
+    if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
     // Queries into the 128-byte swizzle, 16 bytes at a time; rows beyond the last are zero.  A negative softmax scale goes
     // into their sign: the running maximum is one of scaled scores.  All of a thread's loads are requested at once, and ahead
     // of the other tiles: behind them they took up to 14,000 cycles.

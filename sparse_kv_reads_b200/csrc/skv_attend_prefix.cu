@@ -376,8 +376,11 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
         }
         if (ok && turns > 0) ok = mbar_wait_warp(b_done + 8 * w, 0);
         if (!ok) s_fail = 1;
+        // Both slots' products have ended: the tiles' memory is free.  The fences stand on either side of the barrier, since a
+        // warp reads the other slot's sums below, whose end only that slot's warps have waited for.
+        tcgen05_before_sync();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         tcgen05_after_sync();
-        asm volatile("bar.sync 1, 256;" ::: "memory");    // both slots' products have ended: the tiles' memory is free
         const bool fold = both && n > 1;                  // the two slots have the same rows: a half of the columns each
         float *out = reinterpret_cast<float *>(smem + (fold ? 0 : w) * P_OUT) + r * PART_LD;
         const int row = row0 + (both ? 0 : w * PT) + r, b = (int)((unsigned)row / (unsigned)p.G), g = row - b * p.G;

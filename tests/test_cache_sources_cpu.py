@@ -20,3 +20,12 @@ def test_tensor_memory_is_asked_for_behind_the_wait_for_earlier_launches():
     that has still to allocate would never end."""
     body = kernel_body("skv_attend_prefix.cu", "prefix_mma_kernel")
     assert body.count("tmem_alloc(") == 1 and 0 <= body.index("pdl_wait();") < body.index("tmem_alloc(")
+
+
+def test_sums_of_the_other_slot_are_read_behind_a_fence_behind_the_barrier():
+    """A warp that folds the two slots reads sums whose products another warp has waited for: fence, barrier, fence."""
+    body = kernel_body("skv_attend_prefix.cu", "prefix_mma_kernel")
+    tail = body[body.index("b_done + 8 * w, 0"):]
+    steps = [tail.index(x) for x in ("tcgen05_before_sync();", "bar.sync 1, 256;")]
+    fence = tail.find("tcgen05_after_sync();", steps[1])
+    assert steps[0] < steps[1] < fence < tail.index("tmem_ld32(")

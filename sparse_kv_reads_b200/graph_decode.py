@@ -129,6 +129,7 @@ class GraphDecoder:
                                           var_factor=var_factor, var_min=var_min, arena=arena, layer=i)
                          for i in range(nl)]
         self.graph = None
+        self._captured = None                              # what the graph was captured for: (first, ragged)
         self.logits = None
         self.ragged = False                                # True once prepare() was given one length per sequence
         # the bundled bf16 model runs its element-wise decode ops as three fused launches per layer
@@ -186,8 +187,9 @@ class GraphDecoder:
         """Build the attention state from the first ``n`` cached positions (after the prompt).  ``n`` may be a
         list with one length per sequence: the batch then decodes sequences of different lengths (each head reads
         its own sequence's length and position from device memory), which lifts the reference's equal-length limit
-        (README.md:62); ``step`` then takes one position per sequence.  Lengths and positions count a shared prefix."""
-        self.first = getattr(self.cache, "first", 0)
+        (README.md:62); ``step`` then takes one position per sequence.  Lengths and positions count a shared prefix:
+        where its length has changed, a captured step no longer holds and is given up (``capture`` again)."""
+        self._set_first()
         if not isinstance(n, int):
             return self._prepare_ragged([int(x) for x in n])
         if self.mode != "cluster":
@@ -202,6 +204,13 @@ class GraphDecoder:
         if self.fused_insert:
             self.insert_all = AllLayerInsert(self.attn, [self._heads(k) for k in self.cache.k[:len(self.attn)]])
             self._insert_for_first_step(n)
+
+    def _set_first(self) -> None:
+        """Take over the position of the cache's first row.  A captured step has the shared prefix's length, its tensor
+        maps and the offset into the rotary tables in it: one captured for another length is given up."""
+        self.first = getattr(self.cache, "first", 0)
+        if self.graph is not None and self._captured != (self.first, self.ragged):
+            self.graph = None
 
     def _insert_for_first_step(self, n: int | None) -> None:
         """With the insert running at the end of each step for the next one, the first step's insert happens here:
@@ -270,7 +279,7 @@ class GraphDecoder:
         """Restore what ``state_dict`` saved, in place of ``prepare``: no fit runs.  The cache this decoder was
         built on must already hold the ``sd["n"]`` positions the state describes; call ``capture`` afterwards."""
         n = int(sd["n"])
-        self.first = getattr(self.cache, "first", 0)
+        self._set_first()
         self.cache.cur_len = n
         if self.mode != "cluster":
             return
@@ -606,6 +615,7 @@ class GraphDecoder:
             self.logits = self._body()
         self.launches_per_step = _lib.launches - before     # this library's kernels in one replay
         self.graph = g
+        self._captured = (self.first, self.ragged)
 
     @torch.no_grad()
     def step(self, token: torch.Tensor, pos) -> torch.Tensor:

@@ -272,3 +272,33 @@ def test_the_clustered_mode_refuses_the_new_caches_and_steps_are_checked():
     long = GraphDecoder(m, m.alloc_cache(600, bits=8), mode="dense")             # the rotary tables have 256 rows
     with pytest.raises(ValueError, match="outside the cache"):
         long.step(torch.zeros(1, 1, dtype=torch.long), 256)
+
+
+class Replayed:
+    """In place of a captured graph."""
+
+    def replay(self):
+        raise AssertionError("a step captured for another prefix was replayed")
+
+
+def test_a_captured_step_is_given_up_when_the_prefix_changes():
+    """The length of the prefix is part of a captured step: ``prepare`` and ``load_state_dict`` drop one captured for another."""
+    m = Qwen3Model(Qwen3Config(**TINY)).eval()
+    cache = m.alloc_prefix_cache(8, 4, 2)
+    cache.prefix.cur_len = 6
+    dec = GraphDecoder(m, cache, mode="dense")
+    dec.prepare(6)
+    graph = Replayed()
+    dec.graph, dec._captured = graph, (6, False)
+    dec.prepare(7)                                         # the same prefix: the step still holds
+    assert dec.graph is graph
+    cache.prefix.cur_len = 4
+    dec.prepare(5)
+    assert dec.graph is None
+    dec.graph, dec._captured = Replayed(), (6, False)
+    dec.load_state_dict({"n": 4, "layers": []})
+    assert dec.graph is None and dec.first == 4
+    plain = GraphDecoder(m, m.alloc_cache(8), mode="dense")
+    plain.graph, plain._captured = Replayed(), (0, False)
+    plain.prepare(3)
+    assert plain.graph is not None

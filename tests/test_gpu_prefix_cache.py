@@ -306,3 +306,34 @@ def test_a_prefix_cache_is_refused_by_the_clustered_mode():
     with pytest.raises(ValueError, match="plain cache"):
         GraphDecoder(model, model.alloc_prefix_cache(16, 16, 2), mode="cluster")
     assert isinstance(model.alloc_prefix_cache(16, 16, 2), PrefixKVCache)
+
+
+def test_a_captured_step_does_not_outlive_its_prefix():
+    """Another document after the capture: prepare() alone, then a new capture, both as a fresh decoder has it."""
+    model, T, B = tiny_model(), 4, 3
+    g = torch.Generator().manual_seed(6)
+    docs = [torch.randint(0, 1000, (1, n), generator=g).to(DEV) for n in (150, 60)]
+    tail = torch.randint(0, 1000, (B, T), generator=g).to(DEV)
+
+    def steps(dec, P):
+        return torch.stack([dec.step(tail[:, t:t + 1], P + t)[:, -1].float().clone() for t in range(T)], 1)
+
+    with torch.no_grad():
+        cache = model.alloc_prefix_cache(160, T, B)
+        model.prefill(docs[0], cache.prefix)
+        dec = GraphDecoder(model, cache, mode="dense")
+        dec.prepare(150)
+        cache.cur_len = 150
+        dec.capture()
+        first = steps(dec, 150)
+        model.prefill(docs[1], cache.prefix)
+        dec.prepare(60)
+        second = steps(dec, 60)
+        cache.cur_len = 60
+        dec.capture()
+        assert torch.equal(steps(dec, 60), second)
+        fresh = model.alloc_prefix_cache(160, T, B)
+        model.prefill(docs[1], fresh.prefix)
+        other = GraphDecoder(model, fresh, mode="dense")
+        other.prepare(60)
+        assert torch.equal(steps(other, 60), second) and not torch.equal(first, second)

@@ -244,11 +244,15 @@ class GraphDecoder:
             raise ValueError("one length per sequence is needed")
         if not self.fused_dense:
             raise ValueError("a variable-length batch needs the bundled bf16 model's fused layers")
-        dev = self.tok.device
-        self.ragged = True
         lengths = [n - self.first for n in lengths]        # own rows
         if min(lengths) < 0:
             raise ValueError(f"the sequences begin behind the prefix's {self.first} rows")
+        if self.ragged and self.mode != "cluster":         # a captured step reads these buffers: they stay where they are
+            self.pos.copy_(torch.tensor(lengths, dtype=torch.long))
+            self.n_dev.copy_(torch.tensor(lengths, dtype=torch.int32))
+            return
+        self.ragged, self.graph = True, None               # (new buffers: a step captured with others must not be replayed)
+        dev = self.tok.device
         self.pos = torch.tensor(lengths, dtype=torch.long, device=dev)
         self.n_dev = torch.tensor(lengths, dtype=torch.int32, device=dev)
         self.n_next = torch.zeros_like(self.n_dev)

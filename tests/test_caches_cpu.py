@@ -302,3 +302,25 @@ def test_a_captured_step_is_given_up_when_the_prefix_changes():
     plain.graph, plain._captured = Replayed(), (0, False)
     plain.prepare(3)
     assert plain.graph is not None
+
+
+@pytest.mark.parametrize("kind", ["quantised", "prefix"])
+def test_a_captured_ragged_step_keeps_its_buffers_or_is_given_up(kind):
+    """A captured step reads positions and lengths where they lay: a second batch of lengths goes to the same place, and the
+    first such batch, which needs new buffers, gives up a step captured for equal lengths."""
+    m = Qwen3Model(Qwen3Config(**TINY)).eval()
+    cache = m.alloc_cache(64, 2, bits=8) if kind == "quantised" else m.alloc_prefix_cache(8, 40, 2)
+    dec = GraphDecoder(m, cache, mode="dense")
+    dec.fused_dense = True                                 # (of the bf16 model on a GPU; nothing is launched here)
+    dec.prepare(5)
+    dec.graph, dec._captured = Replayed(), (0, False)
+    dec.prepare([5, 9])
+    assert dec.graph is None
+    where = dec.pos.data_ptr(), dec.n_dev.data_ptr()
+    graph = Replayed()
+    dec.graph, dec._captured = graph, (0, True)
+    dec.prepare([11, 2])
+    assert (dec.pos.data_ptr(), dec.n_dev.data_ptr()) == where and dec.graph is graph
+    assert dec.pos.tolist() == [11, 2] and dec.n_dev.tolist() == [11, 2]
+    with pytest.raises(ValueError, match="one length per sequence"):
+        dec.prepare([1])

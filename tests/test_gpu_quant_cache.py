@@ -491,3 +491,30 @@ def test_refused_on_the_gpu_too():
     x = torch.zeros(1, 2, 1, 128, dtype=torch.bfloat16, device=DEV, requires_grad=True)
     with pytest.raises(ValueError, match="no gradient"):
         cache.write(0, x, x, 0)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_a_second_ragged_batch_runs_through_the_captured_step(bits):
+    """New prompts in the same cache, prepare() with their lengths, no new capture: as a fresh decoder has it."""
+    model, T = tiny_model(), 4
+    g = torch.Generator().manual_seed(12)
+    batches = [[torch.randint(0, 1000, (n,), generator=g).to(DEV) for n in lens] for lens in ([40, 3, 77], [8, 90, 21])]
+    tail = torch.randint(0, 1000, (3, T), generator=g).to(DEV)
+
+    def run(dec, cache, prompts, capture):
+        lens = [len(p) for p in prompts]
+        with torch.no_grad():
+            model.prefill_ragged(prompts, cache, chunk=32)
+        dec.prepare(lens)
+        if capture:
+            dec.capture()
+        return torch.stack([dec.step(tail[:, t:t + 1], [n + t for n in lens])[:, -1].float().clone() for t in range(T)], 1)
+
+    cache = model.alloc_cache(128, 3, bits=bits)
+    dec = GraphDecoder(model, cache, mode="dense")
+    run(dec, cache, batches[0], True)
+    graph = dec.graph
+    got = run(dec, cache, batches[1], False)
+    assert dec.graph is graph
+    other = model.alloc_cache(128, 3, bits=bits)
+    assert torch.equal(got, run(GraphDecoder(model, other, mode="dense"), other, batches[1], True))

@@ -15,6 +15,7 @@ from sparse_kv_reads_b200 import (GraphDecoder, PrefixAttentionGraph, PrefixKVCa
 from sparse_kv_reads_b200 import _lib
 from sparse_kv_reads_b200.build import build
 from _caches import pack, quantise
+from _quant_bounds import attention_bound
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OK = 0x1000
@@ -324,3 +325,39 @@ def test_a_captured_ragged_step_keeps_its_buffers_or_is_given_up(kind):
     assert dec.pos.tolist() == [11, 2] and dec.n_dev.tolist() == [11, 2]
     with pytest.raises(ValueError, match="one length per sequence"):
         dec.prepare([1])
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n", [17, 300, 1000])
+def test_what_the_attentions_bounds_leave_outside(bits, n):
+    """Planted mistakes of the attention over quantised rows: each has a component outside the bound in some head."""
+    g = torch.Generator().manual_seed(n)
+    heads = []
+    for _ in range(4):
+        k = (torch.randn(n, 128, generator=g) + 0.7) * torch.randn(128, generator=g).abs()
+        (kc, ks), (vc, vs) = quantise(k, bits), quantise(torch.randn(n, 128, generator=g), bits)
+        heads.append((kc, ks, vc, vs, (torch.randn(2, 128, generator=g) * 2).to(torch.bfloat16)))
+
+    def found(change):
+        bad = []
+        for kc, ks, vc, vs, q in heads:
+            out, bound = attention_bound(q, kc, ks, vc, vs, bits, 128 ** -0.5)
+            wrong = attention_bound(q, *change(kc, ks, vc, vs), bits, 128 ** -0.5)[0]
+            bad.append(bool(((wrong - out).abs() > bound).any()))
+        return any(bad)
+
+    def exchanged(s, i, j):
+        s = s.clone()
+        s[:, [i, j]] = s[:, [j, i]]
+        return s
+
+    assert found(lambda kc, ks, vc, vs: (kc[:-16], ks[:-16], vc[:-16], vs[:-16]))                # the last tile lost
+    assert found(lambda kc, ks, vc, vs: (kc, ks, vc * (torch.arange(n) >= 16).unsqueeze(-1), vs))    # a tile's values lost
+    assert found(lambda kc, ks, vc, vs: (kc[n // 4:], ks[n // 4:], vc[n // 4:], vs[n // 4:]))      # a partial lost
+    assert found(lambda kc, ks, vc, vs: (kc, ks, vc, vs * 0))                                    # all zeros
+    assert found(lambda kc, ks, vc, vs: (kc, ks, vc, vs.float() * 1.1))
+    assert found(lambda kc, ks, vc, vs: (kc, ks.float() * 1.1, vc, vs))
+    if bits == 4:
+        assert found(lambda kc, ks, vc, vs: (kc, exchanged(ks, 0, 1), vc, vs))
+        assert found(lambda kc, ks, vc, vs: (kc, ks, vc, exchanged(vs, 2, 3)))
+    assert not found(lambda kc, ks, vc, vs: (kc, ks, vc, vs))

@@ -1,0 +1,65 @@
+"""Attention over quantised rows within bounds that are close enough to show a lost tile, a wrong scale or a lost partial (the
+CPU tests show what falls outside them), and at the ends of the numbers' range."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from sparse_kv_reads_b200 import QuantAttentionGraph, QuantKVCache
+from sparse_kv_reads_b200._lib import lib
+from _caches import pack, quantise
+from _helpers import DEV
+from _quant_bounds import attention_bound
+
+pytestmark = pytest.mark.gpu
+SCALE = 1.0 / math.sqrt(128)
+
+
+def normal_rows(B, H, L, seed, mean=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(B, H, L, 128, generator=g) + mean) * torch.randn(128, generator=g).abs()
+
+
+def device_cache(codes, bits, lens=None):
+    """``codes``: key codes, key scales, value codes, value scales; rows behind a sequence's length get NaN scales."""
+    kc, ks, vc, vs = codes
+    scale = torch.stack((ks, vs), -2).contiguous()
+    for b, n in enumerate(lens or []):
+        scale[b, :, n:] = float("nan")
+    return QuantKVCache.from_tensors([pack(kc, bits).to(DEV)], [pack(vc, bits).to(DEV)], [scale.to(DEV)], bits)
+
+
+def outside(got, q, codes, lens, bits, scale=SCALE):
+    """Sequences and heads with a component outside the bound."""
+    B, H = codes[0].shape[:2]
+    q, got, bad = q.view(B, H, -1, 128), got.cpu().double().view(B, H, -1, 128), []
+    for b, n in enumerate(lens):
+        for h in range(H):
+            out, bound = attention_bound(q[b, h], *(c[b, h, :n] for c in codes), bits, scale)
+            if not bool(((got[b, h] - out).abs() <= bound).all()):
+                bad.append((b, h, float(((got[b, h] - out).abs() / bound).max())))
+    return bad
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("H,G,lens", [(3, 1, [1]), (3, 2, [16]), (3, 4, [33]), (3, 8, [300]), (2, 3, [1000]), (8, 2, [700]),
+                                      (2, 4, [0, 1, 500, 333, 64, 0, 499]), (1, 8, [0] * 5 + [1] * 5 + [900]),
+                                      (8, 2, [37 * b % 301 for b in range(40)])])
+@pytest.mark.parametrize("ctas", [None, 1, 7, 64])
+def test_attention_within_close_bounds(bits, H, G, lens, ctas):
+    B, L = len(lens), max(lens)
+    codes = (*quantise(normal_rows(B, H, L, L, 0.7), bits), *quantise(normal_rows(B, H, L, L + 1), bits))
+    cache = device_cache(codes, bits, lens)
+    q = (torch.randn(B * H * G, 128, generator=torch.Generator().manual_seed(4)) * 2).to(torch.bfloat16)
+    attn = QuantAttentionGraph(H=B * H * G, H_kv=B * H, d=128, dtype=torch.bfloat16, device=DEV)
+    attn.n_group = H
+    if ctas is not None:
+        attn.ctas = ctas
+        attn.ws = torch.zeros(lib().skv_quant_workspace_bytes(B * H, G, 128, ctas), dtype=torch.uint8, device=DEV)
+    n_dev = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = attn(q.to(DEV), cache, 0, n_dev).clone()
+    assert torch.equal(attn(q.to(DEV), cache, 0, n_dev), out)
+    assert outside(out, q, codes, lens, bits) == []

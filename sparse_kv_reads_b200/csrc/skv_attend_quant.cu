@@ -200,10 +200,11 @@ struct WarpAttendQuant {
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // exponent of the largest component, kept where its inverse is a normal number too
+        // exponent of the largest component (Inf and NaN: none), kept where its inverse is a normal number too: a component in
+        // [2^127, 2^128) becomes one in [2, 4)
         int e = (int)(__float_as_uint(top) >> 23) - 127;
         if (!(top > 0.f) || e > 127) e = 0;
-        e = max(e, -120);
+        e = min(max(e, -120), 126);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
         float sum[GR];
 #pragma unroll

@@ -63,3 +63,31 @@ def test_attention_within_close_bounds(bits, H, G, lens, ctas):
     out = attn(q.to(DEV), cache, 0, n_dev).clone()
     assert torch.equal(attn(q.to(DEV), cache, 0, n_dev), out)
     assert outside(out, q, codes, lens, bits) == []
+
+
+def random_codes(H, n, bits, seed, most=None):
+    top = most or (127 if bits == 8 else 7)
+    return torch.randint(-top, top + 1, (1, H, n, 128), generator=torch.Generator().manual_seed(seed))
+
+
+def scales(H, n, bits, value):
+    return torch.full((1, H, n, 1 if bits == 8 else 4), value, dtype=torch.float32).to(torch.bfloat16)
+
+
+def run_alone(q, codes, bits, dtype=torch.bfloat16):
+    """All rows of a cache of one sequence."""
+    H, n = codes[0].shape[1:3]
+    attn = QuantAttentionGraph(H=q.shape[0], H_kv=H, d=128, dtype=dtype, device=DEV)
+    return attn(q.to(DEV).to(dtype), device_cache(codes, bits), 0, torch.tensor([n], dtype=torch.int32, device=DEV)).clone()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n", [40, 300])
+def test_queries_up_to_the_largest_number(bits, n):
+    """A few components in [2^127, 2^128), keys so small that the scores are ordinary."""
+    H, G = 2, 3
+    codes = (random_codes(H, n, bits, 1, 5), scales(H, n, bits, 2.0 ** -126), *quantise(normal_rows(1, H, n, 2), bits))
+    g = torch.Generator().manual_seed(n)
+    q = torch.randn(H * G, 128, generator=g) * 2.0 ** 110
+    q[:, 5::31] = (1 + 0.99 * torch.rand(H * G, 4, generator=g)) * 2.0 ** 127
+    assert outside(run_alone(q.to(torch.bfloat16), codes, bits), q.to(torch.bfloat16), codes, [n], bits) == []

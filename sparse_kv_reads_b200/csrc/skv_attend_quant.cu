@@ -6,7 +6,8 @@
 //     agree on it, so a lane takes a row's bytes 16 at a time and the queries are fetched in the matching order.  The
 //     offsets (1152 = 1024 + 128 in 8 bits) stay in the codes: the accumulators start at minus the offset times the sum of
 //     the query.  Queries are scaled by a power of two to a largest component in [1, 2), which half floats hold to 2^-25 of
-//     that.
+//     that (4 bits: 2^-21 in odd places, whose codes lie four bits higher).  Scores of up to 2^104 come out right whatever the
+//     sizes of queries and keys.
 //   O^T = V^T (P vs): component d of the values on M, keys on K.  A lane reads the same bytes of the value rows of its
 //     four keys and pairs them up by permutation.  The value's scale goes into the weights (per scale group in 4 bits).
 // A warp has a ring of tiles of its own in shared memory, filled by 16-byte asynchronous copies and laid out so that neither
@@ -205,6 +206,10 @@ struct WarpAttendQuant {
         int e = (int)(__float_as_uint(top) >> 23) - 127;
         if (!(top > 0.f) || e > 127) e = 0;
         e = min(max(e, -120), 126);
+        // The sums of codes (up to 2^15) meet the key's scale (up to 2^121, 2^125 in 4 bits) before the query's power of two.  Queries
+        // so small that the product could leave the numbers though the score does not are held 9 places lower: their half
+        // floats keep 2^-16 of the largest component (odd places of 4 bits: 2^-12).
+        if (e < -20) e += 9;
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
         float sum[GR];
 #pragma unroll
@@ -252,8 +257,8 @@ struct WarpAttendQuant {
                               __byte_perm(w0, F16_1024, 0x5352), __byte_perm(w1, F16_1024, 0x5352), qb[s][0], qb[s][1]);
             }
             const float k0 = bf16_low(r.s[0]), k1 = bf16_low(r.s[1]);
-            z[0] = (c[0] + c2[0]) * qsA * k0; z[1] = (c[1] + c2[1]) * qsB * k0;
-            z[2] = (c[2] + c2[2]) * qsA * k1; z[3] = (c[3] + c2[3]) * qsB * k1;
+            z[0] = (c[0] + c2[0]) * k0 * qsA; z[1] = (c[1] + c2[1]) * k0 * qsB;
+            z[2] = (c[2] + c2[2]) * k1 * qsA; z[3] = (c[3] + c2[3]) * k1 * qsB;
         } else {
             z[0] = z[1] = z[2] = z[3] = 0.f;
 #pragma unroll

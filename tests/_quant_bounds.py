@@ -16,7 +16,8 @@ def attention_bound(q, k_code, k_scale, v_code, v_scale, bits, scale):
     group is at most ``M``: 1,152 (8 bits: 1,024 + 128) times the sum of the queries' magnitudes, in 4 bits 1,032 times that of
     the even components and 1,152 / 16 times that of the odd ones, whose queries are a sixteenth.  A product of 16 terms rounds
     (or cuts) it twice to 2^-22 of its size: 16 times in 8 bits, 4 times per group in 4 bits.  A query is a half float of
-    at least 2^-25 (odd components of 4 bits: 2^-21) of the largest component, with 7 or 127 for the code.  The key's scale and
+    at least 2^-25 (odd components of 4 bits: 2^-21) of the largest component, with 7 or 127 for the code; 2^9 times that where
+    the largest is below 2^-20, since such queries are held nine places lower.  The key's scale and
     the softmax scale apply to all of it; scale, difference and exponential round the base-2 score to 2^-22 of its size.
     Weight times value scale is a half float: half a step is 2^-11 of it, or 2^-25 of the largest one of the component's group.
     Sums of n terms: 2^-24 of the sum of magnitudes each.  The output's own rounding: 2^-8 of it."""
@@ -35,7 +36,8 @@ def attention_bound(q, k_code, k_scale, v_code, v_scale, bits, scale):
     else:
         partial, times = 1032 * a[..., 0::2].sum(-1) + 72 * a[..., 1::2].sum(-1), 4
     top = a.amax((1, 2)).unsqueeze(-1)
-    group = partial * times * 2.0 ** -22 + size * most * top * 2.0 ** (-25 if bits == 8 else -21)     # [G, groups]
+    held = top * torch.where(top < 2.0 ** -20, 512.0, 1.0) * 2.0 ** (-25 if bits == 8 else -21)
+    group = partial * times * 2.0 ** -22 + size * most * held                                         # [G, groups]
     e = group @ ks.T.abs() * abs(scale) + 2 * (z.abs() * 1.45 + 2) * 2.0 ** -22                       # [G, n]
     e = e + e * e                                          # exp(e) - 1, for e well below 1
     e = e + (w * e).sum(-1, keepdim=True)                  # the quotient's denominator moves too

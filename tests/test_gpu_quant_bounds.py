@@ -91,3 +91,14 @@ def test_queries_up_to_the_largest_number(bits, n):
     q = torch.randn(H * G, 128, generator=g) * 2.0 ** 110
     q[:, 5::31] = (1 + 0.99 * torch.rand(H * G, 4, generator=g)) * 2.0 ** 127
     assert outside(run_alone(q.to(torch.bfloat16), codes, bits), q.to(torch.bfloat16), codes, [n], bits) == []
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("size", [2.0 ** e for e in (-126, -122, -110, -60, -30, -20, 0, 60, 100, 116, 120, 122)])
+def test_scores_of_queries_and_keys_at_opposite_ends(bits, size):
+    """Ordinary scores from queries of one end of the numbers and keys of the other."""
+    H, G, n = 2, 3, 300
+    key = 2.0 ** (-4 if bits == 8 else -2) / size
+    codes = (random_codes(H, n, bits, 3), scales(H, n, bits, key), *quantise(normal_rows(1, H, n, 4), bits))
+    q = (torch.randn(H * G, 128, generator=torch.Generator().manual_seed(5)) * size).to(torch.bfloat16)
+    assert outside(run_alone(q, codes, bits), q, codes, [n], bits) == []

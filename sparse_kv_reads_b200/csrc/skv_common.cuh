@@ -9,7 +9,8 @@
 
 namespace skv {
 
-constexpr float NEG_BIG = -1.0e30f;      // finite stand-in for -inf in running maxima (no NaN from inf - inf)
+// finite stand-in for -inf in running maxima (no NaN from inf - inf): the lowest number, so that no finite score lies below it
+constexpr float NEG_BIG = -3.402823466e38f;
 constexpr int HEAD_DIM = 128;            // the only head dimension the kernels are built for
 constexpr float LOG2E = 1.4426950408889634f;
 

@@ -102,3 +102,26 @@ def test_scores_of_queries_and_keys_at_opposite_ends(bits, size):
     codes = (random_codes(H, n, bits, 3), scales(H, n, bits, key), *quantise(normal_rows(1, H, n, 4), bits))
     q = (torch.randn(H * G, 128, generator=torch.Generator().manual_seed(5)) * size).to(torch.bfloat16)
     assert outside(run_alone(q, codes, bits), q, codes, [n], bits) == []
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("size", [2.0 ** 60, 2.0 ** 116, 2.0 ** 120, 2.0 ** 127])
+def test_scores_far_beyond_ordinary_ones(bits, dtype, sign, size):
+    """Finite scores of up to 2^126, all positive or all negative: the largest one takes all."""
+    H, G, n = 2, 2, 200
+    kc = torch.zeros(1, H, n, 128, dtype=torch.int64)
+    top = 120 if bits == 8 else 6
+    kc[..., 7] = torch.tensor([top if sign > 0 else -top] * n)
+    best = [3, 177]
+    for h, j in enumerate(best):                           # one step above the others
+        kc[0, h, j, 7] += 1
+    key = 2.0 ** 50 if size < 2.0 ** 100 else 2.0 ** -7 if bits == 8 else 2.0 ** -3
+    codes = (kc, scales(H, n, bits, key), *quantise(normal_rows(1, H, n, 6), bits))
+    q = torch.zeros(H * G, 128)
+    q[:, 7] = size
+    got = run_alone(q, codes, bits, dtype).cpu().double().view(H, G, 128)
+    value = codes[2].double() * codes[3].double().repeat_interleave(128 if bits == 8 else 32, -1)
+    for h, j in enumerate(best):
+        assert torch.equal(got[h], value[0, h, j].to(dtype).double().expand(G, -1)), h

@@ -337,3 +337,26 @@ def test_a_captured_step_does_not_outlive_its_prefix():
         other = GraphDecoder(model, fresh, mode="dense")
         other.prepare(60)
         assert torch.equal(steps(other, 60), second) and not torch.equal(first, second)
+
+
+def run_plain(q, kp, vp, k, v, B, Hk, G, dtype=torch.bfloat16):
+    attn = PrefixAttentionGraph(B=B, H=Hk * G, H_kv=Hk, d=128, dtype=dtype, device=DEV)
+    n = torch.tensor([k.shape[1]], dtype=torch.int32, device=DEV)
+    return attn(*(t.to(DEV) for t in (q, kp, vp, k, v)), n).clone()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,P,n", [(2, 100, 20), (60, 5000, 20), (130, 5000, 7)])
+@pytest.mark.parametrize("size", [2.0 ** 105, -2.0 ** 105])
+def test_scores_far_beyond_ordinary_ones(dtype, B, P, n, size):
+    """Finite scores of 2^118, all positive or all negative: the largest one takes all, be it the prefix's or an own one."""
+    Hk, G = 1, 2
+    q, kp, vp, k, v = inputs(B, Hk, G, P, n, [n] * B, 3, dtype)
+    q[:], kp[:], k[:] = 0, 0, 0
+    q[:, 9], kp[..., 9], k[..., 9] = size, (65536.0 if size > 0 else 66048.0), (65536.0 if size > 0 else 66048.0)
+    best = 66048.0 if size > 0 else 65536.0
+    kp[0, 77, 9] = best                                    # even sequences: the prefix's row; odd ones: an own row beyond it
+    k[1::2, n // 2, 9] = best * (2 if size > 0 else 0.5)
+    got = run_plain(q, kp, vp, k, v, B, Hk, G, dtype).cpu().view(B, G, 128)
+    for b in range(B):
+        assert torch.equal(got[b], (v[b, n // 2] if b % 2 else vp[0, 77]).expand(G, -1)), b

@@ -643,7 +643,8 @@ static bool prefix_map(CUtensorMap *map, const void *x, int h_kv, int prefix, in
 
 static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
     const int heads = p.batch * p.h_kv, tiles = (p.prefix + PT - 1) / PT;
-    const bool list = (int64_t)heads * p.prefix * 2 * HEAD_DIM * 2 <= LIST_BYTES;
+    // (a scale of zero by the list as well: the tiles mark keys beyond the prefix by scores of -inf, which times zero is no number)
+    const bool list = (int64_t)heads * p.prefix * 2 * HEAD_DIM * 2 <= LIST_BYTES || p.scale_log2 == 0.f;
     int ps = list ? 0 : prefix_splits_of(p.batch, p.h_kv, p.G);
     if (ps > (tiles + 2) / 3) ps = (tiles + 2) / 3;
     if (ps > p.splits - 1) ps = p.splits - 1;

@@ -360,3 +360,17 @@ def test_scores_far_beyond_ordinary_ones(dtype, B, P, n, size):
     got = run_plain(q, kp, vp, k, v, B, Hk, G, dtype).cpu().view(B, G, 128)
     for b in range(B):
         assert torch.equal(got[b], (v[b, n // 2] if b % 2 else vp[0, 77]).expand(G, -1)), b
+
+
+@pytest.mark.parametrize("B,G,P", [(3, 2, 100), (60, 4, 5000), (130, 4, 1000), (130, 4, 1024)])
+def test_a_softmax_scale_of_zero_gives_the_mean(B, G, P):
+    """By the list and in the range of the tiles, whole and ragged: every row counts alike."""
+    Hk, n = 1, 9
+    q, kp, vp, k, v = inputs(B, Hk, G, P, n, [n] * B, 4)
+    attn = PrefixAttentionGraph(B=B, H=G, H_kv=Hk, d=128, dtype=torch.bfloat16, device=DEV)
+    attn._scale = 0.0
+    got = attn(*(t.to(DEV) for t in (q, kp, vp, k, v)), torch.tensor([n], dtype=torch.int32, device=DEV)).cpu().double()
+    for b in range(B):
+        rows = torch.cat((vp[0], v[b])).double()
+        ref, mag = rows.mean(0), rows.abs().mean(0)
+        assert bool(((got.view(B, G, 128)[b] - ref).abs() <= output_bound(ref, mag, torch.bfloat16)).all()), b

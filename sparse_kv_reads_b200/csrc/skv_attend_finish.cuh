@@ -12,6 +12,11 @@ constexpr int PART_LD = 132;               // floats per partial row: 128 sums, 
 template <typename Params>
 __device__ __forceinline__ void stamp(const Params &, int) {}
 
+// A row's output: zero where no key had a weight.  A sum of weights that is no number counts as none, unless the kernel overloads
+// it for its own parameter type.
+template <typename Params>
+__device__ __forceinline__ float quotient(const Params &, float num, float den) { return den > 0.f ? num / den : 0.f; }
+
 // `p` needs: out, part [slots, G, 132], ticket [heads], G.  The head's s_eff partials lie in the slots from slot0 on; this
 // CTA's is number `split` of them.
 // blockDim.x is 128: one thread per output column.
@@ -36,7 +41,7 @@ __device__ __forceinline__ void publish_head(const Params &p, const float *red, 
             nm += f * r[tid];
         }
         if (s_eff == 1) {
-            store_out(out + ((int64_t)head * G + g) * HEAD_DIM + tid, dn > 0.f ? nm / dn : 0.f);
+            store_out(out + ((int64_t)head * G + g) * HEAD_DIM + tid, quotient(p, nm, dn));
         } else {
             __stcg(pa + g * PART_LD + tid, nm);
             if (tid == 0) __stcg(reinterpret_cast<float2 *>(pa + g * PART_LD + HEAD_DIM), make_float2(M, dn));
@@ -116,7 +121,7 @@ __device__ __forceinline__ void merge_head(const Params &p, int head, int s_eff,
                             num += s_sum[qi * wpg + w][tid];
                             den += s_sum[qi * wpg + w][HEAD_DIM];
                         }
-                        store_out(out + ((int64_t)head * G + g0 + gb + qi) * HEAD_DIM + tid, den > 0.f ? num / den : 0.f);
+                        store_out(out + ((int64_t)head * G + g0 + gb + qi) * HEAD_DIM + tid, quotient(p, num, den));
                     }
                 __syncthreads();
             }

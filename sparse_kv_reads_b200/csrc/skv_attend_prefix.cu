@@ -29,6 +29,9 @@ struct PrefixParams {
     float scale_log2;
 };
 
+// A key that is no number leaves its head without one, as the definition has it.
+__device__ __forceinline__ float quotient(const PrefixParams &, float num, float den) { return den == 0.f ? 0.f : num / den; }
+
 // Own rows of (sequence, KV head) `head`: its length, within the rows the cache has (a longer one is recorded).
 __device__ __forceinline__ int own_rows(const PrefixParams &p, int head) {
     const int n = positions_of(p.n_dev, p.n_group, head);
@@ -558,7 +561,7 @@ __global__ void __launch_bounds__(128, STAGES == 1 ? 4 : 3) prefix_own_kernel(co
                 dn += f * r[129];
                 nm += f * r[tid];
             }
-            store_out(static_cast<__nv_bfloat16 *>(p.out) + ((int64_t)head * G + g) * HEAD_DIM + tid, dn > 0.f ? nm / dn : 0.f);
+            store_out(static_cast<__nv_bfloat16 *>(p.out) + ((int64_t)head * G + g) * HEAD_DIM + tid, quotient(p, nm, dn));
         }
         return;
     }

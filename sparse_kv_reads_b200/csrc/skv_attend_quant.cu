@@ -42,6 +42,9 @@ struct AttendQuantParams {
     float scale_log2;
 };
 
+// A key without a number (NaN scale) leaves its head without one, as the definition has it.
+__device__ __forceinline__ float quotient(const AttendQuantParams &, float num, float den) { return den == 0.f ? 0.f : num / den; }
+
 template <typename T, int BITS, int GP>
 __global__ void __launch_bounds__(128) attend_quant_simple_kernel(const AttendQuantParams p) {
     using Q = Quant<BITS>;
@@ -515,10 +518,9 @@ __device__ __forceinline__ void merge_few(const Params &p, int row, int head, in
         nm.x = fmaf(fi, a[i].x, nm.x); nm.y = fmaf(fi, a[i].y, nm.y);
         nm.z = fmaf(fi, a[i].z, nm.z); nm.w = fmaf(fi, a[i].w, nm.w);
     }
-    const bool any = den > 0.f;
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + ((int64_t)head * p.G + row) * HEAD_DIM + lane * 4;
-    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(any ? nm.x / den : 0.f, any ? nm.y / den : 0.f),
-                                                 pack_bf16(any ? nm.z / den : 0.f, any ? nm.w / den : 0.f));
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(quotient(p, nm.x, den), quotient(p, nm.y, den)),
+                                                 pack_bf16(quotient(p, nm.z, den), quotient(p, nm.w, den)));
 }
 
 constexpr int QUANT_CTAS_PER_SM = 2;

@@ -374,3 +374,16 @@ def test_a_softmax_scale_of_zero_gives_the_mean(B, G, P):
         rows = torch.cat((vp[0], v[b])).double()
         ref, mag = rows.mean(0), rows.abs().mean(0)
         assert bool(((got.view(B, G, 128)[b] - ref).abs() <= output_bound(ref, mag, torch.bfloat16)).all()), b
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,P,n", [(2, 100, 20), (60, 5000, 20), (60, 5000, 300), (130, 5000, 7)])
+def test_a_key_that_is_no_number_leaves_no_number(dtype, B, P, n):
+    """By the list and by the tiles: NaN in a prefix key spoils its KV head for all, in an own key its sequence's head."""
+    Hk, G = 2, 2
+    q, kp, vp, k, v = inputs(B, Hk, G, P, n, [n] * B, 3, dtype)
+    kp[1, P - 2, 5] = float("nan")
+    k[1 * Hk + 0, n - 1, 9] = float("nan")
+    got = run_plain(q, kp, vp, k, v, B, Hk, G, dtype).view(B, Hk, G, 128).isnan()
+    assert bool(got[:, 1].all()) and bool(got[1, 0].all())
+    assert not bool(got[0, 0].any()) and not bool(got[2:, 0].any())

@@ -125,3 +125,17 @@ def test_scores_far_beyond_ordinary_ones(bits, dtype, sign, size):
     value = codes[2].double() * codes[3].double().repeat_interleave(128 if bits == 8 else 32, -1)
     for h, j in enumerate(best):
         assert torch.equal(got[h], value[0, h, j].to(dtype).double().expand(G, -1)), h
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [20, 300, 3000])
+def test_a_key_without_a_number_leaves_no_number_and_a_value_its_own_group(bits, dtype, n):
+    """NaN scales among the rows: of a key, and the head has no answer; of a value, and its components have none."""
+    H, G, size = 4, 2, 128 if bits == 8 else 32
+    kc, ks, vc, vs = (*quantise(normal_rows(1, H, n, 7, 0.7), bits), *quantise(normal_rows(1, H, n, 8), bits))
+    ks[0, 1, n // 2, -1] = vs[0, 3, n - 1, 0] = float("nan")
+    q = (torch.randn(H * G, 128, generator=torch.Generator().manual_seed(1)) * 2).to(torch.bfloat16)
+    got = run_alone(q, (kc, ks, vc, vs), bits, dtype).view(H, G, 128).isnan()
+    assert bool(got[1].all()) and not bool(got[0].any()) and not bool(got[2].any())
+    assert bool(got[3, :, :size].all()) and not bool(got[3, :, size:].any())

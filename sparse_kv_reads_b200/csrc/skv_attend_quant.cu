@@ -15,10 +15,11 @@
 // against 92 us for 64 heads of 32,768 8-bit rows, 85 against 75 us in 4 bits.)
 // What bounds it: 8 bits, the memory (64 heads of 32,768 rows: 83 us at the measured copy rate); 4 bits, the instructions
 // that turn two codes a byte into fragments (322 per 16 rows; the integer pipe is 54 % busy, the memory 61 %).
-// Two running references per head, in base 2: m for the sum of weights (largest score) and r for the accumulators (largest
-// score + log2 of the value's scale), so that the half floats 2^(z - r) vs keep their precision whatever the scales.  A
-// reference is only raised when something passes it by 8: products up to 256 cost a half float nothing, and most tiles
-// then need no shuffles.  A weight is rounded to 11 bits; sums and accumulators are float32.
+// Running references per head, in base 2: m for the sum of weights (largest score) and, for each scale group of the values, r for
+// the group's accumulators (largest score + log2 of the value's scale), so that the half floats 2^(z - r) vs keep their
+// precision whatever the scales of rows and groups (of weights down to 2^-126 of the head's largest).  m is only raised when
+// a score passes it by 8, r when a half float passes 2^15 (to 2^4 then), so that most tiles need no shuffles.
+// A weight is rounded to 11 bits; sums and accumulators are float32.
 // float32 queries: half a warp per row, float32 arithmetic on the CUDA cores.
 #include <cuda_fp16.h>
 
@@ -138,6 +139,11 @@ __device__ __forceinline__ uint32_t hfma(uint32_t x, float mul, float add) {
     const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&x), __float2half2_rn(mul), __float2half2_rn(add));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
+// the larger magnitudes of two pairs (NaN where both have none)
+__device__ __forceinline__ uint32_t hmax(uint32_t x, uint32_t y) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2 *>(&x), __habs2(*reinterpret_cast<const __half2 *>(&y)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
 __device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -183,7 +189,7 @@ struct WarpAttendQuant {
     float acc[8][4];                   // O^T: 8-bit tile j: components 16 g + 2 j and the next; 4-bit tile (group, i): 32 group
                                        // + 4 g + 2 i and the next
     float mA, mB, lA, lB;              // reference of the weights / partial sum of heads 2t, 2t + 1
-    float rA, rB, fA, fB;              // reference of the accumulators, and 2^(m - r)
+    float rA[GR], rB[GR], fA[GR], fB[GR];                    // reference of each scale group's accumulators, and 2^(m - r)
     float qsA, qsB;                    // score scale of the two heads, with the query's power of two
     int g, t;
 
@@ -245,8 +251,9 @@ struct WarpAttendQuant {
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
         mA = mB = NEG_BIG;
-        rA = rB = NEG_BIG;
-        lA = lB = fA = fB = 0.f;
+#pragma unroll
+        for (int i = 0; i < GR; ++i) { rA[i] = rB[i] = NEG_BIG; fA[i] = fB[i] = 0.f; }
+        lA = lB = 0.f;
     }
 
     // scores of keys g, g + 8 for heads 2t, 2t + 1: z = (A, g), (B, g), (A, g + 8), (B, g + 8), in base 2
@@ -302,6 +309,35 @@ struct WarpAttendQuant {
         b = hsub(__byte_perm(p, F16_1024, 0x5352), 1152.f);
     }
 
+    // Raise the accumulators' references to what these positions need; z: their scores, in base 2.
+    template <int U>
+    __device__ __forceinline__ void raise(const RawTile<BITS> (&r)[U], const float (&z)[U][4]) {
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            float yA = NEG_BIG, yB = NEG_BIG;              // largest score + log2 of the value's scale
+#pragma unroll
+            for (int u = 0; u < U; ++u) {                  // (-inf for values of zero: they never raise r)
+                const float v0 = log2_scale(fabsf(value_scale(r[u], 0, gr))), v1 = log2_scale(fabsf(value_scale(r[u], 1, gr)));
+                yA = fmaxf(yA, fmaxf(z[u][0] + v0, z[u][2] + v1)); yB = fmaxf(yB, fmaxf(z[u][1] + v0, z[u][3] + v1));
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                yA = fmaxf(yA, __shfl_xor_sync(0xffffffffu, yA, o));
+                yB = fmaxf(yB, __shfl_xor_sync(0xffffffffu, yB, o));
+            }
+            // (weights of 16 now; r no further below m than a float's exponent reaches with a weight of 2^8)
+            const float sA = fmaxf(fmaxf(rA[gr], yA - 4.f), mA - 118.f), sB = fmaxf(fmaxf(rB[gr], yB - 4.f), mB - 118.f);
+            const float alA = fast_exp2(rA[gr] - sA), alB = fast_exp2(rB[gr] - sB);
+            rA[gr] = sA; rB[gr] = sB;
+            fA[gr] = fast_exp2(mA - sA); fB[gr] = fast_exp2(mB - sB);
+#pragma unroll
+            for (int j = gr * (8 / GR); j < (gr + 1) * (8 / GR); ++j) {
+                acc[j][0] *= alA; acc[j][1] *= alB;
+                acc[j][2] *= alA; acc[j][3] *= alB;
+            }
+        }
+    }
+
     // U blocks of 16 positions, `left` positions cached (16 U or more: all)
     template <int U>
     __device__ __forceinline__ void consume(const RawTile<BITS> (&r)[U], float (&z)[U][4], int left) {
@@ -312,57 +348,58 @@ struct WarpAttendQuant {
                 if (g + 8 + 16 * u >= left) z[u][2] = z[u][3] = NEG_BIG;
             }
         }
-        float tA = NEG_BIG, tB = NEG_BIG, yA = NEG_BIG, yB = NEG_BIG;
+        float tA = NEG_BIG, tB = NEG_BIG;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            float v0 = 0.f, v1 = 0.f;                      // largest value scale of the lane's two keys
-#pragma unroll
-            for (int gr = 0; gr < GR; ++gr) {
-                v0 = fmaxf(v0, value_scale(r[u], 0, gr));
-                v1 = fmaxf(v1, value_scale(r[u], 1, gr));
-            }
-            v0 = log2_scale(v0); v1 = log2_scale(v1);      // (-inf for values of zero: they never raise r)
             tA = fmaxf(tA, fmaxf(z[u][0], z[u][2])); tB = fmaxf(tB, fmaxf(z[u][1], z[u][3]));
-            yA = fmaxf(yA, fmaxf(z[u][0] + v0, z[u][2] + v1)); yB = fmaxf(yB, fmaxf(z[u][1] + v0, z[u][3] + v1));
         }
-        if (__any_sync(0xffffffffu, fmaxf(tA - mA, yA - rA) > 8.f || fmaxf(tB - mB, yB - rB) > 8.f)) {
+        bool up = __any_sync(0xffffffffu, fmaxf(tA - mA, tB - mB) > 8.f);
+        if (up) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 tA = fmaxf(tA, __shfl_xor_sync(0xffffffffu, tA, o)); tB = fmaxf(tB, __shfl_xor_sync(0xffffffffu, tB, o));
-                yA = fmaxf(yA, __shfl_xor_sync(0xffffffffu, yA, o)); yB = fmaxf(yB, __shfl_xor_sync(0xffffffffu, yB, o));
             }
             const float nA = fmaxf(mA, tA), nB = fmaxf(mB, tB);
             lA *= fast_exp2(mA - nA); lB *= fast_exp2(mB - nB);
             mA = nA; mB = nB;
-            // (r no further below m than a float's exponent reaches)
-            const float sA = fmaxf(fmaxf(rA, yA), mA - 120.f), sB = fmaxf(fmaxf(rB, yB), mB - 120.f);
-            const float alA = fast_exp2(rA - sA), alB = fast_exp2(rB - sB);
-            rA = sA; rB = sB;
-            fA = fast_exp2(mA - rA); fB = fast_exp2(mB - rB);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                acc[j][0] *= alA; acc[j][1] *= alB;
-                acc[j][2] *= alA; acc[j][3] *= alB;
-            }
         }
+        float w[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            z[u][0] = fast_exp2(z[u][0] - mA); z[u][1] = fast_exp2(z[u][1] - mB);
-            z[u][2] = fast_exp2(z[u][2] - mA); z[u][3] = fast_exp2(z[u][3] - mB);
+            w[u][0] = fast_exp2(z[u][0] - mA); w[u][1] = fast_exp2(z[u][1] - mB);
+            w[u][2] = fast_exp2(z[u][2] - mA); w[u][3] = fast_exp2(z[u][3] - mB);
             if (left < 16 * U) {
-                if (g + 16 * u >= left) z[u][0] = z[u][1] = 0.f;
-                if (g + 8 + 16 * u >= left) z[u][2] = z[u][3] = 0.f;
+                if (g + 16 * u >= left) w[u][0] = w[u][1] = 0.f;
+                if (g + 8 + 16 * u >= left) w[u][2] = w[u][3] = 0.f;
             }
-            lA += z[u][0] + z[u][2]; lB += z[u][1] + z[u][3];
-            z[u][0] *= fA; z[u][1] *= fB; z[u][2] *= fA; z[u][3] *= fB;
+            lA += w[u][0] + w[u][2]; lB += w[u][1] + w[u][3];
+        }
+        // Weights times value scales as half floats; again with raised references where one of them is beyond 2^15.
+        uint32_t pw[U][GR][2];
+        auto weigh = [&]() {
+            uint32_t top = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) {
+                    const float2 f = make_float2(fA[gr], fB[gr]);
+                    const float2 x = mul2(make_float2(w[u][0], w[u][1]), f), y = mul2(make_float2(w[u][2], w[u][3]), f);
+                    const float s0 = value_scale(r[u], 0, gr), s1 = value_scale(r[u], 1, gr);
+                    pw[u][gr][0] = pack_f16(x.x * s0, x.y * s0);
+                    pw[u][gr][1] = pack_f16(y.x * s1, y.y * s1);
+                    top = hmax(hmax(top, pw[u][gr][0]), pw[u][gr][1]);
+                }
+            return ((top + 0x07ff07ffu) & 0x80008000u) != 0;
+        };
+        if (__any_sync(0xffffffffu, weigh() || up)) {
+            raise(r, z);
+            weigh();
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int gr = 0; gr < GR; ++gr) {
-                const float w0 = value_scale(r[u], 0, gr), w1 = value_scale(r[u], 1, gr);
-                const uint32_t b0 = movmatrix_trans(pack_f16(z[u][0] * w0, z[u][1] * w0));
-                const uint32_t b1 = movmatrix_trans(pack_f16(z[u][2] * w1, z[u][3] * w1));
+                const uint32_t b0 = movmatrix_trans(pw[u][gr][0]), b1 = movmatrix_trans(pw[u][gr][1]);
                 if constexpr (BITS == 8) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -400,10 +437,10 @@ struct WarpAttendQuant {
             if (head >= G) continue;
             float *o = red + (warp * G + head) * 132;
             // back to weights relative to m, in two steps: values near the largest numbers have 2^(r - m) beyond them
-            const float up = fast_exp2(0.5f * (which ? rB - mB : rA - mA));
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int d = BITS == 8 ? 16 * g + 2 * j : 32 * (j >> 1) + 4 * g + 2 * (j & 1);
+                const int d = BITS == 8 ? 16 * g + 2 * j : 32 * (j >> 1) + 4 * g + 2 * (j & 1), gr = j / (8 / GR);
+                const float up = fast_exp2(0.5f * (which ? rB[gr] - mB : rA[gr] - mA));
                 *reinterpret_cast<float2 *>(o + d) = make_float2(acc[j][which] * up * up, acc[j][2 + which] * up * up);
             }
             if (g == 0) { o[128] = which ? mB : mA; o[129] = which ? lB : lA; }

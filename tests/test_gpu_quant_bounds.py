@@ -139,3 +139,20 @@ def test_a_key_without_a_number_leaves_no_number_and_a_value_its_own_group(bits,
     got = run_alone(q, (kc, ks, vc, vs), bits, dtype).view(H, G, 128).isnan()
     assert bool(got[1].all()) and not bool(got[0].any()) and not bool(got[2].any())
     assert bool(got[3, :, :size].all()) and not bool(got[3, :, size:].any())
+
+
+@pytest.mark.parametrize("apart", [0, 6, 12, 16, 20, 24, 40, 100])
+@pytest.mark.parametrize("n", [16, 300, 1000])
+def test_value_groups_of_very_different_sizes(apart, n):
+    """The four value scales of a 4-bit row lie far apart, and not in the same order in every row or head."""
+    H, G = 3, 3
+    kc, ks, vc, vs = (*quantise(normal_rows(1, H, n, 7, 0.7), 4), *quantise(normal_rows(1, H, n, 8), 4))
+    down = torch.zeros(1, H, n, 4)
+    down[:, 0, :, 1:] = torch.tensor([apart / 3, apart * 2 / 3, apart])                 # the same order everywhere
+    down[:, 1, :, 2] = apart                                                            # one small group
+    g = torch.Generator().manual_seed(n)
+    down[:, 2] = torch.randint(0, 2, (n, 4), generator=g) * apart                       # by row
+    vs = (vs.float() * torch.exp2(-down.round())).to(torch.bfloat16)
+    codes = (kc, ks, vc, vs)
+    q = (torch.randn(H * G, 128, generator=g) * 2).to(torch.bfloat16)
+    assert outside(run_alone(q, codes, 4), q, codes, [n], 4) == []

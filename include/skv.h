@@ -505,6 +505,8 @@ typedef struct skv_prefix {
  * A row without any key gets zeros. */
 int skv_prefix_splits(int batch, int h_kv, int G, int dtype);
 int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d, int splits);
+/* How many kernels such a call launches (1 or 2: bf16 prefixes beyond a size have a launch of their own), or an SKV_E_* code. */
+int skv_prefix_launches(const skv_prefix *c, int splits, float scale);
 int skv_attend_prefix(const skv_prefix *c, const void *q, const int32_t *n_dev, void *out, void *workspace, int splits,
                       int32_t *status, float scale, void *stream);
 

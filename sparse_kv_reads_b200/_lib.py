@@ -23,7 +23,7 @@ EXPORTS = ("skv_version", "skv_error_string", "skv_last_cuda_error", "skv_attend
            "skv_add_rmsnorm", "skv_qk_rope_cache", "skv_silu_mul", "skv_gemv", "skv_gemv_attended", "skv_gemv_supported", "skv_gemv_tp", "skv_comm_bytes", "skv_comm_alloc",
            "skv_comm_export", "skv_comm_open", "skv_comm_close", "skv_comm_free", "skv_comm_view", "skv_comm_tick", "skv_comm_push", "skv_comm_reduce", "skv_comm_status",
            "skv_quant_write", "skv_quant_read", "skv_qk_rope_quant", "skv_quant_ctas", "skv_quant_workspace_bytes", "skv_attend_quant", "skv_prefix_splits",
-           "skv_prefix_workspace_bytes", "skv_attend_prefix")
+           "skv_prefix_workspace_bytes", "skv_prefix_launches", "skv_attend_prefix")
 
 
 class SkvError(RuntimeError):
@@ -192,6 +192,8 @@ def _declare(lib) -> None:
     lib.skv_prefix_splits.argtypes = [i32, i32, i32, i32]
     lib.skv_prefix_workspace_bytes.restype = i64
     lib.skv_prefix_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
+    lib.skv_prefix_launches.restype = i32
+    lib.skv_prefix_launches.argtypes = [C.POINTER(SkvPrefix), i32, f32]
     lib.skv_attend_prefix.restype = i32
     lib.skv_attend_prefix.argtypes = [C.POINTER(SkvPrefix), vp, vp, vp, vp, i32, vp, f32, vp]
     lib.skv_rebin.restype = i32
@@ -212,7 +214,8 @@ def lib():
 
 
 # entry points that launch exactly one kernel each: counted, so that a caller can tell how many of the library's
-# kernels a captured decode step holds (GraphDecoder.launches_per_step); skv_attend_prefix launches one or two and counts one
+# kernels a captured decode step holds (GraphDecoder.launches_per_step); the second launch of skv_attend_prefix is added by its
+# caller, which knows of it once per layout
 _ONE_LAUNCH = {"skv_insert", "skv_select", "skv_attend", "skv_attend_weighted", "skv_attend_labels", "skv_step", "skv_gemv", "skv_gemv_tp", "skv_gemv_attended",
                "skv_add_rmsnorm", "skv_qk_rope_cache", "skv_silu_mul", "skv_comm_push", "skv_comm_reduce", "skv_comm_tick",
                "skv_quant_write", "skv_quant_read", "skv_qk_rope_quant", "skv_attend_quant", "skv_attend_prefix"}

@@ -644,17 +644,24 @@ static bool prefix_map(CUtensorMap *map, const void *x, int h_kv, int prefix, in
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
+// CTAs per KV head and 256 query rows of the prefix's own launch, with its maps; 0: the second launch reads the prefix as well.
+static int prefix_tile_ctas(const PrefixParams &p, CUtensorMap *kmap, CUtensorMap *vmap) {
     const int heads = p.batch * p.h_kv, tiles = (p.prefix + PT - 1) / PT;
     // (a scale of zero by the list as well: the tiles mark keys beyond the prefix by scores of -inf, which times zero is no number)
     const bool list = (int64_t)heads * p.prefix * 2 * HEAD_DIM * 2 <= LIST_BYTES || p.scale_log2 == 0.f;
     int ps = list ? 0 : prefix_splits_of(p.batch, p.h_kv, p.G);
     if (ps > (tiles + 2) / 3) ps = (tiles + 2) / 3;
     if (ps > p.splits - 1) ps = p.splits - 1;
-    CUtensorMap kmap, vmap;
-    if (ps > 0 && (!prefix_map(&kmap, p.kp, p.h_kv, p.prefix, p.kph, p.kpr) ||
-                   !prefix_map(&vmap, p.vp, p.h_kv, p.prefix, p.vph, p.vpr)))
+    if (ps > 0 && (!prefix_map(kmap, p.kp, p.h_kv, p.prefix, p.kph, p.kpr) ||
+                   !prefix_map(vmap, p.vp, p.h_kv, p.prefix, p.vph, p.vpr)))
         ps = 0;                            // (strides that no map can have)
+    return ps;
+}
+
+static int launch_prefix_mma(PrefixParams p, cudaStream_t st) {
+    const int heads = p.batch * p.h_kv;
+    CUtensorMap kmap, vmap;
+    const int ps = prefix_tile_ctas(p, &kmap, &vmap);
     int own = skv_attend_splits(heads);
     if (own > p.splits - ps) own = p.splits - ps;
     p.prefix_splits = ps;
@@ -696,9 +703,9 @@ extern "C" int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d,
     return skv_attend_workspace_bytes(batch * h_kv, G, d, splits);
 }
 
-extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32_t *n_dev, void *out, void *workspace, int splits,
-                                 int32_t *status, float scale, void *stream) {
-    if (!c || !q || !n_dev || !out || !workspace) return SKV_E_NULL;
+// The caches of a call into the kernels' parameters, checked.
+static int prefix_check(const skv_prefix *c, int splits, float scale, PrefixParams &p) {
+    if (!c) return SKV_E_NULL;
     if ((c->prefix > 0 && (!c->k_prefix || !c->v_prefix)) || (c->rows_limit > 0 && (!c->k || !c->v))) return SKV_E_NULL;
     if (c->d != HEAD_DIM) return SKV_E_DIM;
     if (c->dtype != SKV_BF16 && c->dtype != SKV_F32) return SKV_E_DTYPE;
@@ -706,9 +713,7 @@ extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32
     if (c->batch <= 0 || c->h_kv <= 0 || (int64_t)c->batch * c->h_kv > 65535 || c->prefix < 0 || c->rows_limit < 0 ||
         (int64_t)c->prefix + c->rows_limit > 0x7fffffff - 64 || splits <= 0 || splits > 65535 || c->n_group < 0)
         return SKV_E_RANGE;
-    if (!aligned16(q) || !aligned16(c->k) || !aligned16(c->v) || !aligned16(out) || !aligned16(workspace) ||
-        !aligned16(c->k_prefix) || !aligned16(c->v_prefix))
-        return SKV_E_ALIGN;
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_prefix) || !aligned16(c->v_prefix)) return SKV_E_ALIGN;
     const int per16 = c->dtype == SKV_BF16 ? 8 : 4;
     const int64_t strides[8] = {c->kp_head_stride, c->kp_row_stride, c->vp_head_stride, c->vp_row_stride,
                                 c->k_head_stride, c->k_row_stride, c->v_head_stride, c->v_row_stride};
@@ -716,15 +721,33 @@ extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32
         const int rows = i < 4 ? c->prefix : c->rows_limit;
         if (strides[i] % per16 || ((i & 1) && rows > 1 && strides[i] < HEAD_DIM)) return SKV_E_ALIGN;
     }
-    PrefixParams p = {};
-    p.q = q; p.kp = c->k_prefix; p.vp = c->v_prefix; p.k = c->k; p.v = c->v; p.n_dev = n_dev; p.out = out; p.status = status;
+    p.kp = c->k_prefix; p.vp = c->v_prefix; p.k = c->k; p.v = c->v;
     p.batch = c->batch; p.h_kv = c->h_kv; p.G = c->G; p.n_group = c->n_group; p.prefix = c->prefix; p.rows_limit = c->rows_limit;
     p.splits = splits;
-    p.part = static_cast<float *>(workspace);
-    p.ticket = reinterpret_cast<int32_t *>(p.part + (int64_t)c->batch * c->h_kv * splits * c->G * PART_LD);
     p.kph = c->kp_head_stride; p.kpr = c->kp_row_stride; p.vph = c->vp_head_stride; p.vpr = c->vp_row_stride;
     p.ksh = c->k_head_stride; p.ksr = c->k_row_stride; p.vsh = c->v_head_stride; p.vsr = c->v_row_stride;
     p.scale_log2 = scale * LOG2E;
+    return SKV_OK;
+}
+
+extern "C" int skv_prefix_launches(const skv_prefix *c, int splits, float scale) {
+    PrefixParams p = {};
+    const int rc = prefix_check(c, splits, scale, p);
+    if (rc) return rc;
+    CUtensorMap kmap, vmap;
+    return c->dtype == SKV_BF16 && prefix_tile_ctas(p, &kmap, &vmap) > 0 ? 2 : 1;
+}
+
+extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32_t *n_dev, void *out, void *workspace, int splits,
+                                 int32_t *status, float scale, void *stream) {
+    if (!q || !n_dev || !out || !workspace) return SKV_E_NULL;
+    PrefixParams p = {};
+    const int rc = prefix_check(c, splits, scale, p);
+    if (rc) return rc;
+    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace)) return SKV_E_ALIGN;
+    p.q = q; p.n_dev = n_dev; p.out = out; p.status = status;
+    p.part = static_cast<float *>(workspace);
+    p.ticket = reinterpret_cast<int32_t *>(p.part + (int64_t)c->batch * c->h_kv * splits * c->G * PART_LD);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->dtype == SKV_F32) return launch_prefix_simple<float>(p, st);
     return launch_prefix_mma(p, st);

@@ -8,6 +8,7 @@ from contextlib import nullcontext
 
 import torch
 
+from . import _lib
 from ._lib import SkvError, SkvPrefix, check, dtype_code, elsewhere, lib, stream_ptr
 from .qwen3 import KVCache
 
@@ -94,6 +95,7 @@ class PrefixAttentionGraph:
         self.device = self.out.device                      # (with its index)
         self._shape, self._scale = self.out.shape, 1.0 / math.sqrt(d)
         self._layout = self._call = None                   # of the last call, and what it passed on
+        self._second = None                                # launches of such a call beyond the first
 
     def _plan(self, Kp, Vp, K, V) -> SkvPrefix:
         """What calls with caches of this layout pass on, checked once."""
@@ -113,7 +115,7 @@ class PrefixAttentionGraph:
         ``n_dev`` int32 on the device, own lengths: one, or one per ``n_group`` KV heads.  A row without keys gets zeros."""
         layout = (Kp.shape, Kp.stride(), Vp.shape, Vp.stride(), K.shape, K.stride(), V.shape, V.stride())
         if layout != self._layout:                         # (a decode step has the same layout again and again)
-            self._call, self._layout = self._plan(Kp, Vp, K, V), layout
+            self._call, self._layout, self._second = self._plan(Kp, Vp, K, V), layout, None
         dev, dtype = self.device, self.dtype
         if q.shape != self._shape or q.dtype is not dtype:
             raise ValueError(f"queries must be {tuple(self._shape)} {dtype}")
@@ -136,4 +138,8 @@ class PrefixAttentionGraph:
         check(lib().skv_attend_prefix(c, q.data_ptr(), n_dev.data_ptr(), self.out.data_ptr(), self.ws.data_ptr(),
                                       self.num_splits, self.status.data_ptr(), self._scale, stream_ptr(dev)),
               "skv_attend_prefix")
+        if self._second != 0:
+            if self._second is None:
+                self._second = lib().skv_prefix_launches(c, self.num_splits, self._scale) - 1
+            _lib.launches += self._second
         return self.out

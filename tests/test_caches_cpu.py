@@ -361,3 +361,13 @@ def test_what_the_attentions_bounds_leave_outside(bits, n):
         assert found(lambda kc, ks, vc, vs: (kc, exchanged(ks, 0, 1), vc, vs))
         assert found(lambda kc, ks, vc, vs: (kc, ks, vc, exchanged(vs, 2, 3)))
     assert not found(lambda kc, ks, vc, vs: (kc, ks, vc, vs))
+
+
+def test_the_launches_of_a_shared_prefix_call_are_known_ahead(L):
+    c = _lib.SkvPrefix(OK, OK, OK, OK, 128 * 100, 128, 128 * 100, 128, 128 * 64, 128, 128 * 64, 128, 100, 64, 2, 4, 2, 128, 0, 0)
+    assert L.skv_prefix_launches(ctypes.byref(c), 4, 0.1) == 1                   # a short prefix: by the list
+    c.dtype, c.prefix = 1, 100000
+    assert L.skv_prefix_launches(ctypes.byref(c), 4, 0.1) == 1                   # float32: always one
+    assert L.skv_prefix_launches(None, 4, 0.1) == -1
+    c.d = 64
+    assert L.skv_prefix_launches(ctypes.byref(c), 4, 0.1) == -2

@@ -387,3 +387,21 @@ def test_a_key_that_is_no_number_leaves_no_number(dtype, B, P, n):
     got = run_plain(q, kp, vp, k, v, B, Hk, G, dtype).view(B, Hk, G, 128).isnan()
     assert bool(got[:, 1].all()) and bool(got[1, 0].all())
     assert not bool(got[0, 0].any()) and not bool(got[2:, 0].any())
+
+
+@pytest.mark.parametrize("P,extra", [(100, 0), (40000, 1)])
+def test_a_captured_step_counts_the_prefixs_own_launch(P, extra):
+    """By the list a step has as many launches as over whole caches, by the tiles one more per layer."""
+    with torch.device(DEV):
+        model = Qwen3Model(Qwen3Config(**{**TINY, "max_position_embeddings": 50000}))
+    model = model.to(torch.bfloat16).eval().init_random(seed=3, std=0.05)
+    counts = []
+    for cache in (model.alloc_cache(64, 4), model.alloc_prefix_cache(P, 8, 4)):
+        if isinstance(cache, PrefixKVCache):
+            cache.prefix.cur_len = P                       # (rows of zeros)
+            cache.cur_len = P
+        dec = GraphDecoder(model, cache, mode="dense")
+        dec.prepare(cache.cur_len)
+        dec.capture()
+        counts.append(dec.launches_per_step)
+    assert counts[1] == counts[0] + extra * len(model.layers)

@@ -49,7 +49,7 @@ extern "C" {
 #define SKV_ST_NO_SLOT      1 /* a cluster passed its cap but every slot is in use */
 #define SKV_ST_SPLIT_TOO_BIG 2 /* a cluster over the cap has more members than the split can stage */
 #define SKV_ST_BAD_INDEX    4 /* a listed position or a label was out of range and was skipped */
-#define SKV_ST_WAIT_TIMEOUT 8 /* a bounded wait for another GPU's partial sums gave up (skv_comm.status) */
+#define SKV_ST_WAIT_TIMEOUT 8 /* a bounded wait gave up: for another GPU's partial sums (skv_comm.status), or within skv_attend_prefix */
 
 /* Cluster state of `heads` independent (layer, sequence, KV head) entries, structure of arrays.
  * Arrays are contiguous over heads: x[head][...].  Mirrors the tensors of

@@ -593,6 +593,14 @@ class GraphDecoder:
             raise ValueError(f"position {min(at) if min(at) < self.first else max(at)} lies outside the cache's "
                              f"[{self.first}, {end})")
 
+    def check_status(self) -> int:
+        """OR of the device status words of the attention objects and of the cache (synchronises); 0 means that no step has
+        recorded a problem: a position or a length outside the cache, a wait that gave up, the clusters' own."""
+        word = 0
+        for x in {id(x): x for x in (self.cache, *self.attn) if hasattr(x, "check_status")}.values():
+            word |= x.check_status()
+        return word
+
     def capture(self) -> None:
         """Record one decode step.  Call after ``prepare`` and before the first ``step``; the warm-up
         runs write a placeholder at the current position, which the first real step overwrites."""

@@ -97,6 +97,14 @@ class PrefixAttentionGraph:
         self._layout = self._call = None                   # of the last call, and what it passed on
         self._second = None                                # launches of such a call beyond the first
 
+    def check_status(self) -> int:
+        """Bits of ``SKV_ST_*`` over all heads (a length beyond the own rows, a wait that gave up and left a wrong output);
+        synchronises."""
+        bits = 0
+        for s in set(self.status.tolist()):
+            bits |= s
+        return bits
+
     def _plan(self, Kp, Vp, K, V) -> SkvPrefix:
         """What calls with caches of this layout pass on, checked once."""
         heads = self.B * self.H_kv

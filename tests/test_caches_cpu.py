@@ -371,3 +371,16 @@ def test_the_launches_of_a_shared_prefix_call_are_known_ahead(L):
     assert L.skv_prefix_launches(None, 4, 0.1) == -1
     c.d = 64
     assert L.skv_prefix_launches(ctypes.byref(c), 4, 0.1) == -2
+
+
+def test_the_status_words_of_a_decoder_are_read_together(L):
+    m = Qwen3Model(Qwen3Config(**TINY)).eval()
+    prefix = GraphDecoder(m, m.alloc_prefix_cache(8, 4, 2), mode="dense")
+    assert prefix.check_status() == 0 == prefix.attn[0].check_status()
+    prefix.attn[0].status[1], prefix.attn[0].status[3] = 4, 16
+    assert prefix.attn[0].check_status() == 20 == prefix.check_status()
+    quantised = GraphDecoder(m, m.alloc_cache(16, 2, bits=8), mode="dense")
+    assert quantised.check_status() == 0
+    quantised.cache.status[2] = 4
+    assert quantised.check_status() == 4
+    assert GraphDecoder(m, m.alloc_cache(16), mode="dense").check_status() == 0

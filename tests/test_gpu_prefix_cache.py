@@ -405,3 +405,18 @@ def test_a_captured_step_counts_the_prefixs_own_launch(P, extra):
         dec.capture()
         counts.append(dec.launches_per_step)
     assert counts[1] == counts[0] + extra * len(model.layers)
+
+
+def test_a_decoder_over_a_shared_prefix_reports_a_length_beyond_its_rows():
+    model, B = tiny_model(), 2
+    cache = model.alloc_prefix_cache(20, 6, B)
+    with torch.no_grad():
+        model.prefill(torch.arange(20, device=DEV).view(1, -1), cache.prefix)
+        dec = GraphDecoder(model, cache, mode="dense")
+        dec.prepare(20)
+        dec.step(torch.zeros(B, 1, dtype=torch.long, device=DEV), 20)
+        assert dec.check_status() == 0
+        kh, vh = dec._heads(cache.k[0]), dec._heads(cache.v[0])
+        q = torch.zeros(B * dec.H, 128, dtype=torch.bfloat16, device=DEV)
+        dec.attn[0](q, *cache.prefix_rows(0), kh, vh, torch.tensor([7], dtype=torch.int32, device=DEV))
+    assert dec.check_status() == 4

@@ -246,14 +246,19 @@ def dtype_code(dt: torch.dtype) -> int:
     raise ValueError(f"unsupported cache dtype {dt}; the kernels take bfloat16 or float32")
 
 
+# The short ways to the current device and to a device's current stream; PyTorch's public ones take 2.3 us a call instead of 0.1
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def elsewhere(device) -> bool:
     """Whether another CUDA device than ``device`` (given with its index) is the current one: a launch goes to the current
     device, a caller's tensors may live on another."""
-    return device.type == "cuda" and device.index != torch._C._cuda_getDevice()
+    return device.type == "cuda" and device.index != _current_device()
 
 
 def stream_ptr(device=None) -> int:
-    """Address of the device's current stream.  A device with its index takes the short way (0.1 us instead of 2.3)."""
-    if device is not None and device.index is not None:
-        return torch._C._cuda_getCurrentRawStream(device.index)
+    """Address of the device's current stream; ``device`` as ``torch.cuda.current_stream`` takes it."""
+    if _raw_stream is not None and isinstance(device, torch.device) and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream

@@ -384,3 +384,15 @@ def test_the_status_words_of_a_decoder_are_read_together(L):
     quantised.cache.status[2] = 4
     assert quantised.check_status() == 4
     assert GraphDecoder(m, m.alloc_cache(16), mode="dense").check_status() == 0
+
+
+def test_the_current_stream_of_any_kind_of_device(monkeypatch):
+    """A device with its index takes the short way where PyTorch has one; anything else goes to its public function."""
+    asked = []
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: asked.append(d) or type("S", (), {"cuda_stream": 77}))
+    monkeypatch.setattr(_lib, "_raw_stream", lambda index: 100 + index)
+    assert _lib.stream_ptr(torch.device("cuda", 3)) == 103 and asked == []
+    for device in (None, 1, "cuda", "cuda:1", torch.device("cuda")):
+        assert _lib.stream_ptr(device) == 77 and asked[-1] == device
+    monkeypatch.setattr(_lib, "_raw_stream", None)
+    assert _lib.stream_ptr(torch.device("cuda", 2)) == 77 and asked[-1] == torch.device("cuda", 2)

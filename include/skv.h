@@ -437,13 +437,13 @@ int skv_gemv_supported(int N, int K, int B, int mode);
  * or 8.  A group whose scale would be below the smallest normal number holds zeros; a group with an Inf or NaN has a NaN
  * scale and reads back as NaN. */
 typedef struct skv_qcache {
-    void *k, *v;          /* [batch, h_kv, capacity, 16 * bits] bytes, 16-byte aligned */
-    void *scale;          /* [batch, h_kv, capacity, 2, groups] bf16: the key's scales, then the value's */
-    int32_t *status;      /* [batch * h_kv] SKV_ST_* bits, or null */
+    void *k, *v;          /* [skip + batch, h_kv, capacity, 16 * bits] bytes */
+    void *scale;          /* [.., h_kv, capacity, 2, groups] bf16: the key's scales, then the value's; all three 16-byte aligned */
+    int32_t *status;      /* [.. * h_kv] SKV_ST_* bits, or null */
     int32_t batch, h_kv, capacity;
     int32_t d;            /* 128 */
     int32_t bits;         /* 8 or 4 */
-    int32_t reserved;
+    int32_t skip;         /* sequences of the buffers ahead of these `batch` ones: buffers and status are the whole cache's */
 } skv_qcache;
 
 /* Rows of a call below: k, v [batch, h_kv, tokens, 128] (dtype; element strides, unit last stride, rows 16-byte aligned) and

@@ -49,7 +49,7 @@ class SkvQCache(C.Structure):
     """``skv_qcache`` of include/skv.h: one layer of a quantised KV cache."""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("scale", C.c_void_p), ("status", C.c_void_p),
                 ("batch", C.c_int32), ("h_kv", C.c_int32), ("capacity", C.c_int32), ("d", C.c_int32),
-                ("bits", C.c_int32), ("reserved", C.c_int32)]
+                ("bits", C.c_int32), ("skip", C.c_int32)]
 
 
 class SkvRows(C.Structure):

@@ -836,8 +836,8 @@ extern "C" int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, i
     p.ctas = ctas; p.splits = (ctas + p.heads) / p.heads;
     p.rows = quant_rows(G);
     p.q = q; p.out = out; p.n_dev = n_dev;
-    p.kc = static_cast<const unsigned char *>(c->k); p.vc = static_cast<const unsigned char *>(c->v);
-    p.scale = static_cast<const __nv_bfloat16 *>(c->scale);
+    const QuantRows at = qcache_rows(c);
+    p.kc = at.k; p.vc = at.v; p.scale = at.scale;
     p.part = static_cast<float *>(workspace);
     p.ticket = reinterpret_cast<int32_t *>(p.part + ((int64_t)ctas + p.heads) * G * PART_LD);
     p.scale_log2 = scale * LOG2E;

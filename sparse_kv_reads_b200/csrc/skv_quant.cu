@@ -353,8 +353,8 @@ static int rows_check(const skv_qcache *c, const void *k, const void *v, int dty
         return SKV_E_ALIGN;
     p.k = const_cast<void *>(k); p.v = const_cast<void *>(v);
     p.kb = kb; p.kh = kh; p.kr = kr; p.vb = vb; p.vh = vh; p.vr = vr;
-    p.kc = static_cast<unsigned char *>(c->k); p.vc = static_cast<unsigned char *>(c->v);
-    p.scale = static_cast<__nv_bfloat16 *>(c->scale); p.status = c->status;
+    const QuantRows at = qcache_rows(c);
+    p.kc = at.k; p.vc = at.v; p.scale = at.scale; p.status = at.status;
     p.pos = pos; p.pos0 = pos0;
     p.batch = batch; p.h_kv = c->h_kv; p.capacity = c->capacity; p.tokens = tokens;
     p.items = (uint32_t)batch * c->h_kv * tokens;

@@ -136,9 +136,25 @@ static inline int qcache_check(const skv_qcache *c) {
     if (!c || !c->k || !c->v || !c->scale) return SKV_E_NULL;
     if (c->d != HEAD_DIM) return SKV_E_DIM;
     if (c->bits != 8 && c->bits != 4) return SKV_E_RANGE;
-    if (c->batch <= 0 || c->h_kv <= 0 || c->capacity <= 0 || (int64_t)c->batch * c->h_kv > 65535) return SKV_E_RANGE;
+    if (c->batch <= 0 || c->skip < 0 || c->h_kv <= 0 || c->capacity <= 0 ||
+        ((int64_t)c->skip + c->batch) * c->h_kv > 65535)
+        return SKV_E_RANGE;
     if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->scale)) return SKV_E_ALIGN;
     return SKV_OK;
+}
+
+// Where the rows of the struct's sequences begin.  (The scales may begin on any position's: no load of them takes more than one
+// position's, 4 bytes in 8 bits and 16 in 4.)
+struct QuantRows {
+    unsigned char *k, *v;
+    __nv_bfloat16 *scale;
+    int32_t *status;
+};
+static inline QuantRows qcache_rows(const skv_qcache *c) {
+    const int64_t heads = (int64_t)c->skip * c->h_kv, rows = heads * c->capacity, codes = rows * (HEAD_DIM * c->bits / 8);
+    return {static_cast<unsigned char *>(c->k) + codes, static_cast<unsigned char *>(c->v) + codes,
+            static_cast<__nv_bfloat16 *>(c->scale) + rows * (c->bits == 8 ? Quant<8>::SCALES : Quant<4>::SCALES),
+            c->status ? c->status + heads : nullptr};
 }
 
 }  // namespace skv

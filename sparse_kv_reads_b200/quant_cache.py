@@ -78,9 +78,14 @@ class QuantKVCache:
 
     def sequence(self, b: int) -> "QuantKVCache":
         """Sequence ``b`` alone, on the same memory."""
+        if not 0 <= b < self.batch:
+            raise ValueError(f"the cache holds {self.batch} sequences")
         h = self.h_kv
-        return self.from_tensors([t[b:b + 1] for t in self.k], [t[b:b + 1] for t in self.v],
-                                 [t[b:b + 1] for t in self.scale], self.bits, self.status[b * h:(b + 1) * h])
+        one = self.from_tensors([t[b:b + 1] for t in self.k], [t[b:b + 1] for t in self.v],
+                                [t[b:b + 1] for t in self.scale], self.bits, self.status[b * h:(b + 1) * h])
+        # (its own scales may begin off the 16-byte boundary that a call's buffers have to be on: the whole cache's, and b on)
+        one._st = [SkvQCache(s.k, s.v, s.scale, s.status, 1, h, self.max_seq_len, self.d, self.bits, s.skip + b) for s in self._st]
+        return one
 
     def check_status(self) -> int:
         """Bits of ``SKV_ST_*`` over all heads (a position outside the cache was skipped); synchronises."""

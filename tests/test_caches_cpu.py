@@ -396,3 +396,18 @@ def test_the_current_stream_of_any_kind_of_device(monkeypatch):
         assert _lib.stream_ptr(device) == 77 and asked[-1] == device
     monkeypatch.setattr(_lib, "_raw_stream", None)
     assert _lib.stream_ptr(torch.device("cuda", 2)) == 77 and asked[-1] == torch.device("cuda", 2)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_a_sequence_of_a_cache_of_odd_length_is_taken_from_the_whole(L, bits):
+    """The scales of a later sequence may begin off the 16-byte boundary: its struct has the whole cache's addresses and the
+    number of sequences ahead of it."""
+    c = QuantKVCache(1, 3, 1, 33, 128, bits, CPU)
+    one = c.sequence(2).sequence(0)
+    st = one._st[0]
+    assert st.skip == 2 and st.batch == 1 and st.scale == c.scale[0].data_ptr() and st.k == c.k[0].data_ptr()
+    assert one.k[0].data_ptr() == c.k[0][2].data_ptr() and one.scale[0].data_ptr() == c.scale[0][2].data_ptr()
+    for b in (-1, 3):
+        with pytest.raises(ValueError, match="3 sequences"):
+            c.sequence(b)
+    assert L.skv_quant_write(qcache(skip=-1), ctypes.byref(_lib.SkvRows(OK, OK, None, 0, 0, 0, 128, 0, 0, 128, 0, 0, 1, 1)), None) == -5

@@ -518,3 +518,27 @@ def test_a_second_ragged_batch_runs_through_the_captured_step(bits):
     assert dec.graph is graph
     other = model.alloc_cache(128, 3, bits=bits)
     assert torch.equal(got, run(GraphDecoder(model, other, mode="dense"), other, batches[1], True))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("H,L", [(1, 33), (3, 27), (1, 34)])
+def test_a_sequence_whose_scales_begin_off_the_boundary(bits, H, L):
+    """One KV head and an odd length: written, read and attended over as the same rows of the whole cache."""
+    B, G, n = 4, 2, 20
+    whole, parts = (QuantKVCache(1, B, H, L, 128, bits, DEV) for _ in range(2))
+    k, v = rows_of(B, H, n, torch.bfloat16, 1, False).to(DEV), rows_of(B, H, n, torch.bfloat16, 2, False).to(DEV)
+    whole.write(0, k, v, 5)
+    q = torch.randn(B, H * G, 128, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(DEV)
+    n_dev = torch.tensor([5 + n], dtype=torch.int32, device=DEV)
+    for b in range(B):
+        parts.sequence(b).write(0, k[b:b + 1], v[b:b + 1], 5)
+        assert torch.equal(parts.sequence(b).read(0, 5, n)[0], whole.read(0, 5, n)[0][b:b + 1])
+    parts.sequence(3).write(0, k[:1], v[:1], torch.tensor([L - 3], device=DEV))              # recorded in its own words
+    assert parts.status.view(B, H).cpu().tolist() == [[0] * H] * 3 + [[4] * H]
+    assert all(torch.equal(a[:3], b[:3]) for a, b in zip((whole.k[0], whole.v[0], whole.scale[0]),
+                                                         (parts.k[0], parts.v[0], parts.scale[0])))
+    attn = QuantAttentionGraph(H=H * G, H_kv=H, d=128, dtype=torch.bfloat16, device=DEV)
+    whole_attn = QuantAttentionGraph(H=B * H * G, H_kv=B * H, d=128, dtype=torch.bfloat16, device=DEV)
+    want = whole_attn(q.view(B * H * G, 128), whole, 0, n_dev).view(B, H * G, 128)
+    for b in range(3):
+        assert torch.equal(attn(q[b], parts.sequence(b), 0, n_dev), want[b])

@@ -347,16 +347,17 @@ class GraphDecoder:
         """QK-norm + rotary + cache write of the new token, one launch.  ``pos`` counts the cache's own rows; the
         tables are taken from the position of the first."""
         m, a = self.model, self.model.layers[i].attn
-        cos, sin = m.rope_cos[self.first:], m.rope_sin[self.first:]
+        at = self.first * self.d * m.rope_cos.element_size()
+        cos, sin = m.rope_cos.data_ptr() + at, m.rope_sin.data_ptr() + at
         if isinstance(self.cache, QuantKVCache):
             check(lib().skv_qk_rope_quant(self.cache._st[i], qkv.data_ptr(), a.q_norm.weight.data_ptr(),
-                                          a.k_norm.weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), self.pos.data_ptr(),
+                                          a.k_norm.weight.data_ptr(), cos, sin, self.pos.data_ptr(),
                                           int(self.ragged), qh.data_ptr(), self.B, self.H, a.q_norm.eps, st),
                   "skv_qk_rope_quant")
             return
         kc, vc = self.cache.k[i], self.cache.v[i]
         check(lib().skv_qk_rope_cache(qkv.data_ptr(), a.q_norm.weight.data_ptr(), a.k_norm.weight.data_ptr(),
-                                      cos.data_ptr(), sin.data_ptr(), self.pos.data_ptr(), int(self.ragged), qh.data_ptr(),
+                                      cos, sin, self.pos.data_ptr(), int(self.ragged), qh.data_ptr(),
                                       kc.data_ptr(), vc.data_ptr(), self.B, self.H, self.H_kv, self.d, kc.stride(0),
                                       kc.stride(1), kc.stride(2), a.q_norm.eps, st), "skv_qk_rope_cache")
 

@@ -411,3 +411,39 @@ def test_a_sequence_of_a_cache_of_odd_length_is_taken_from_the_whole(L, bits):
         with pytest.raises(ValueError, match="3 sequences"):
             c.sequence(b)
     assert L.skv_quant_write(qcache(skip=-1), ctypes.byref(_lib.SkvRows(OK, OK, None, 0, 0, 0, 128, 0, 0, 128, 0, 0, 1, 1)), None) == -5
+
+
+def test_the_rotary_launch_takes_its_tables_by_address(L, monkeypatch):
+    """From the position of the cache's first row, without a tensor operation per layer (an eager step has 28 of them)."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from sparse_kv_reads_b200 import graph_decode
+
+    class Nothing(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            raise AssertionError(f"{func} was called")
+
+    got = {}
+
+    class Fake:
+        def skv_qk_rope_cache(self, *a):
+            got["cos"], got["sin"] = a[3], a[4]
+            return 0
+
+        def skv_qk_rope_quant(self, *a):
+            got["cos"], got["sin"] = a[4], a[5]
+            return 0
+
+    m = Qwen3Model(Qwen3Config(**TINY)).eval()
+    prefix = m.alloc_prefix_cache(8, 4, 2)
+    prefix.prefix.cur_len = 6
+    x = torch.zeros(2, 8 * 128)
+    for cache, first in ((m.alloc_cache(8, 2), 0), (m.alloc_cache(8, 2, bits=8), 0), (prefix, 6)):
+        dec = GraphDecoder(m, cache, mode="dense")
+        dec.prepare(first)
+        monkeypatch.setattr(graph_decode, "lib", Fake)
+        with Nothing():
+            dec._rope(0, x, x, 0)
+        monkeypatch.undo()
+        row = m.rope_cos[0].numel() * m.rope_cos.element_size()
+        assert got == {"cos": m.rope_cos.data_ptr() + first * row, "sin": m.rope_sin.data_ptr() + first * row}

@@ -15,6 +15,7 @@ import os
 
 import ctypes
 import math
+from operator import index
 
 import torch
 
@@ -588,7 +589,10 @@ class GraphDecoder:
             raise ValueError("positions in a quantised or shared-prefix cache are given on the host, where they are checked")
         if self.first != self.cache.first:
             raise ValueError("the shared prefix has changed since prepare()")
-        at = [int(pos)] if isinstance(pos, int) or (torch.is_tensor(pos) and pos.dim() == 0) else [int(x) for x in pos]
+        try:
+            at = [index(pos)]
+        except TypeError:                                  # one per sequence
+            at = [index(x) for x in pos]
         end = min(self.cache.max_seq_len, self.model.rope_cos.shape[0])
         if min(at) < self.first or max(at) >= end:
             raise ValueError(f"position {min(at) if min(at) < self.first else max(at)} lies outside the cache's "

@@ -29,7 +29,8 @@ class PrefixKVCache:
     @property
     def first(self) -> int:
         """Position of the sequences' first own row: the prefix's length."""
-        return self.prefix.cur_len
+        n = self.prefix.cur_len
+        return n[0] if isinstance(n, list) else n          # (a list: prefilled as a ragged batch of one)
 
     @property
     def max_seq_len(self) -> int:

@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 import threading
 from contextlib import nullcontext
+from operator import index
 
 import torch
 
@@ -102,7 +103,7 @@ class QuantKVCache:
                 raise ValueError("positions are an int, or int64 [1] or [sequences] on the cache's device")
             rows.pos, rows.pos_per_seq = pos.data_ptr(), int(pos.shape[0] != 1)
             return
-        at = int(pos)
+        at = index(pos)
         if not 0 <= at <= self.max_seq_len - count:
             raise ValueError(f"rows [{at}, {at + count}) lie outside the cache's {self.max_seq_len} positions")
         rows.pos, rows.pos_per_seq, rows.pos0 = None, 0, at

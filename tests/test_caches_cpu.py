@@ -447,3 +447,32 @@ def test_the_rotary_launch_takes_its_tables_by_address(L, monkeypatch):
         monkeypatch.undo()
         row = m.rope_cos[0].numel() * m.rope_cos.element_size()
         assert got == {"cos": m.rope_cos.data_ptr() + first * row, "sin": m.rope_sin.data_ptr() + first * row}
+
+
+def test_positions_are_whole_numbers_of_any_kind(L):
+    np = pytest.importorskip("numpy")
+    c = QuantKVCache(1, 1, 2, 16, 128, 8, CPU)
+    x = torch.zeros(1, 2, 1, 128, dtype=torch.bfloat16)
+    with pytest.raises(TypeError):
+        c.write(0, x, x, 2.7)                              # (was taken for 2)
+    with pytest.raises(ValueError, match="CUDA device only"):
+        c.write(0, x, x, np.int64(3))
+    m = Qwen3Model(Qwen3Config(**TINY)).eval()
+    cache = m.alloc_prefix_cache(8, 4, 2)
+    cache.prefix.cur_len = 6
+    dec = GraphDecoder(m, cache, mode="dense")
+    dec.prepare(6)
+    for pos in (np.int64(10), torch.tensor(10), torch.tensor([10]), [6, 10]):
+        with pytest.raises(ValueError, match="position 10 lies outside"):
+            dec.step(torch.zeros(2, 1, dtype=torch.long), pos)
+
+
+def test_a_prefix_prefilled_as_a_ragged_batch_of_one():
+    m = Qwen3Model(Qwen3Config(**TINY)).eval().init_random(seed=3, std=0.1)
+    cache = m.alloc_prefix_cache(40, 16, 2)
+    with torch.no_grad():
+        m.prefill_ragged([torch.arange(30)], cache.prefix)
+        assert cache.first == 30 and cache.max_seq_len == 46 and cache.cur_len == 30
+        got = m.prefill(torch.arange(5).view(1, -1).expand(2, -1), cache)
+        want = m.prefill(torch.cat((torch.arange(30), torch.arange(5))).view(1, -1), m.alloc_cache(64))
+    torch.testing.assert_close(got[:1], want, rtol=1e-4, atol=1e-4)

@@ -64,14 +64,20 @@ class QuantKVCache:
         return self
 
     def _set(self, k, v, scale, bits, status) -> None:
-        self.k, self.v, self.scale, self.bits = k, v, scale, bits
+        self._k, self._v, self._scale, self.bits = tuple(k), tuple(v), tuple(scale), bits
         self.batch, self.h_kv, self.max_seq_len, _ = k[0].shape
         self.d, self.device = 128, k[0].device
         self.cur_len = 0
         self._kept = threading.local()                     # plans of writes and reads (below), one set per thread
-        self.status = torch.zeros(self.batch * self.h_kv, dtype=torch.int32, device=self.device) if status is None else status
+        self._status = torch.zeros(self.batch * self.h_kv, dtype=torch.int32, device=self.device) if status is None else status
         self._st = [SkvQCache(a.data_ptr(), b.data_ptr(), s.data_ptr(), self.status.data_ptr(), self.batch, self.h_kv,
                               self.max_seq_len, self.d, bits, 0) for a, b, s in zip(k, v, scale)]
+
+    # (read-only: calls go by the addresses taken above)
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    scale = property(lambda self: self._scale)
+    status = property(lambda self: self._status)
 
     def _on_gpu(self) -> None:
         if self.device.type != "cuda":

@@ -476,3 +476,14 @@ def test_a_prefix_prefilled_as_a_ragged_batch_of_one():
         got = m.prefill(torch.arange(5).view(1, -1).expand(2, -1), cache)
         want = m.prefill(torch.cat((torch.arange(30), torch.arange(5))).view(1, -1), m.alloc_cache(64))
     torch.testing.assert_close(got[:1], want, rtol=1e-4, atol=1e-4)
+
+
+def test_the_tensors_of_a_quantised_cache_stay_its_own(L):
+    """Their addresses are part of the cache: a layer's tensor cannot be exchanged for another behind its back."""
+    c = QuantKVCache(2, 1, 2, 16, 128, 8, CPU)
+    for ts in (c.k, c.v, c.scale, c.sequence(0).k):
+        with pytest.raises(TypeError):
+            ts[0] = torch.zeros_like(ts[0])
+    for name in ("k", "v", "scale", "status"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name))

@@ -435,7 +435,8 @@ int skv_gemv_supported(int N, int K, int B, int mode);
  * 32 values, 64 bytes, two codes per byte (the lower nibble first), the row's 32 runs of four values in the order
  * (run % 8, run / 8).  scale = bf16(largest magnitude / M), M = 127 or 7; stored = round(x / scale) within +-M, plus 128
  * or 8.  A group whose scale would be below the smallest normal number holds zeros; a group with an Inf or NaN has a NaN
- * scale and reads back as NaN. */
+ * scale and reads back as NaN.  code * scale is within half a scale of x; within 2^-8 of the largest bf16 number its rounding
+ * to bf16 can be Inf. */
 typedef struct skv_qcache {
     void *k, *v;          /* [skip + batch, h_kv, capacity, 16 * bits] bytes */
     void *scale;          /* [.., h_kv, capacity, 2, groups] bf16: the key's scales, then the value's; all three 16-byte aligned */
@@ -460,8 +461,8 @@ typedef struct skv_rows {
     int32_t tokens;
 } skv_rows;
 
-/* Quantises rows as they are written.  Rows that fall outside the cache by a device position are left out and recorded
- * (SKV_ST_BAD_INDEX); a pos0 outside is SKV_E_RANGE. */
+/* Quantises rows as they are written.  Rows that a device position puts behind the cache's end are left out and recorded
+ * (SKV_ST_BAD_INDEX), and all of a sequence's rows where its first position is negative; a pos0 outside is SKV_E_RANGE. */
 int skv_quant_write(const skv_qcache *c, const skv_rows *rows, void *stream);
 /* The way back: value = code * scale, rounded once to dtype.  Rows outside the cache come back as zeros, recorded. */
 int skv_quant_read(const skv_qcache *c, const skv_rows *rows, void *stream);
@@ -475,7 +476,10 @@ int skv_qk_rope_quant(const skv_qcache *c, const void *qkv, const void *q_norm_w
  * (ssa/kernels/graph_kernels.py:27-59) for a quantised cache.  q, out [batch * h_kv * G, 128] dtype, G <= 8; n_dev and
  * n_group as everywhere (a length beyond the capacity counts as the capacity).  `ctas` CTAs share all heads' rows evenly
  * (skv_quant_ctas: as many as the current device runs at once); workspace of skv_quant_workspace_bytes(batch * h_kv, G, 128,
- * ctas), zero-initialised once.  A head without rows gets zeros. */
+ * ctas), zero-initialised once.  A head without rows gets zeros, one with a key that is no number gets NaN.
+ * bf16 queries: scores and sums in float32, right for scores of up to 2^104; the products take half floats: the queries
+ * (components to 2^-25 of the largest, 2^-21 in odd places of 4 bits, 2^-16 and 2^-12 where the largest is below 2^-20) and the
+ * weights times the value scales (11 bits of each, whatever the scales; weights below 2^-126 of the largest count as zero).  float32 queries: float32 throughout. */
 int skv_quant_ctas(void);
 int64_t skv_quant_workspace_bytes(int heads, int G, int d, int ctas);
 int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, int G, const int32_t *n_dev, int n_group, void *out,
@@ -502,7 +506,9 @@ typedef struct skv_prefix {
  *   q, out     [batch * h_kv * G, 128]
  *   n_dev      own lengths; one beyond rows_limit counts as rows_limit and is recorded in `status` ([batch * h_kv], may be null)
  *   splits     skv_prefix_splits(batch, h_kv, G, dtype); workspace of skv_prefix_workspace_bytes bytes, zero-initialised once
- * A row without any key gets zeros. */
+ * A row without any key gets zeros, one with a key that is no number NaN.  bf16: scores and sums in float32; the weights are rounded
+ * to bf16 (8 bits) for the product with the values, as skv_attend does it, while their sum takes them unrounded: the output's
+ * error against 64 bits is 2.3e-3 of its size instead of the 1.7e-3 of its own rounding.  float32: float32 throughout. */
 int skv_prefix_splits(int batch, int h_kv, int G, int dtype);
 int64_t skv_prefix_workspace_bytes(int batch, int h_kv, int G, int d, int splits);
 /* How many kernels such a call launches (1 or 2: bf16 prefixes beyond a size have a launch of their own), or an SKV_E_* code. */

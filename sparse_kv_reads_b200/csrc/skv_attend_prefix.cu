@@ -113,7 +113,9 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
 // have an accumulator each (slot 0 and 1): with more than 128 query rows they take 128 rows each of every tile, else both
 // have the same rows and take the tiles in turn, and are merged at the end.  A thread owns one row: it reads its 128 scores
 // from tensor memory, so that no maximum needs a shuffle, and writes the weights back over them in bf16 as the A operand of
-// the second product.  One thread feeds the ring of K and V tiles by TMA (rows beyond the prefix read as zeros), one issues
+// the second product (which takes A and B of one type, and the values are bf16; half floats would not hold them all, and a
+// product with the weights' remainders as well would add a half to those that bound the wide case.  The sum of the weights
+// is taken before they are rounded, in float32).  One thread feeds the ring of K and V tiles by TMA (rows beyond the prefix read as zeros), one issues
 //   S = Q K^T  (both K-major in shared memory)        O += P V  (P in tensor memory, V MN-major)
 // with the two slots strictly in turn, so that one's products run beside the other's softmax.  Accumulators are rescaled only
 // when a row's maximum rises by more than 8 (base 2).
@@ -122,8 +124,8 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
 // out.  With more rows the one sequence of products: for each slot of a tile about 560 cycles for the weighted values, 650 for
 // the scores (both operands from shared memory, beside the incoming tiles) and 500 of waits and commits between them, 3,430
 // cycles a tile where the tensor cores alone need 2,048; a slot's weights lie ready 360 cycles before their turn comes (its
-// softmax takes 1,650: loads 115, maximum 280, exponentials 1,230).
-// Measured and not kept (128 sequences x 4 query heads x 16,383 keys, 53.5 us with the second launch): scores and weights by
+// softmax takes 1,650: loads 115, maximum 280, exponentials 1,230; taken with scale and difference in one fused operation).
+// Measured and not kept (128 sequences x 4 query heads x 16,383 keys, 53.5 us with the second launch, as it then was): scores and weights by
 // halves of a tile (71.6 us: with 64 keys on N the queries are read from shared memory twice as often), an issuing thread per
 // slot (62.4 us: the slots fall into step), weights released by halves (54.9 us).  Within 1 us of it, either way, since the
 // softmax does not bound it: half the weights against the standing reference while the maximum is found, products issued by

@@ -14,7 +14,9 @@
 // the rows' nor the columns' reads meet in a bank.  (Loads straight into registers kept one tile in flight per warp: 109 us
 // against 92 us for 64 heads of 32,768 8-bit rows, 85 against 75 us in 4 bits.)
 // What bounds it: 8 bits, the memory (64 heads of 32,768 rows: 83 us at the measured copy rate); 4 bits, the instructions
-// that turn two codes a byte into fragments (322 per 16 rows; the integer pipe is 54 % busy, the memory 61 %).
+// that turn two codes a byte into fragments (325 per 16 rows; the integer pipe is 53 % busy, the memory 60 %).
+// A reference for each value group costs 5 of them (75.4 against 74.2 us with one for all four, which held a group 2^-16 of the
+// largest to 5e-4 only).
 // Running references per head, in base 2: m for the sum of weights (largest score) and, for each scale group of the values, r for
 // the group's accumulators (largest score + log2 of the value's scale), so that the half floats 2^(z - r) vs keep their
 // precision whatever the scales of rows and groups (of weights down to 2^-126 of the head's largest).  m is only raised when

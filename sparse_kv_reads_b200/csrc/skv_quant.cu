@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(128) qk_rope_quant_kernel(const __nv_bfloat16 
 }
 
 // A flat grid where a chunk's CTA would be mostly idle (a decode step writes one position per sequence).
-static bool rows_flat(const RowsParams &p) { return p.tokens < 16 * AT_ONCE || p.batch > 65535 || p.h_kv > 65535; }
+static bool rows_flat(const RowsParams &p) { return p.tokens < 16 * AT_ONCE; }
 static dim3 rows_grid(const RowsParams &p) {
     if (rows_flat(p)) return dim3((p.items + 15) / 16);
     return dim3((unsigned)(p.tokens + 16 * AT_ONCE - 1) / (16 * AT_ONCE), (unsigned)p.h_kv, (unsigned)p.batch);

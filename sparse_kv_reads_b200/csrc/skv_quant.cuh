@@ -51,7 +51,7 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 
 // The stored codes of eight values, as the low bits of the results.  Adding 1.5 * 2^23 rounds a quotient to an integer, ties
-// to even, and leaves it, biased, in the low bits; no clamp is needed, since the scale is at most 2^-9 of itself too small.
+// to even, and leaves it, biased, in the low bits; no clamp is needed, since the scale is at most 2^-8 of itself too small.
 // EXACT: an IEEE quotient.  Else the values are bf16, like the scale: a quotient from a reciprocal y with one correction by
 // its exact remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).  Where the true
 // quotient lies half-way between two codes it is a float32 number t, the first quotient is t + d, its remainder -s d, and the

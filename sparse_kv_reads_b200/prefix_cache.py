@@ -74,7 +74,9 @@ class PrefixKVCache:
 class PrefixAttentionGraph:
     """Exact decode attention of ``B`` sequences over a prefix they share and over their own rows ``[0, n)`` behind it,
     with ``n`` in device memory.  ``H, H_kv`` are per sequence.  The object owns the workspace and the output buffer,
-    which the next call overwrites: calls of one object (and graphs captured from it) must not overlap on the GPU."""
+    which the next call overwrites: calls of one object (and graphs captured from it) must not overlap on the GPU.  bf16:
+    weights are rounded to bf16 in the product with the values, as in ``DenseAttentionGraph``; scores and sums are float32.
+    ``check_status()`` tells of lengths beyond the own rows and of a wait that gave up."""
 
     def __init__(self, *, B: int, H: int, H_kv: int, d: int, dtype, device):
         if H % H_kv:

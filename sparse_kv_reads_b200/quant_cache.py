@@ -140,8 +140,8 @@ class QuantKVCache:
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, pos) -> None:
         """Quantise ``k, v [b, H_kv, T, 128]`` (bf16 or float32, any strides) into the rows ``[pos, pos + T)`` of the
-        first ``b`` sequences.  ``pos``: an int, or int64 in device memory, one for all or one per sequence; rows of a
-        device position that fall outside the cache are left out and recorded in ``status``."""
+        first ``b`` sequences.  ``pos``: an int, or int64 in device memory, one for all or one per sequence; rows that a
+        device position puts behind the cache's end (all rows, where it is negative) are left out and recorded in ``status``."""
         rows, straight = self._plan((k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype), lambda: self._plan_write(k, v))
         dev = self.device
         if k.device != dev or v.device != dev:
@@ -200,7 +200,8 @@ class QuantKVCache:
 class QuantAttentionGraph:
     """Exact decode attention over the quantised rows ``[0, n)``, with ``n`` in device memory: ``DenseAttentionGraph``
     for a ``QuantKVCache``.  The object owns the workspace and the output buffer, which the next call overwrites: calls
-    of one object (and graphs captured from it) must not overlap on the GPU."""
+    of one object (and graphs captured from it) must not overlap on the GPU.  bf16: a weight times a value's scale is a half
+    float (11 bits) in the product with the codes; scores and sums are float32."""
 
     def __init__(self, *, H: int, H_kv: int, d: int, dtype, device):
         if H % H_kv:

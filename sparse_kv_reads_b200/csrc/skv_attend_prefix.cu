@@ -39,7 +39,7 @@ __device__ __forceinline__ int own_rows(const PrefixParams &p, int head) {
     return min(max(n, 0), p.rows_limit);
 }
 
-template <typename T, int GP>
+template <int GP>
 __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixParams p) {
     constexpr int WARPS = 4;
     __shared__ __align__(16) float red[2 * WARPS * GP * 132];
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
     const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
     const int sub = lane & 15, half = lane >> 4;
     const unsigned hmask = half ? 0xffff0000u : 0x0000ffffu;
-    const T *q = static_cast<const T *>(p.q) + (int64_t)head * G * HEAD_DIM;
+    const float *q = static_cast<const float *>(p.q) + (int64_t)head * G * HEAD_DIM;
 
     float qr[GP][8], acc[GP][8], m[GP], l[GP];
 #pragma unroll
@@ -70,10 +70,10 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
     for (int r = t0 * TILE_ROWS + half; r < r1; r += 2) {
         const bool shared = r < p.prefix;
         const int64_t own = r - p.prefix;
-        const T *kr = shared ? static_cast<const T *>(p.kp) + h * p.kph + (int64_t)r * p.kpr
-                             : static_cast<const T *>(p.k) + head * p.ksh + own * p.ksr;
-        const T *vr = shared ? static_cast<const T *>(p.vp) + h * p.vph + (int64_t)r * p.vpr
-                             : static_cast<const T *>(p.v) + head * p.vsh + own * p.vsr;
+        const float *kr = shared ? static_cast<const float *>(p.kp) + h * p.kph + (int64_t)r * p.kpr
+                             : static_cast<const float *>(p.k) + head * p.ksh + own * p.ksr;
+        const float *vr = shared ? static_cast<const float *>(p.vp) + h * p.vph + (int64_t)r * p.vpr
+                             : static_cast<const float *>(p.v) + head * p.vsh + own * p.vsr;
         float kv[8], vv[8];
         load8(kr + sub * 8, kv);
         load8(vr + sub * 8, vv);
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
         if (sub == 0) { r[128] = m[g]; r[129] = l[g]; }
     }
     __syncthreads();
-    finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
+    finish_head<float>(p, red, 2 * WARPS, head, split, s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -577,13 +577,12 @@ __global__ void __launch_bounds__(128, STAGES == 1 ? 4 : 3) prefix_own_kernel(co
     merge_head<__nv_bfloat16>(p, head, parts, slot0, red, WARPS * STAGES * 8192 / (PART_LD * 4));
 }
 
-template <typename T>
 static int launch_prefix_simple(const PrefixParams &p, cudaStream_t st) {
     const dim3 grid(p.splits, p.batch * p.h_kv);
-    if (p.G <= 1) attend_prefix_simple_kernel<T, 1><<<grid, 128, 0, st>>>(p);
-    else if (p.G <= 2) attend_prefix_simple_kernel<T, 2><<<grid, 128, 0, st>>>(p);
-    else if (p.G <= 4) attend_prefix_simple_kernel<T, 4><<<grid, 128, 0, st>>>(p);
-    else attend_prefix_simple_kernel<T, 8><<<grid, 128, 0, st>>>(p);
+    if (p.G <= 1) attend_prefix_simple_kernel<1><<<grid, 128, 0, st>>>(p);
+    else if (p.G <= 2) attend_prefix_simple_kernel<2><<<grid, 128, 0, st>>>(p);
+    else if (p.G <= 4) attend_prefix_simple_kernel<4><<<grid, 128, 0, st>>>(p);
+    else attend_prefix_simple_kernel<8><<<grid, 128, 0, st>>>(p);
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -751,6 +750,6 @@ extern "C" int skv_attend_prefix(const skv_prefix *c, const void *q, const int32
     p.part = static_cast<float *>(workspace);
     p.ticket = reinterpret_cast<int32_t *>(p.part + (int64_t)c->batch * c->h_kv * splits * c->G * PART_LD);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (c->dtype == SKV_F32) return launch_prefix_simple<float>(p, st);
+    if (c->dtype == SKV_F32) return launch_prefix_simple(p, st);
     return launch_prefix_mma(p, st);
 }

@@ -48,7 +48,7 @@ struct AttendQuantParams {
 // A key without a number (NaN scale) leaves its head without one, as the definition has it.
 __device__ __forceinline__ float quotient(const AttendQuantParams &, float num, float den) { return den == 0.f ? 0.f : num / den; }
 
-template <typename T, int BITS, int GP>
+template <int BITS, int GP>
 __global__ void __launch_bounds__(128) attend_quant_simple_kernel(const AttendQuantParams p) {
     using Q = Quant<BITS>;
     constexpr int WARPS = 4;
@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(128) attend_quant_simple_kernel(const AttendQu
     const int t0 = min((split * WARPS + warp) * per, tiles), t1 = min(t0 + per, tiles);
     const int sub = lane & 15, half = lane >> 4;
     const unsigned hmask = half ? 0xffff0000u : 0x0000ffffu;
-    const T *q = static_cast<const T *>(p.q) + (int64_t)head * G * HEAD_DIM;
+    const float *q = static_cast<const float *>(p.q) + (int64_t)head * G * HEAD_DIM;
 
     float qr[GP][8], acc[GP][8], m[GP], l[GP];
 #pragma unroll
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(128) attend_quant_simple_kernel(const AttendQu
         if (sub == 0) { r[128] = m[g]; r[129] = l[g]; }
     }
     __syncthreads();
-    finish_head<T>(p, red, 2 * WARPS, head, split, s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
+    finish_head<float>(p, red, 2 * WARPS, head, split, s_eff, (int64_t)head * p.splits, &s_flag, red, 2 * WARPS * GP);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -801,13 +801,13 @@ static int launch_quant_mma(const AttendQuantParams &p, cudaStream_t st) {
     return SKV_OK;
 }
 
-template <typename T, int BITS>
+template <int BITS>
 static int launch_quant_simple(const AttendQuantParams &p, cudaStream_t st) {
     const dim3 grid(p.splits, p.heads);
-    if (p.G <= 1) attend_quant_simple_kernel<T, BITS, 1><<<grid, 128, 0, st>>>(p);
-    else if (p.G <= 2) attend_quant_simple_kernel<T, BITS, 2><<<grid, 128, 0, st>>>(p);
-    else if (p.G <= 4) attend_quant_simple_kernel<T, BITS, 4><<<grid, 128, 0, st>>>(p);
-    else attend_quant_simple_kernel<T, BITS, 8><<<grid, 128, 0, st>>>(p);
+    if (p.G <= 1) attend_quant_simple_kernel<BITS, 1><<<grid, 128, 0, st>>>(p);
+    else if (p.G <= 2) attend_quant_simple_kernel<BITS, 2><<<grid, 128, 0, st>>>(p);
+    else if (p.G <= 4) attend_quant_simple_kernel<BITS, 4><<<grid, 128, 0, st>>>(p);
+    else attend_quant_simple_kernel<BITS, 8><<<grid, 128, 0, st>>>(p);
     SKV_CUDA_OK(cudaGetLastError());
     return SKV_OK;
 }
@@ -844,6 +844,6 @@ extern "C" int skv_attend_quant(const skv_qcache *c, const void *q, int dtype, i
     p.ticket = reinterpret_cast<int32_t *>(p.part + ((int64_t)ctas + p.heads) * G * PART_LD);
     p.scale_log2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == SKV_F32) return c->bits == 8 ? launch_quant_simple<float, 8>(p, st) : launch_quant_simple<float, 4>(p, st);
+    if (dtype == SKV_F32) return c->bits == 8 ? launch_quant_simple<8>(p, st) : launch_quant_simple<4>(p, st);
     return c->bits == 8 ? launch_quant_mma<8, 2, 2>(p, st) : launch_quant_mma<4, 2, 3>(p, st);
 }

@@ -24,15 +24,16 @@ struct RowsParams {
 
 constexpr int AT_ONCE = 2;       // positions of a half warp in a chunk
 
-// Position of token `t` of sequence `b`; -1 (recorded in the head's status) when it lies outside the cache.
-__device__ __forceinline__ int64_t row_position(const RowsParams &p, int b, int head, int t) {
+// Cache row of a call's first token of sequence `b` (-1 - capacity: none of its rows lies in the cache).
+__device__ __forceinline__ int64_t first_row(const RowsParams &p, int b) {
     const int64_t first = p.pos ? p.pos[p.pos_per_seq ? b : 0] : p.pos0;
-    const int64_t at = first + t;
-    if (first < 0 || first > p.capacity || at >= p.capacity) {
-        if (p.status) atomicOr(p.status + head, SKV_ST_BAD_INDEX);
-        return -1;
-    }
-    return at;
+    return first < 0 || first > p.capacity ? -1 - (int64_t)p.capacity : first;
+}
+// The row as an index; -1 (recorded in the head's status) where it lies outside the cache.
+__device__ __forceinline__ int cache_row(const RowsParams &p, int head, int64_t at) {
+    if (at >= 0 && at < p.capacity) return (int)at;
+    if (p.status) atomicOr(p.status + head, SKV_ST_BAD_INDEX);
+    return -1;
 }
 
 // The positions of a half warp.  A chunk: 3-d grid (positions, KV heads, sequences), N positions 16 apart, so that only the
@@ -41,7 +42,7 @@ template <bool FLAT>
 struct Places {
     static constexpr int N = FLAT ? 1 : AT_ONCE;
     int b, h, t, head, count;    // first token; positions there are
-    int64_t first;               // cache row of token 0 (-1 - capacity: none of them lies in the cache)
+    int64_t first;               // cache row of token 0
     __device__ __forceinline__ explicit Places(const RowsParams &p) {
         const int half = threadIdx.x >> 4;
         if (FLAT) {
@@ -59,16 +60,10 @@ struct Places {
             count = t < p.tokens ? min(N, (p.tokens - t + 15) >> 4) : 0;
         }
         if (!count) b = h = head = t = 0;
-        first = p.pos ? p.pos[p.pos_per_seq ? b : 0] : p.pos0;
-        if (first < 0 || first > p.capacity) first = -1 - (int64_t)p.capacity;
+        first = first_row(p, b);
     }
-    // cache row of the r-th position; -1 (recorded in the head's status) where it lies outside
-    __device__ __forceinline__ int row(const RowsParams &p, int r) const {
-        const int64_t at = first + t + 16 * r;
-        if (at >= 0 && at < p.capacity) return (int)at;
-        if (p.status) atomicOr(p.status + head, SKV_ST_BAD_INDEX);
-        return -1;
-    }
+    // cache row of the r-th position
+    __device__ __forceinline__ int row(const RowsParams &p, int r) const { return cache_row(p, head, first + t + 16 * r); }
 };
 
 // A lane's eight values of a key or value row.
@@ -292,7 +287,7 @@ __global__ void __launch_bounds__(128) qk_rope_quant_kernel(const __nv_bfloat16 
     if (item >= p.batch * per) return;
     const int b = item / per, j = item % per;
     const int head = b * p.h_kv + (j < H ? j / (H / p.h_kv) : (j - H) % p.h_kv);
-    const int64_t pos = row_position(p, b, head, 0);
+    const int64_t pos = cache_row(p, head, first_row(p, b));
     if (pos < 0) return;                                              // recorded; the tables have `capacity` rows at least
     const __nv_bfloat16 *src = qkv + ((int64_t)b * per + j) * HEAD_DIM;
     float4 r;

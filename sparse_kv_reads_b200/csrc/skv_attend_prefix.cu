@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
 // from tensor memory, so that no maximum needs a shuffle, and writes the weights back over them in bf16 as the A operand of
 // the second product (which takes A and B of one type, and the values are bf16; half floats would not hold them all, and a
 // product with the weights' remainders as well would add a half to those that bound the wide case.  The sum of the weights
-// is taken before they are rounded, in float32).  One thread feeds the ring of K and V tiles by TMA (rows beyond the prefix read as zeros), one issues
+// is taken before they are rounded, in float32).  One thread feeds the ring of K and V tiles by TMA (rows beyond the prefix read
+// as zeros), one issues
 //   S = Q K^T  (both K-major in shared memory)        O += P V  (P in tensor memory, V MN-major)
 // with the two slots strictly in turn, so that one's products run beside the other's softmax.  Accumulators are rescaled only
 // when a row's maximum rises by more than 8 (base 2).
@@ -125,8 +126,8 @@ __global__ void __launch_bounds__(128) attend_prefix_simple_kernel(const PrefixP
 // the scores (both operands from shared memory, beside the incoming tiles) and 500 of waits and commits between them, 3,430
 // cycles a tile where the tensor cores alone need 2,048; a slot's weights lie ready 360 cycles before their turn comes (its
 // softmax takes 1,650: loads 115, maximum 280, exponentials 1,230; taken with scale and difference in one fused operation).
-// Measured and not kept (128 sequences x 4 query heads x 16,383 keys, 53.5 us with the second launch, as it then was): scores and weights by
-// halves of a tile (71.6 us: with 64 keys on N the queries are read from shared memory twice as often), an issuing thread per
+// Measured and not kept (128 sequences x 4 query heads x 16,383 keys, 53.5 us with the second launch, as it then was): scores and
+// weights by halves of a tile (71.6 us: with 64 keys on N the queries are read from shared memory twice as often), an issuing thread per
 // slot (62.4 us: the slots fall into step), weights released by halves (54.9 us).  Within 1 us of it, either way, since the
 // softmax does not bound it: half the weights against the standing reference while the maximum is found, products issued by
 // a converged warp, barriers looked at ahead of their turn (this one 2.5 us slower for 32 sequences x 32,768 keys); 1 to 5 us
@@ -213,7 +214,10 @@ prefix_mma_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kmap
         }
         // Only behind the wait: an allocation blocks without a limit, so a launch that has started early must not hold the
         // columns that a launch ahead of it has still to ask for.
-        if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
+        if (warp == 9) {
+            __syncwarp();                                 // (its lanes may have parted at the last row)
+            tmem_alloc(smem_u32(&s_tmem), 512);
+        }
 #pragma unroll
         for (int e = 0; e < CHUNKS; ++e) {
             const int i = tid + e * P_THREADS, r = i >> 4, c = i & 15, rr = r & (PT - 1);

@@ -29,3 +29,10 @@ def test_sums_of_the_other_slot_are_read_behind_a_fence_behind_the_barrier():
     steps = [tail.index(x) for x in ("tcgen05_before_sync();", "bar.sync 1, 256;")]
     fence = tail.find("tcgen05_after_sync();", steps[1])
     assert steps[0] < steps[1] < fence < tail.index("tmem_ld32(")
+
+
+def test_a_warp_allocates_tensor_memory_together():
+    """The allocation is an instruction of a whole warp, whose lanes the loads of the last rows ahead of it may have parted."""
+    body = kernel_body("skv_attend_prefix.cu", "prefix_mma_kernel")
+    ahead = body[:body.index("tmem_alloc(")]
+    assert ahead.rstrip().endswith("__syncwarp();")

@@ -216,10 +216,10 @@ struct WarpAttendQuant {
         // [2^127, 2^128) becomes one in [2, 4)
         int e = (int)(__float_as_uint(top) >> 23) - 127;
         if (!(top > 0.f) || e > 127) e = 0;
-        e = min(max(e, -120), 126);
+        e = min(max(e, -126), 126);
         // The sums of codes (up to 2^15) meet the key's scale (up to 2^121, 2^125 in 4 bits) before the query's power of two.  Queries
         // so small that the product could leave the numbers though the score does not are held 9 places lower: their half
-        // floats keep 2^-16 of the largest component (odd places of 4 bits: 2^-12).
+        // floats keep 2^-16 of the largest component (odd places of 4 bits: 2^-12), and numbers below 2^-126 whole.
         if (e < -20) e += 9;
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
         float sum[GR];

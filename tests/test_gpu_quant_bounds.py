@@ -156,3 +156,13 @@ def test_value_groups_of_very_different_sizes(apart, n):
     codes = (kc, ks, vc, vs)
     q = (torch.randn(H * G, 128, generator=g) * 2).to(torch.bfloat16)
     assert outside(run_alone(q, codes, 4), q, codes, [n], 4) == []
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("size", [2.0 ** -128, 2.0 ** -130])
+def test_queries_below_the_normal_numbers(bits, size):
+    """Every bf16 number down to 2^-133 counts, with keys so large that the scores are ordinary."""
+    H, G, n = 2, 3, 300
+    codes = (random_codes(H, n, bits, 3), scales(H, n, bits, 2.0 ** (122 if bits == 8 else 127)), *quantise(normal_rows(1, H, n, 4), bits))
+    q = (torch.randn(H * G, 128, generator=torch.Generator().manual_seed(5)) * size).to(torch.bfloat16)
+    assert outside(run_alone(q, codes, bits), q, codes, [n], bits) == []

@@ -420,3 +420,27 @@ def test_a_decoder_over_a_shared_prefix_reports_a_length_beyond_its_rows():
         q = torch.zeros(B * dec.H, 128, dtype=torch.bfloat16, device=DEV)
         dec.attn[0](q, *cache.prefix_rows(0), kh, vh, torch.tensor([7], dtype=torch.int32, device=DEV))
     assert dec.check_status() == 4
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,Hk,G,P,n", [(2, 2, 2, 333, 17), (4, 8, 2, 5000, 100), (40, 4, 2, 5003, 40), (70, 8, 4, 4097, 9),
+                                        (9, 1, 8, 20000, 700), (130, 1, 2, 900, 1)])
+def test_every_tile_and_partial_counts(dtype, B, Hk, G, P, n):
+    """Values that are one in a component of their own for each 1/128 of the rows, weights all alike: an output component is
+    the share of its rows, so that one that is lost or counted twice shows."""
+    total = P + n
+    g = torch.Generator().manual_seed(total)
+    q = (torch.randn(B * Hk * G, 128, generator=g) * 0.05).to(dtype)
+    kp, k = torch.randn(Hk, P, 128, generator=g).to(dtype), torch.randn(B * Hk, n, 128, generator=g).to(dtype)
+    where = torch.arange(total) * 128 // total
+    one = torch.eye(128)[where].to(dtype)
+    vp, v = one[:P].expand(Hk, -1, -1).contiguous(), one[P:].expand(B * Hk, -1, -1).contiguous()
+    got = run_plain(q, kp, vp, k, v, B, Hk, G, dtype).cpu().double().view(B, Hk, G, 128)
+    qq = q.double().view(B, Hk, G, 128)
+    zp = torch.einsum("bhgd,hpd->bhgp", qq, kp.double())
+    zo = torch.einsum("bhgd,bhnd->bhgn", qq, k.double().view(B, Hk, n, 128))
+    w = torch.softmax(torch.cat((zp, zo), -1) * SCALE, -1)
+    ref = torch.zeros(B, Hk, G, 128, dtype=torch.float64).index_add_(3, where, w)
+    # scores well below one: their own error is nothing beside the weights' rounding
+    assert bool(((got - ref).abs() <= output_bound(ref, ref, dtype, 2.0 ** -18)).all())
+    assert 16 * 128 / total > 4 * 3 * 2.0 ** -8            # (16 rows of a component are far outside the bound)

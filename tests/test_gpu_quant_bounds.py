@@ -166,3 +166,25 @@ def test_queries_below_the_normal_numbers(bits, size):
     codes = (random_codes(H, n, bits, 3), scales(H, n, bits, 2.0 ** (122 if bits == 8 else 127)), *quantise(normal_rows(1, H, n, 4), bits))
     q = (torch.randn(H * G, 128, generator=torch.Generator().manual_seed(5)) * size).to(torch.bfloat16)
     assert outside(run_alone(q, codes, bits), q, codes, [n], bits) == []
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("H,G,lens,ctas", [(8, 2, [300], None), (8, 2, [20000], None), (4, 4, [3000, 17, 0, 9000, 128], None),
+                                           (2, 8, [37 * b % 301 + 1 for b in range(80)], None), (1, 1, [6000, 1, 500], 7)])
+def test_every_tile_and_partial_counts(bits, H, G, lens, ctas):
+    """Values that are one in a component of their own for each 1/128 of the rows, weights all alike: an output component is
+    the share of its rows, so that one that is lost or counted twice shows."""
+    B, L = len(lens), max(lens)
+    g = torch.Generator().manual_seed(L)
+    v = torch.zeros(B, H, L, 128)
+    for b, n in enumerate(lens):
+        v[b, :, :n] = torch.eye(128)[torch.arange(n) * 128 // max(n, 1)]
+    codes = (*quantise(torch.randn(B, H, L, 128, generator=g), bits), *quantise(v, bits))
+    q = (torch.randn(B * H * G, 128, generator=g) * 0.05).to(torch.bfloat16)
+    attn = QuantAttentionGraph(H=B * H * G, H_kv=B * H, d=128, dtype=torch.bfloat16, device=DEV)
+    attn.n_group = H
+    if ctas is not None:
+        attn.ctas = ctas
+        attn.ws = torch.zeros(lib().skv_quant_workspace_bytes(B * H, G, 128, ctas), dtype=torch.uint8, device=DEV)
+    out = attn(q.to(DEV), device_cache(codes, bits, lens), 0, torch.tensor(lens, dtype=torch.int32, device=DEV))
+    assert outside(out, q, codes, lens, bits) == []

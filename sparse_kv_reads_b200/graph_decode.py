@@ -102,6 +102,7 @@ class GraphDecoder:
             raise ValueError("clustered attention reads a plain cache: decode this one with mode='dense'")
         self.model, self.cache, self.mode = model, cache, mode
         self.first = 0                                     # position of the cache's first row (a shared prefix: its length)
+        self._prefix = None                                # the prefix that prepare() saw
         self.H, self.H_kv, self.d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         self.B = B = cache.k[0].shape[0]
         p = next(model.parameters())
@@ -208,9 +209,10 @@ class GraphDecoder:
 
     def _set_first(self) -> None:
         """Take over the position of the cache's first row.  A captured step has the shared prefix's length, its tensor
-        maps and the offset into the rotary tables in it: one captured for another length is given up."""
-        self.first = getattr(self.cache, "first", 0)
-        if self.graph is not None and self._captured != (self.first, self.ragged):
+        maps and the offset into the rotary tables in it: one captured for another prefix or length is given up."""
+        self.first, before = getattr(self.cache, "first", 0), self._prefix
+        self._prefix = getattr(self.cache, "prefix", None)
+        if self.graph is not None and (self._captured != (self.first, self.ragged) or self._prefix is not before):
             self.graph = None
 
     def _insert_for_first_step(self, n: int | None) -> None:
@@ -587,7 +589,7 @@ class GraphDecoder:
             return
         if torch.is_tensor(pos) and pos.is_cuda:
             raise ValueError("positions in a quantised or shared-prefix cache are given on the host, where they are checked")
-        if self.first != self.cache.first:
+        if self.first != self.cache.first or (self._prefix is not getattr(self.cache, "prefix", None) and self.first):
             raise ValueError("the shared prefix has changed since prepare()")
         try:
             at = [index(pos)]

@@ -487,3 +487,19 @@ def test_the_tensors_of_a_quantised_cache_stay_its_own(L):
     for name in ("k", "v", "scale", "status"):
         with pytest.raises(AttributeError):
             setattr(c, name, getattr(c, name))
+
+
+def test_another_prefix_in_a_caches_place_is_noticed():
+    """A prefix cache exchanged for another of the same length: a step is refused, prepare() drops what was captured."""
+    m = Qwen3Model(Qwen3Config(**TINY)).eval()
+    cache = m.alloc_prefix_cache(8, 4, 2)
+    cache.prefix.cur_len = 6
+    dec = GraphDecoder(m, cache, mode="dense")
+    dec.prepare(6)
+    dec.graph, dec._captured = Replayed(), (6, False)
+    cache.prefix = m.alloc_cache(8)
+    cache.prefix.cur_len = 6
+    with pytest.raises(ValueError, match="prefix has changed"):
+        dec.step(torch.zeros(2, 1, dtype=torch.long), 6)
+    dec.prepare(6)
+    assert dec.graph is None
